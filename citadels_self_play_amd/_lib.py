@@ -14,7 +14,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "citadels.h")
 
 _lib = None
 
-vp, i32, i64, u64 = C.c_void_p, C.c_int, C.c_int64, C.c_uint64
+vp, i32, i64, u64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float
 
 _SIGS = {
     "cit_abi_version": ([], i32),
@@ -71,6 +71,17 @@ _SIGS = {
                             vp, vp, vp], i32),
     "cit_cfr_pred_fused": ([vp, vp, vp, vp, vp, vp, i32, i32, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp, vp,
                             vp], i32),
+    "cit_linear_forward_work_bytes": ([i32, i32, i32, i32], u64),
+    "cit_linear_forward": ([vp, i64, vp, i64, vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, vp, u64, vp], i32),
+    "cit_linear_backward_work_bytes": ([i32, i32, i32, i32, i32], u64),
+    "cit_linear_backward": ([vp, i64, vp, vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, vp, u64, vp], i32),
+    "cit_policy_loss_work_bytes": ([i64], u64),
+    "cit_policy_loss": ([vp, i64, vp, i64, vp, i64, vp, i64, i64, i32, vp, vp, vp, vp, f32, f32, f32, i32, vp, vp, vp,
+                         vp, vp, u64, vp], i32),
+    "cit_policy_loss_backward": ([vp, i64, vp, i64, vp, i64, vp, i64, i64, i32, vp, vp, vp, vp, f32, f32, f32, i32,
+                                  vp, i32, vp, vp], i32),
+    "cit_clip_grad_norm_work_bytes": ([i32], u64),
+    "cit_clip_grad_norm": ([vp, vp, vp, vp, vp, i32, C.c_double, vp, vp, u64, vp], i32),
 }
 
 

@@ -1,0 +1,518 @@
+// The linear layer y = act(x W^T + b) + r (models.py's fc1..fc4 at any size and
+// type), its gradients and its form for a few rows.
+//
+//   z = x W^T + b,  y = act(z) + r             act: none, relu, gelu (erf), silu
+//   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz
+//
+// One tile kernel serves the three products: each operand is either "kc" (the
+// reduction index runs along memory: x and W of the forward pass, dz of dx) or
+// "ks" (it runs down the rows: W of dx, both of dW); the ks operands of 16-bit
+// types are transposed on their way out of LDS (ds_read_tr16_b64), so no
+// transposed copy is ever written.  Sums are fp32 in the matrix cores'
+// accumulators from the first product to the epilogue; the one rounding to the
+// element type is the store.
+#include "cit_ops.h"
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 fp16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((__vector_size__(8)));
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
+
+__device__ __forceinline__ float act_fwd(int act, float z) {
+  if (act == ACT_RELU) return z < 0.0f ? 0.0f : z;                  // NaN stays
+  if (act == ACT_GELU) return 0.5f * z * erfcf(-z * 0.70710678118654752f);   // erfc: no cancellation at z < 0
+  if (act == ACT_SILU) return z / (1.0f + expf(-z));
+  return z;
+}
+__device__ __forceinline__ float act_grad(int act, float z) {
+  if (act == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if (act == ACT_GELU)
+    return 0.5f * erfcf(-z * 0.70710678118654752f) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+  if (act == ACT_SILU) {
+    const float s = 1.0f / (1.0f + expf(-z));
+    return s * (1.0f + z * (1.0f - s));
+  }
+  return 1.0f;
+}
+
+// z kept for the backward pass in the element type.  The rounding is to
+// nearest, except that a finite z stays finite and a nonzero one nonzero: relu
+// asks for its sign (fp16 underflows below 2^-25), and gelu's z * exp(-z^2 / 2)
+// is inf * 0 at an infinity that only the rounding made.
+template <typename T> __device__ __forceinline__ T keep_z(float z) { return from_f<T>(z); }
+template <> __device__ __forceinline__ fp16_t keep_z<fp16_t>(float z) {
+  const float a = fabsf(z);
+  if (a > 65504.0f && a <= 3.4028234663852886e38f) return (fp16_t)copysignf(65504.0f, z);
+  if (a < 5.9604644775390625e-08f && a > 0.0f) return (fp16_t)copysignf(5.9604644775390625e-08f, z);
+  return (fp16_t)z;
+}
+template <> __device__ __forceinline__ bf16_t keep_z<bf16_t>(float z) {
+  if (fabsf(z) > 3.3895313892515355e38f && fabsf(z) <= 3.4028234663852886e38f)
+    return (bf16_t)copysignf(3.3895313892515355e38f, z);
+  return (bf16_t)z;
+}
+
+struct Epilogue {               // what follows a product's sum at row m, column n
+  const void* bias;             // [N] or null
+  const void* res;              // [M][ldr] or null
+  void* out;                    // [M][ldo]
+  void* z;                      // [M][N] pre-activation for the backward pass, or null
+  float* part;                  // split sums: [split][M][N] fp32 instead of out
+  int64_t ldr, ldo;
+  int act;
+};
+
+template <typename T>
+__device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int n, int N, float v) {
+  if (e.bias) v += to_f(static_cast<const T*>(e.bias)[n]);
+  if (e.z) static_cast<T*>(e.z)[m * N + n] = keep_z<T>(v);
+  v = act_fwd(e.act, v);
+  if (e.res) v += to_f(static_cast<const T*>(e.res)[m * e.ldr + n]);
+  static_cast<T*>(e.out)[m * e.ldo + n] = from_f<T>(v);
+}
+
+struct __attribute__((packed, aligned(2))) any_f4 { float v[4]; };
+
+// Four neighbouring columns of one row (count of them inside N).
+template <typename T>
+__device__ __forceinline__ void finish4(const Epilogue& e, int64_t m, int n, int N, f32x4 v, int split, int64_t M) {
+  if (e.part) {
+    float* p = e.part + ((int64_t)split * M + m) * N + n;
+    if (n + 4 <= N) {
+      any_f4 o;
+      for (int i = 0; i < 4; i++) o.v[i] = v[i];
+      *reinterpret_cast<any_f4*>(p) = o;
+    } else {
+      for (int i = 0; n + i < N; i++) p[i] = v[i];
+    }
+    return;
+  }
+  struct __attribute__((packed, aligned(2))) row4 { T v[4]; };
+  if (n + 4 > N) {
+    for (int i = 0; n + i < N; i++) finish<T>(e, m, n + i, N, v[i]);
+    return;
+  }
+  if (e.bias) {
+    const row4 b = *reinterpret_cast<const row4*>(static_cast<const T*>(e.bias) + n);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] += to_f((T)b.v[i]);
+  }
+  if (e.z) {
+    row4 z;
+#pragma unroll
+    for (int i = 0; i < 4; i++) z.v[i] = keep_z<T>(v[i]);
+    *reinterpret_cast<row4*>(static_cast<T*>(e.z) + m * N + n) = z;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = act_fwd(e.act, v[i]);
+  if (e.res) {
+    const row4 r = *reinterpret_cast<const row4*>(static_cast<const T*>(e.res) + m * e.ldr + n);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] += to_f((T)r.v[i]);
+  }
+  row4 o;
+#pragma unroll
+  for (int i = 0; i < 4; i++) o.v[i] = from_f<T>(v[i]);
+  *reinterpret_cast<row4*>(static_cast<T*>(e.out) + m * e.ldo + n) = o;
+}
+
+// ---- operand tiles ------------------------------------------------------------
+//
+// A tile holds R rows (of the output's m or n) by 128 bytes of the reduction:
+// BK = 64 16-bit or 32 32-bit elements.  kc tiles lie as [R][128 B], ks tiles as
+// [BK][R elements]; both are R * 128 bytes in chunks of 16, and a row's chunks
+// are permuted (xor) so that the lanes of one LDS read, which walk down rows
+// or along k, meet different banks.
+
+template <typename T> constexpr int BK = 128 / (int)sizeof(T);
+
+template <typename T, bool KS, int R>
+struct Tile {
+  static constexpr int E = 16 / sizeof(T);            // elements of a chunk
+  static constexpr int CPR = KS ? R / E : 8;          // chunks of a tile row
+  static constexpr int CHUNKS = R * 8;
+
+  __device__ static __forceinline__ int swz(int row) {
+    if (!KS) return row & 7;
+    return sizeof(T) == 2 ? (row & 3) << 1 : ((row >> 2) & 3) << 2;
+  }
+  // Byte offset of the 16-byte chunk c of tile row `row`.
+  __device__ static __forceinline__ int at(int row, int c) { return (row * CPR + (c ^ swz(row))) << 4; }
+
+  // Global chunk behind LDS chunk `id`: (tile row, chunk of the row).
+  __device__ static __forceinline__ void from(int id, int& row, int& c) {
+    row = id / CPR;
+    c = (id % CPR) ^ swz(row);
+  }
+};
+
+// A matrix of `rows` x `cols` elements, ld elements apart.
+struct Mat {
+  const void* p;
+  int64_t ld;
+  int rows, cols;
+};
+
+// 16 bytes of row r from column c on, zero outside the matrix: any alignment.
+template <typename T>
+__device__ __forceinline__ u32x4 fetch(const Mat& a, int r, int c) {
+  constexpr int E = 16 / sizeof(T);
+  Pack16<T> v;
+  v.raw = u32x4{0, 0, 0, 0};
+  if (r < a.rows && c < a.cols) {
+    const T* p = static_cast<const T*>(a.p) + (int64_t)r * a.ld + c;
+    if (c + E <= a.cols) {
+      v.raw = load16(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i++)
+        if (c + i < a.cols) v.e[i] = p[i];
+    }
+  }
+  return v.raw;
+}
+
+// Loads of one thread for one tile, through registers (THREADS threads).
+template <typename T, bool KS, int R, int THREADS>
+struct Stage {
+  typedef Tile<T, KS, R> L;
+  static constexpr int PER = L::CHUNKS / THREADS;
+  u32x4 v[PER];
+  __device__ __forceinline__ void load(const Mat& a, int r0, int k0) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      int row, c;
+      L::from(i * THREADS + (int)threadIdx.x, row, c);
+      v[i] = KS ? fetch<T>(a, k0 + row, r0 + c * L::E) : fetch<T>(a, r0 + row, k0 + c * L::E);
+    }
+  }
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+      *reinterpret_cast<u32x4*>(lds + ((i * THREADS + (int)threadIdx.x) << 4)) = v[i];
+  }
+};
+
+// ---- matrix instructions --------------------------------------------------------
+
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, bf16_t) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                 0);
+}
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, fp16_t) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fp16x8, a), __builtin_bit_cast(fp16x8, b), c, 0, 0,
+                                                0);
+}
+// Four k of each lane: the k a lane group holds differ from the instruction's
+// own order, but A and B hold the same ones, and a sum has no order.
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, float) {
+  const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+  for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
+  return c;
+}
+
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+// The 16 rows from `r0` on of a tile, k step s (32 16-bit or 16 32-bit
+// elements): lane l holds row r0 + l % 16 and its quarter l / 16 of the k.
+template <typename T, bool KS, int R>
+__device__ __forceinline__ u32x4 frag(const char* lds, int r0, int s) {
+  typedef Tile<T, KS, R> L;
+  const int l = threadIdx.x & 63, g = l >> 4, i = l & 15;
+  if (!KS) return *reinterpret_cast<const u32x4*>(lds + L::at(r0 + i, s * 4 + g));
+  if (sizeof(T) == 2) {
+    // Two transposing reads of 4 k x 16 rows: lane i of a group reads 4 elements
+    // of k row i / 4 and receives the 4 k of row i.
+    union { u32x4 raw; s16x4 h[2]; } v;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int k = s * 32 + g * 8 + h * 4 + (i >> 2);
+      const int off = L::at(k, (r0 >> 3) + ((i & 3) >> 1)) + ((i & 1) << 3);
+      v.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(lds + off));
+    }
+    return v.raw;
+  }
+  union { u32x4 raw; float f[4]; } v;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int k = s * 16 + g * 4 + j, c = r0 + i;
+    v.f[j] = *reinterpret_cast<const float*>(lds + L::at(k, c >> 2) + ((c & 3) << 2));
+  }
+  return v.raw;
+}
+
+// ---- the tile kernel ------------------------------------------------------------
+//
+// Workgroup (tile, split): BM x BN outputs by WM x WN waves, over the split's
+// share of the reduction.  Two LDS buffers: while the matrix cores work on one
+// tile, the next one's loads are in flight.
+
+template <typename T, bool AKS, bool BKS, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, int M, int N, int K, int tiles_n,
+                                                      int k_per_split) {
+  constexpr int THREADS = WM * WN * 64;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int STEPS = 2;                              // k steps of a tile: 64 bytes of each row
+  __shared__ __attribute__((aligned(16))) char lds[2][(BM + BN) * 128];
+
+  const int tile = blockIdx.x, split = blockIdx.y;
+  const int m0 = (tile / tiles_n) * BM, n0 = (tile % tiles_n) * BN;
+  const int kb = split * k_per_split, ke = min(K, kb + k_per_split);
+  Mat a = A, b = B;                                     // the split's share of the reduction
+  if (AKS) a.rows = ke; else a.cols = ke;
+  if (BKS) b.rows = ke; else b.cols = ke;
+
+  const int w = threadIdx.x >> 6;
+  const int wm = (w / WN) * (BM / WM), wn = (w % WN) * (BN / WN);
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  Stage<T, AKS, BM, THREADS> sa;
+  Stage<T, BKS, BN, THREADS> sb;
+  sa.load(a, m0, kb);
+  sb.load(b, n0, kb);
+  sa.store(lds[0]);
+  sb.store(lds[0] + BM * 128);
+  __syncthreads();
+  int cur = 0;
+  for (int k = kb; k < ke; k += BK<T>) {
+    const bool more = k + BK<T> < ke;
+    if (more) {
+      sa.load(a, m0, k + BK<T>);
+      sb.load(b, n0, k + BK<T>);
+    }
+    const char* la = lds[cur];
+    const char* lb = lds[cur] + BM * 128;
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) {
+      u32x4 fa[TM], fb[TN];
+#pragma unroll
+      for (int i = 0; i < TM; i++) fa[i] = frag<T, AKS, BM>(la, wm + i * 16, s);
+#pragma unroll
+      for (int j = 0; j < TN; j++) fb[j] = frag<T, BKS, BN>(lb, wn + j * 16, s);
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = mma(fb[j], fa[i], acc[i][j], T{});
+    }
+    if (more) {
+      sa.store(lds[cur ^ 1]);
+      sb.store(lds[cur ^ 1] + BM * 128);
+    }
+    __syncthreads();
+    cur ^= 1;
+  }
+
+  // B went in as the instruction's rows, so a lane holds 4 neighbouring n of one m.
+  const int l = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < TM; i++) {
+    const int m = m0 + wm + i * 16 + (l & 15);
+#pragma unroll
+    for (int j = 0; j < TN; j++) {
+      const int n = n0 + wn + j * 16 + (l >> 4) * 4;
+      if (m < M && n < N) finish4<T>(e, m, n, N, acc[i][j], split, M);
+    }
+  }
+}
+
+// The splits' sums in their order, then the epilogue.
+template <typename T>
+__global__ __launch_bounds__(256) void k_join(Epilogue e, int64_t M, int N, int splits) {
+  const int64_t count = M * N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    float v = 0.0f;
+    for (int s = 0; s < splits; s++) v += e.part[s * count + i];
+    const int64_t m = i / N;
+    finish<T>(e, m, (int)(i - m * N), N, v);
+  }
+}
+
+// ---- dz and db --------------------------------------------------------------------
+//
+// Block (column block, row share): 64 columns of the share's rows, 4 waves down
+// the rows.  dz = dy act'(z) rounded once to the element type (the matrix
+// cores' input), its column sums taken before that rounding.
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_dz(const T* dy, int64_t ldy, const T* z, T* dz, float* db, int M, int N,
+                                            int act, int rows_per) {
+  __shared__ float sums[4][64];
+  const int n = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  const int mb = blockIdx.y * rows_per, me = min(M, mb + rows_per);
+  float s = 0.0f;
+  if (n < N)
+    for (int m = mb + w; m < me; m += 4) {
+      float v = to_f(dy[(int64_t)m * ldy + n]);
+      if (act != ACT_NONE) v *= act_grad(act, to_f(z[(int64_t)m * N + n]));
+      s += v;
+      if (dz) dz[(int64_t)m * N + n] = from_f<T>(v);
+    }
+  if (!db) return;
+  sums[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w == 0 && n < N)
+    db[(int64_t)blockIdx.y * N + n] =
+        (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_db(const float* part, T* db, int N, int shares) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  float s = 0.0f;
+  for (int i = 0; i < shares; i++) s += part[(int64_t)i * N + n];
+  db[n] = from_f<T>(s);
+}
+
+// ---- host side ---------------------------------------------------------------------
+
+int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+struct Plan {
+  int tiles_m, tiles_n, splits, k_per;
+};
+
+Plan plan_tiles(int M, int N, int K, int bm, int bn, int bk) {
+  Plan p;
+  p.tiles_m = cdiv(M, bm);
+  p.tiles_n = cdiv(N, bn);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  // fewer tiles than half the compute units: the reduction is shared out too, in shares of at least 4 k tiles
+  int want = tiles < 128 ? (int)(256 / tiles) : 1;
+  const int kt = cdiv(K, bk);
+  want = want < kt / 4 ? want : kt / 4;
+  if (want < 1) want = 1;
+  p.k_per = cdiv(kt, want) * bk;
+  p.splits = K > 0 ? cdiv(K, p.k_per) : 1;
+  return p;
+}
+
+int elt(int dtype) { return dtype == CIT_FP32 ? 4 : 2; }
+
+int64_t product_work(int M, int N, int K, int dtype) {
+  if (M <= 0 || N <= 0) return 0;
+  const Plan p = plan_tiles(M, N, K, 64, 64, 128 / elt(dtype));
+  return p.splits > 1 ? align256((int64_t)p.splits * M * N * 4) : 0;
+}
+
+template <typename T, bool AKS, bool BKS>
+int product(Mat A, Mat B, Epilogue e, int M, int N, int K, void* work, hipStream_t stream) {
+  const Plan p = plan_tiles(M, N, K, 64, 64, BK<T>);
+  if (p.splits > 1) e.part = static_cast<float*>(work);
+  hipLaunchKernelGGL((k_gemm<T, AKS, BKS, 64, 64, 2, 2>), dim3(p.tiles_m * p.tiles_n, p.splits), dim3(256), 0, stream,
+                     A, B, e, M, N, K, p.tiles_n, p.k_per);
+  if (p.splits > 1)
+    hipLaunchKernelGGL((k_join<T>), dim3(cdiv((int64_t)M * N, 256) < 4096 ? cdiv((int64_t)M * N, 256) : 4096), dim3(256), 0, stream, e, (int64_t)M, N,
+                       p.splits);
+  return launch_status();
+}
+
+int dz_rows(int M, int N) {
+  const int columns = cdiv(N, 64);
+  int shares = cdiv(1024, columns);
+  const int most = cdiv(M, 64);
+  if (shares > most) shares = most;
+  if (shares > 256) shares = 256;
+  return cdiv(M, shares);
+}
+
+template <typename T>
+int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const Epilogue& e, int M, int N, int K, void* work,
+            hipStream_t stream) {
+  return product<T, false, false>(Mat{x, ldx, M, K}, Mat{w, ldw, N, K}, e, M, N, K, work, stream);
+}
+
+template <typename T>
+int backward(const void* dy, int64_t ldy, const void* z, const void* x, int64_t ldx, const void* w, int64_t ldw,
+             void* dx, void* dw, void* db, int M, int N, int K, int act, char* work, hipStream_t stream) {
+  const T* d = static_cast<const T*>(dy);
+  int64_t ldd = ldy;
+  const int rows = dz_rows(M, N), shares = cdiv(M, rows);
+  T* dz = nullptr;
+  float* sums = nullptr;
+  if (act != ACT_NONE && (dx || dw)) {
+    dz = reinterpret_cast<T*>(work);
+    work += align256((int64_t)M * N * sizeof(T));
+  }
+  if (db) {
+    sums = reinterpret_cast<float*>(work);
+    work += align256((int64_t)shares * N * 4);
+  }
+  if (dz || db) {
+    hipLaunchKernelGGL((k_dz<T>), dim3(cdiv(N, 64), shares), dim3(256), 0, stream, d, ldy, static_cast<const T*>(z), dz,
+                       sums, M, N, act, rows);
+    if (db)
+      hipLaunchKernelGGL((k_db<T>), dim3(cdiv(N, 256)), dim3(256), 0, stream, sums, static_cast<T*>(db), N, shares);
+  }
+  if (dz) d = dz, ldd = N;
+  int rc = 0;
+  if (dx && K > 0) {
+    Epilogue e = {};
+    e.out = dx;
+    e.ldo = K;
+    rc = product<T, false, true>(Mat{d, ldd, M, N}, Mat{w, ldw, N, K}, e, M, K, N, work, stream);
+  }
+  if (!rc && dw && K > 0) {
+    Epilogue e = {};
+    e.out = dw;
+    e.ldo = K;
+    rc = product<T, true, true>(Mat{d, ldd, M, N}, Mat{x, ldx, M, K}, e, N, K, M, work, stream);
+  }
+  return rc ? rc : launch_status();
+}
+
+bool bad_types(int dtype, int act) { return dtype < CIT_FP32 || dtype > CIT_FP16 || act < ACT_NONE || act > ACT_SILU; }
+
+}  // namespace
+
+extern "C" {
+
+size_t cit_linear_forward_work_bytes(int M, int N, int K, int dtype) {
+  return bad_types(dtype, 0) ? 0 : (size_t)product_work(M, N, K, dtype);
+}
+
+size_t cit_linear_backward_work_bytes(int M, int N, int K, int dtype, int act) {
+  if (bad_types(dtype, act) || M <= 0 || N <= 0 || K < 0) return 0;
+  const int64_t a = product_work(M, K, N, dtype), b = product_work(N, K, M, dtype);
+  const int64_t dz = act != ACT_NONE ? align256((int64_t)M * N * elt(dtype)) : 0;
+  return (size_t)(dz + align256((int64_t)cdiv(M, dz_rows(M, N)) * N * 4) + (a > b ? a : b));
+}
+
+int cit_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
+                       int64_t ldr, void* y, void* z, int M, int N, int K, int dtype, int act, void* work,
+                       size_t work_bytes, hipStream_t stream) {
+  if (M < 0 || N < 0 || K < 0 || bad_types(dtype, act)) return -1;
+  if (!M || !N) return 0;
+  if (!y || (K && (!x || !w || ldx < K || ldw < K)) || (residual && ldr < N)) return -1;
+  const size_t need = cit_linear_forward_work_bytes(M, N, K, dtype);
+  if (need && (!work || work_bytes < need)) return -1;
+  Epilogue e = {};
+  e.bias = bias, e.res = residual, e.out = y, e.z = z, e.ldr = ldr, e.ldo = N, e.act = act;
+  if (dtype == CIT_FP32) return forward<float>(x, ldx, w, ldw, e, M, N, K, work, stream);
+  if (dtype == CIT_BF16) return forward<bf16_t>(x, ldx, w, ldw, e, M, N, K, work, stream);
+  return forward<fp16_t>(x, ldx, w, ldw, e, M, N, K, work, stream);
+}
+
+int cit_linear_backward(const void* dy, int64_t ldy, const void* z, const void* x, int64_t ldx, const void* w,
+                        int64_t ldw, void* dx, void* dw, void* db, int M, int N, int K, int dtype, int act, void* work,
+                        size_t work_bytes, hipStream_t stream) {
+  if (M <= 0 || N <= 0 || K < 0 || bad_types(dtype, act)) return -1;
+  if (!dy || ldy < N || (act != ACT_NONE && !z) || (dx && (!w || ldw < K)) || (dw && (!x || ldx < K))) return -1;
+  const size_t need = cit_linear_backward_work_bytes(M, N, K, dtype, act);
+  if (need && (!work || work_bytes < need)) return -1;
+  char* p = static_cast<char*>(work);
+  if (dtype == CIT_FP32) return backward<float>(dy, ldy, z, x, ldx, w, ldw, dx, dw, db, M, N, K, act, p, stream);
+  if (dtype == CIT_BF16) return backward<bf16_t>(dy, ldy, z, x, ldx, w, ldw, dx, dw, db, M, N, K, act, p, stream);
+  return backward<fp16_t>(dy, ldy, z, x, ldx, w, ldw, dx, dw, db, M, N, K, act, p, stream);
+}
+
+}  // extern "C"

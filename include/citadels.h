@@ -400,6 +400,59 @@ int cit_cfr_targets(void* pool, int B, int node_cap, int edge_cap, const int32_t
                     uint32_t* mt_idx, const int32_t* offsets, int32_t* meta, float* feat, double* value, double* dist,
                     float* opt_feat, hipStream_t stream);
 
+/* ---- operators of a net's training step and of serving it (ops.py) ----------
+ * Element types of their buffers; matrices are rows of neighbouring elements,
+ * `ld` elements apart, at the element's own alignment.  Workspaces belong to
+ * one call until it has run. */
+#define CIT_FP32 0
+#define CIT_BF16 1
+#define CIT_FP16 2
+
+/* y [M][N] = act(x w^T + bias) + residual: x [M][K], w [N][K], bias [N] and
+ * residual [M][N] may be NULL; act 0 none, 1 relu, 2 gelu (erf), 3 silu; sums
+ * in fp32.  z [M][N] (may be NULL) receives the pre-activation for the
+ * backward pass in the element type (a finite value stays finite, a nonzero one nonzero).
+ * cit_linear_backward: from dy [M][N] (and z; relu without a residual may give y
+ * for z; act none ignores it) dx [M][K], dw [N][K] and db [N], each unless NULL. */
+size_t cit_linear_forward_work_bytes(int M, int N, int K, int dtype);
+int cit_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
+                       int64_t ldr, void* y, void* z, int M, int N, int K, int dtype, int act, void* work,
+                       size_t work_bytes, hipStream_t stream);
+size_t cit_linear_backward_work_bytes(int M, int N, int K, int dtype, int act);
+int cit_linear_backward(const void* dy, int64_t ldy, const void* z, const void* x, int64_t ldx, const void* w,
+                        int64_t ldw, void* dx, void* dw, void* db, int M, int N, int K, int dtype, int act, void* work,
+                        size_t work_bytes, hipStream_t stream);
+
+/* The clipped policy loss with a KL term over `rows` positions (ops.policy_loss
+ * has the formula): logits [rows][width] (offsets NULL), or one list of `total`
+ * entries, position i's from offsets[i] up to offsets[i + 1]; ref (may be NULL)
+ * and mask (bytes, 0 = illegal; may be NULL) lie as the logits do; weights NULL
+ * = 1 / rows.  Writes loss[0], logp[rows], kl[rows] and, unless grad is NULL,
+ * the gradient of the loss (dense rows without gaps; list entries of no
+ * position get 0).  cit_policy_loss_backward writes the gradient times
+ * upstream[0]; with skip_one, grad holds cit_policy_loss's and stays as it is
+ * if that is 1. */
+size_t cit_policy_loss_work_bytes(int64_t rows);
+int cit_policy_loss(const void* logits, int64_t ld, const void* ref, int64_t ld_ref, const uint8_t* mask,
+                    int64_t ld_mask, const int64_t* offsets, int64_t total, int64_t rows, int width,
+                    const int64_t* actions, const float* old_logp, const float* advantages, const float* weights,
+                    float low, float high, float kl_coef, int dtype, float* loss, float* logp, float* kl, void* grad,
+                    void* work, size_t work_bytes, hipStream_t stream);
+int cit_policy_loss_backward(const void* logits, int64_t ld, const void* ref, int64_t ld_ref, const uint8_t* mask,
+                             int64_t ld_mask, const int64_t* offsets, int64_t total, int64_t rows, int width,
+                             const int64_t* actions, const float* old_logp, const float* advantages,
+                             const float* weights, float low, float high, float kl_coef, int dtype,
+                             const float* upstream, int skip_one, void* grad, hipStream_t stream);
+
+/* norm[0] = sqrt(sum of all squares) of `tensors` gradients (host arrays of
+ * device pointers, element counts and types) and, unless out is NULL,
+ * out[t] = grads[t] * min(1, max_norm / (norm + 1e-6)): out[t] may be grads[t],
+ * else it overlaps no gradient; out_types[t] is types[t] or CIT_FP32. */
+size_t cit_clip_grad_norm_work_bytes(int tensors);
+int cit_clip_grad_norm(const void* const* grads, void* const* out, const int64_t* sizes, const int32_t* types,
+                       const int32_t* out_types, int tensors, double max_norm, float* norm, void* work,
+                       size_t work_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
