@@ -15,6 +15,8 @@
 // keep their digits (sum p d cancels to nothing there).  A row of weight 0 is
 // not read; a row that leaves no entry counts nothing, and the gradients of
 // both are 0.  An action outside its row makes the row NaN.
+#include <type_traits>
+
 #include "cit_ops.h"
 
 namespace {
@@ -57,52 +59,49 @@ __device__ __forceinline__ Row row_of(const Policy& a, int64_t i) {
   return r;
 }
 
-// p (d + exp(-d) - 1) for p > 0: the series where the three cancel.
-__device__ __forceinline__ float kl_term(float p, float q, float d) {
-  if (!(p > 0.0f)) return q;
+// e (x + exp(-x) - 1) from e = exp(a), er = e exp(-x): the series where the three
+// cancel (to 2^-25 of the value at |x| < 1/2), er itself where e is 0.
+__device__ __forceinline__ float kl_term(float e, float er, float x) {
   float s = 1.0f / 40320.0f;
-  s = fmaf(s, -d, 1.0f / 5040.0f);
-  s = fmaf(s, -d, 1.0f / 720.0f);
-  s = fmaf(s, -d, 1.0f / 120.0f);
-  s = fmaf(s, -d, 1.0f / 24.0f);
-  s = fmaf(s, -d, 1.0f / 6.0f);
-  s = fmaf(s, -d, 0.5f);
-  return fabsf(d) < 0.5f ? p * (d * d * s) : fmaf(p, d, q - p);
+  s = fmaf(s, -x, 1.0f / 5040.0f);
+  s = fmaf(s, -x, 1.0f / 720.0f);
+  s = fmaf(s, -x, 1.0f / 120.0f);
+  s = fmaf(s, -x, 1.0f / 24.0f);
+  s = fmaf(s, -x, 1.0f / 6.0f);
+  s = fmaf(s, -x, 0.5f);
+  const float t = fabsf(x) < 0.5f ? e * (x * x * s) : fmaf(e, x - 1.0f, er);
+  return e == 0.0f ? er : t;
 }
 
-struct Lse {                     // running maximum and sum of exp(x - maximum)
-  float m = -INFINITY, s = 0.0f;
-  __device__ __forceinline__ void add(float x) {
-    if (x == -INFINITY) return;                      // nothing, also before the first entry
-    if (x > m) {
-      s = fmaf(s, expf(m - x), 1.0f);
-      m = x;
-    } else {
-      s += m == INFINITY ? NAN : expf(x - m);        // a NaN comes through here too
-    }
-  }
-  __device__ __forceinline__ void join(float m2, float s2) {
-    const float t = fmaxf(m, m2);
-    const float a = m == t ? 1.0f : expf(m - t), b = m2 == t ? 1.0f : expf(m2 - t);
-    s = t == -INFINITY ? s + s2 : fmaf(s, a, s2 * b);
-    m = t;
+// Sums and maxima over the G lanes that share a row: shuffles, and LDS between the waves of a wide row.
+template <int G>
+struct Lanes {
+  static constexpr int WAVES = G > 64 ? G / 64 : 1;
+  float (*lds)[4];               // [WAVES][4], wide rows only
+
+  template <int N, bool MAX>
+  __device__ __forceinline__ void all(float (&v)[N]) const {
+#pragma unroll
+    for (int d = (G > 64 ? 64 : G) / 2; d; d >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const float o = __shfl_xor(v[i], d, 64);
+        v[i] = MAX ? fmaxf(v[i], o) : v[i] + o;
+      }
+    if (G <= 64) return;
+    const int w = threadIdx.x >> 6;
+    __syncthreads();                                 // the last round's readers are done
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < N; i++) lds[w][i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = lds[0][i];
+    for (int k = 1; k < WAVES; k++)
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = MAX ? fmaxf(v[i], lds[k][i]) : v[i] + lds[k][i];
   }
 };
-
-template <int G>
-__device__ __forceinline__ void join_lanes(Lse& v) {
-#pragma unroll
-  for (int d = G / 2; d; d >>= 1) {
-    const float m = __shfl_xor(v.m, d, 64), s = __shfl_xor(v.s, d, 64);
-    v.join(m, s);
-  }
-}
-template <int G>
-__device__ __forceinline__ float sum_lanes(float v) {
-#pragma unroll
-  for (int d = G / 2; d; d >>= 1) v += __shfl_xor(v, d, 64);
-  return v;
-}
 
 // What a row's statistics say about the loss: from lse, the action's logit and kl.
 struct Verdict {
@@ -132,64 +131,197 @@ __device__ __forceinline__ float action_logit(const Policy& a, const Row& r, int
   return to_f(static_cast<const T*>(a.logits)[r.at + k]);
 }
 
-__device__ __forceinline__ float grad_of(const Policy& a, float p, float d, const Verdict& v, bool chosen, float w) {
-  float t = a.ref && a.beta != 0.0f ? a.beta * (d - v.kl) - v.dlogp : -v.dlogp;
-  t = p > 0.0f ? p * t : p * 0.0f;                   // an entry of no probability has no gradient of its own
-  return w * (chosen ? t + v.dlogp : t);
+// E neighbouring entries of a row, in the words they were loaded as.
+template <typename T, int E>
+struct Pack {
+  static constexpr int W = E * (int)sizeof(T) > 4 ? E * (int)sizeof(T) / 4 : 1;
+  uint32_t w[W];
+
+  __device__ __forceinline__ float get(int k) const {
+    if (sizeof(T) == 4) return __builtin_bit_cast(float, w[k]);
+    const uint16_t h = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+    return to_f(__builtin_bit_cast(T, (typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type)h));
+  }
+  __device__ __forceinline__ void set(int k, float f) {
+    const T v = from_f<T>(f);
+    if (sizeof(T) == 4) {
+      w[k] = __builtin_bit_cast(uint32_t, f);
+      return;
+    }
+    uint16_t h;
+    __builtin_memcpy(&h, &v, 2);
+    w[k >> 1] = k & 1 ? (w[k >> 1] & 0xffffu) | ((uint32_t)h << 16) : (w[k >> 1] & 0xffff0000u) | h;
+  }
+  // Not to be unpacked once for all passes: that doubles the registers a row takes.
+  __device__ __forceinline__ void keep_packed() {
+#pragma unroll
+    for (int i = 0; i < W; i++) asm volatile("" : "+v"(w[i]));
+  }
+};
+template <typename T, int E>
+__device__ __forceinline__ Pack<T, E> load_pack(const T* row, const uint8_t* ok, int j, int len) {
+  Pack<T, E> v;
+  if (E > 1 && j + E <= len) {
+    const u32x4 u = load16(row + j);
+#pragma unroll
+    for (int i = 0; i < Pack<T, E>::W; i++) v.w[i] = u[i & 3];
+  } else {
+#pragma unroll
+    for (int i = 0; i < Pack<T, E>::W; i++) v.w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < E; i++) v.set(i, j + i < len ? to_f(row[j + i]) : -INFINITY);
+  }
+  if (ok) {                      // illegal entries are -inf from here on
+#pragma unroll
+    for (int i = 0; i < E; i++)
+      if (j + i < len && !ok[j + i]) v.set(i, -INFINITY);
+  }
+  return v;
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_pack(T* row, int j, int len, const Pack<T, E>& v) {
+  if (E > 1 && j + E <= len) {
+    u32x4 u;
+#pragma unroll
+    for (int i = 0; i < Pack<T, E>::W; i++) u[i & 3] = v.w[i];
+    store16(row + j, u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i++)
+      if (j + i < len) row[j + i] = from_f<T>(v.get(i));
+  }
 }
 
-// A row by G lanes, entry by entry (short rows).
-template <typename T, int G>
-__global__ __launch_bounds__(256) void k_policy_rows(Policy a, int row_blocks) {
-  __shared__ double sums[256 / G];
+// Entries of the list in front of the first row and behind the last: no gradient.
+template <typename T>
+__device__ void clear_ends(const Policy& a, int block, int blocks) {
+  T* grad = static_cast<T*>(a.grad);
+  const int64_t n = a.total;
+  int64_t first = a.offsets[0], last = a.offsets[a.rows];
+  first = first < 0 ? 0 : first > n ? n : first;
+  last = last < first ? first : last > n ? n : last;
+  const int64_t at = (int64_t)block * blockDim.x + threadIdx.x, step = (int64_t)blocks * blockDim.x;
+  for (int64_t j = at; j < first; j += step) grad[j] = from_f<T>(0.0f);
+  for (int64_t j = last + at; j < n; j += step) grad[j] = from_f<T>(0.0f);
+}
+
+#define LOG2E 1.44269504088896341f
+#define LN2 0.693147180559945309f
+
+// A row by G lanes, each with up to NV packs of E entries in registers, so that
+// the logits come from memory once; a longer row is read again in each pass.
+//
+//   pass 1  the maxima of l and of the reference r
+//   pass 2  with powers of two (v_exp_f32):  e = 2^(l log2(e) - m2), m2 a whole
+//           number; x = l - r - c0 and er = e exp(-x), c0 the difference of the
+//           maxima on a grid of log(2) / 4096 (m2 and c0's power of two exact: no
+//           error that all entries share).  s = sum e, sr = sum er, F = sum e (x + exp(-x) - 1):
+//           with eta = 1 - sr / s,  d = x - L, L = -log1p(-eta), and
+//           KL = F / s + eta - L.  One pass gives KL without its cancellation.
+//   pass 3  the gradient: p = 2^(l log2(e) - log2(e) lse), one exp more
+template <typename T, int G, int NV, int E, bool REF>
+__global__ __launch_bounds__(G > 256 ? G : 256, G > 256 ? 4 : 2) void k_policy(Policy a, int row_blocks) {
+  constexpr int THREADS = G > 256 ? G : 256, GROUPS = THREADS / G;
+  __shared__ double sums[GROUPS];
+  __shared__ float between[G > 64 ? G / 64 : 1][4];
   const float up = a.upstream ? *a.upstream : 1.0f;
   if (a.upstream && a.skip_one && up == 1.0f) return;
-  T* grad = static_cast<T*>(a.grad);
-  if ((int)blockIdx.x >= row_blocks) {               // entries in front of the first row and behind the last: no gradient
-    const int64_t n = a.total;
-    int64_t first = a.offsets[0], last = a.offsets[a.rows];
-    first = first < 0 ? 0 : first > n ? n : first;
-    last = last < first ? first : last > n ? n : last;
-    const int64_t at = (int64_t)((int)blockIdx.x - row_blocks) * 256 + threadIdx.x;
-    const int64_t step = (int64_t)((int)gridDim.x - row_blocks) * 256;
-    for (int64_t j = at; j < first; j += step) grad[j] = from_f<T>(0.0f);
-    for (int64_t j = last + at; j < n; j += step) grad[j] = from_f<T>(0.0f);
+  if ((int)blockIdx.x >= row_blocks) {
+    clear_ends<T>(a, (int)blockIdx.x - row_blocks, (int)gridDim.x - row_blocks);
     return;
   }
   const int lane = threadIdx.x % G;
-  const int64_t i = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const int64_t i = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G;
+  const Lanes<G> lanes{between};
   double counted = 0.0;
-  if (i < a.rows) {
+  if (i < a.rows) {              // the same for all lanes of a row: barriers inside are met by all of a wide row
     const Row r = row_of(a, i);
     const float w = weight_of(a, i);
-    const T* l = static_cast<const T*>(a.logits) + r.at;
-    const T* q = a.ref ? static_cast<const T*>(a.ref) + r.at_ref : nullptr;
+    const T* lrow = static_cast<const T*>(a.logits) + r.at;
+    const T* qrow = REF ? static_cast<const T*>(a.ref) + r.at_ref : nullptr;
     const uint8_t* ok = a.mask ? a.mask + r.at_mask : nullptr;
+    T* grow = a.grad ? static_cast<T*>(a.grad) + r.at_grad : nullptr;
     Verdict v = {0.0f, 0.0f, 0.0f, 0.0f};
-    float lse = 0.0f, lse_q = 0.0f;
     bool live = w != 0.0f && !r.bad;
-    if (live) {
-      Lse x, y;
-      for (int j = lane; j < r.len; j += G) {
-        if (ok && !ok[j]) continue;
-        x.add(to_f(l[j]));
-        if (q) y.add(to_f(q[j]));
-      }
-      join_lanes<G>(x);
-      join_lanes<G>(y);
-      live = !(x.s == 0.0f);
-      if (live) {
-        lse = x.m + logf(x.s), lse_q = y.m + logf(y.s);
-        float kl = 0.0f;
-        if (q) {
-          for (int j = lane; j < r.len; j += G) {
-            if (ok && !ok[j]) continue;
-            const float lp = to_f(l[j]) - lse, lq = to_f(q[j]) - lse_q;
-            kl += kl_term(expf(lp), expf(lq), lp - lq);
+    float lse2 = 0.0f, c0 = 0.0f, shift = 0.0f;
+    const bool held = r.len <= G * NV * E;
+    Pack<T, E> l[NV], q[NV];
+    // f(j, l, q) for every pack of the row this lane has
+    auto visit = [&](auto&& f) {
+      if (held) {
+#pragma unroll
+        for (int n = 0; n < NV; n++)
+          if ((n * G + lane) * E < r.len) {
+            l[n].keep_packed();
+            if (REF) q[n].keep_packed();
+            f((n * G + lane) * E, l[n], q[n]);
           }
-          kl = sum_lanes<G>(kl);
+      } else {
+        for (int j = lane * E; j < r.len; j += G * E) {
+          const Pack<T, E> x = load_pack<T, E>(lrow, ok, j, r.len);
+          f(j, x, REF ? load_pack<T, E>(qrow, ok, j, r.len) : x);
         }
-        v = judge(a, i, action_logit<T>(a, r, i) - lse, kl);
+      }
+    };
+    if (live) {
+      const float old_action = action_logit<T>(a, r, i);
+      if (held) {
+#pragma unroll
+        for (int n = 0; n < NV; n++) {
+          const int j = (n * G + lane) * E;
+          if (j < r.len) {
+            l[n] = load_pack<T, E>(lrow, ok, j, r.len);
+            if (REF) q[n] = load_pack<T, E>(qrow, ok, j, r.len);
+          }
+        }
+      }
+      float m[2] = {-INFINITY, -INFINITY};
+      visit([&](int, const Pack<T, E>& x, const Pack<T, E>& y) {
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+          m[0] = fmaxf(m[0], x.get(k));
+          if (REF) m[1] = fmaxf(m[1], y.get(k));
+        }
+      });
+      lanes.template all<2, true>(m);
+      // Far from 0 (a type's lowest value as a mask) the scaled exponents would leave fp32: such a row is moved
+      // by its maximum first, which a softmax does not see.
+      shift = fabsf(m[0]) > 1e30f && fabsf(m[0]) < INFINITY ? m[0] : 0.0f;
+      const float shift_q = REF && fabsf(m[1]) > 1e30f && fabsf(m[1]) < INFINITY ? m[1] : 0.0f;
+      const float top = m[0] - shift, top_q = m[1] - shift_q;
+      const float m2 = top == -INFINITY ? 0.0f : ceilf(top * LOG2E);
+      float c2 = 0.0f;
+      if (REF) c2 = rintf((top - top_q) * (LOG2E * 4096.0f)) * (1.0f / 4096.0f);
+      if (!(fabsf(c2) < 1e30f)) c2 = 0.0f;
+      c0 = c2 * LN2 + shift - shift_q;
+      const float at_q = c2 - m2;
+      float t[3] = {0.0f, 0.0f, 0.0f};
+      visit([&](int, const Pack<T, E>& x, const Pack<T, E>& y) {
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+          const float lx = x.get(k) - shift;
+          const float e = __builtin_amdgcn_exp2f(fmaf(lx, LOG2E, -m2));
+          t[0] += e;
+          if (REF) {
+            const float qx = y.get(k) - shift_q;
+            const float er = __builtin_amdgcn_exp2f(fmaf(qx, LOG2E, at_q));
+            t[1] += er;
+            t[2] += kl_term(e, er, lx - qx - c2 * LN2);
+          }
+        }
+      });
+      lanes.template all<3, false>(t);
+      live = !(t[0] == 0.0f);
+      if (live) {
+        lse2 = m2 + __builtin_amdgcn_logf(t[0]);
+        float kl = 0.0f;
+        if (REF) {
+          const float eta = (t[0] - t[1]) / t[0], L = -log1pf(-eta);
+          kl = t[2] / t[0] + (fabsf(eta) < 0.01f ? -eta * eta * fmaf(eta, fmaf(eta, 0.25f, 1.0f / 3.0f), 0.5f) : eta - L);
+          kl = kl < 0.0f ? 0.0f : kl;
+          c0 += L;               // d = l - r - c0 from here on
+        }
+        v = judge(a, i, (old_action - shift) - lse2 * LN2, kl);
       }
     }
     if (r.bad && w != 0.0f) v = {NAN, NAN, NAN, NAN};
@@ -197,16 +329,42 @@ __global__ __launch_bounds__(256) void k_policy_rows(Policy a, int row_blocks) {
       a.logp[i] = v.logp, a.kl[i] = v.kl;
       counted = w != 0.0f ? (double)w * (double)v.loss : 0.0;
     }
-    if (grad) {
-      const int64_t act = a.actions[i];
-      T* g = grad + r.at_grad;
-      for (int j = lane; j < r.len; j += G) {
-        float t = 0.0f;
-        if (live && !(ok && !ok[j])) {
-          const float lp = to_f(l[j]) - lse;
-          t = grad_of(a, expf(lp), q ? lp - (to_f(q[j]) - lse_q) : 0.0f, v, j == act, up * w);
-        }
-        g[j] = from_f<T>(t);
+    if (grow) {
+      const int64_t action = a.actions[i];
+      const float uw = up * w;
+      if (live) {
+        const float bw = REF ? uw * a.beta : 0.0f;
+        const float flat = -uw * v.dlogp - (bw != 0.0f ? bw * (c0 + v.kl) : 0.0f);   // p (bw (l - r) + flat)
+        visit([&](int j, const Pack<T, E>& x, const Pack<T, E>& y) {
+          Pack<T, E> g = x;
+#pragma unroll
+          for (int k = 0; k < E; k++) {
+            const float lx = x.get(k);
+            const float p = __builtin_amdgcn_exp2f(fmaf(lx - shift, LOG2E, -lse2));
+            float d = flat;
+            if (REF) d = bw != 0.0f ? fmaf(bw, lx - y.get(k), flat) : flat;
+            d = p == 0.0f ? flat : d;                // an entry of no probability: 0, not 0 times infinity
+            g.set(k, p * d);
+          }
+          store_pack<T, E>(grow, j, r.len, g);
+          if (action >= j && action < j + E && action < r.len) {
+            // the chosen entry has uw dlogp besides; its lane has just stored the pack
+            const int k = (int)(action - j);
+            float lx = -INFINITY, qx = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < E; c++)
+              if (c == k) {
+                lx = x.get(c);
+                if (REF) qx = y.get(c);
+              }
+            const float p = __builtin_amdgcn_exp2f(fmaf(lx - shift, LOG2E, -lse2));
+            float d = REF && bw != 0.0f && p != 0.0f ? fmaf(bw, lx - qx, flat) : flat;
+            if (!(ok && !ok[action])) grow[action] = from_f<T>(fmaf(p, d, uw * v.dlogp));
+          }
+        });
+      } else {
+        Pack<T, E> zero = {};
+        for (int j = lane * E; j < r.len; j += G * E) store_pack<T, E>(grow, j, r.len, zero);
       }
     }
   }
@@ -215,42 +373,82 @@ __global__ __launch_bounds__(256) void k_policy_rows(Policy a, int row_blocks) {
   __syncthreads();
   if (threadIdx.x == 0) {
     double s = 0.0;
-    for (int k = 0; k < 256 / G; k++) s += sums[k];
+    for (int k = 0; k < GROUPS; k++) s += sums[k];
     a.part[blockIdx.x] = s;
   }
 }
 
-__global__ __launch_bounds__(1024) void k_policy_sum(const double* part, int64_t count, float* loss) {
+#define SUM_BLOCKS 256
+
+// Sums in a fixed order: each workgroup its share to part2, or one workgroup the whole to loss.
+__global__ __launch_bounds__(1024) void k_policy_sum(const double* part, int64_t count, double* part2, float* loss) {
   __shared__ double sums[16];
+  const int64_t share = (count + gridDim.x - 1) / gridDim.x;
+  const int64_t first = share * blockIdx.x, last = first + share < count ? first + share : count;
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < count; i += 1024) s += part[i];
+  for (int64_t i = first + threadIdx.x; i < last; i += 1024) s += part[i];
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x) return;
   s = 0.0;
   for (int i = 0; i < 16; i++) s += sums[i];
-  *loss = (float)s;
+  if (part2) part2[blockIdx.x] = s;
+  else *loss = (float)s;
 }
 
-int64_t row_blocks(int64_t rows) { return (rows + 3) / 4; }            // 64 lanes a row, 4 rows a workgroup
+// Lanes of a row and entries they hold: `width` is a dense row's, or twice a
+// ragged batch's mean (its rows' lengths stay on the device).
+struct Shape {
+  int lanes, packs;              // lanes of a row; packs of 16 bytes (packs = 0: single entries, 4 a lane)
+};
+Shape shape_of(int64_t width, int dtype) {
+  const int64_t e = dtype == CIT_FP32 ? 4 : 8;
+  if (width <= 64) return {16, 0};
+  if (width <= 256) return {64, 0};
+  if (width <= 64 * 4 * e) return {64, 4};
+  if (width <= 256 * 4 * e) return {256, 4};
+  if (width <= 512 * 8 * e) return {512, 8};
+  return {1024, 8};
+}
+int64_t width_of(int64_t rows, int64_t total, int width, bool ragged) {
+  return ragged ? (rows > 0 ? 2 * (total / rows) : 0) : width;
+}
+int64_t row_blocks(int64_t rows, const Shape& s) {
+  const int groups = s.lanes > 256 ? 1 : 256 / s.lanes;
+  return (rows + groups - 1) / groups;
+}
+
+template <typename T, int G, int NV, int E>
+void launch_shape(const Policy& a, int64_t blocks, hipStream_t stream) {
+  const int tail = a.grad && a.offsets ? 64 : 0;
+  const dim3 grid((unsigned)(blocks + tail)), block(G > 256 ? G : 256);
+  if (a.ref) hipLaunchKernelGGL((k_policy<T, G, NV, E, true>), grid, block, 0, stream, a, (int)blocks);
+  else hipLaunchKernelGGL((k_policy<T, G, NV, E, false>), grid, block, 0, stream, a, (int)blocks);
+}
 
 template <typename T>
-int launch(const Policy& a, hipStream_t stream) {
-  const int64_t blocks = row_blocks(a.rows);
-  const int tail = a.grad && a.offsets ? 64 : 0;
-  hipLaunchKernelGGL((k_policy_rows<T, 64>), dim3((unsigned)(blocks + tail)), dim3(256), 0, stream, a, (int)blocks);
+int launch(const Policy& a, const Shape& s, hipStream_t stream) {
+  constexpr int E = 16 / sizeof(T);
+  const int64_t blocks = row_blocks(a.rows, s);
+  if (s.lanes == 16) launch_shape<T, 16, 4, 1>(a, blocks, stream);
+  else if (s.lanes == 64 && !s.packs) launch_shape<T, 64, 4, 1>(a, blocks, stream);
+  else if (s.lanes == 64) launch_shape<T, 64, 4, E>(a, blocks, stream);
+  else if (s.lanes == 256) launch_shape<T, 256, 4, E>(a, blocks, stream);
+  else if (s.lanes == 512) launch_shape<T, 512, 8, E>(a, blocks, stream);
+  else launch_shape<T, 1024, 8, E>(a, blocks, stream);
   return launch_status();
 }
 
 int run(const Policy& a, int dtype, hipStream_t stream) {
-  if (dtype == CIT_FP32) return launch<float>(a, stream);
-  if (dtype == CIT_BF16) return launch<bf16_t>(a, stream);
-  return launch<fp16_t>(a, stream);
+  const Shape s = shape_of(width_of(a.rows, a.total, a.width, a.offsets != nullptr), dtype);
+  if (dtype == CIT_FP32) return launch<float>(a, s, stream);
+  if (dtype == CIT_BF16) return launch<bf16_t>(a, s, stream);
+  return launch<fp16_t>(a, s, stream);
 }
 
 bool bad(const Policy& a, int dtype) {
-  if (dtype < CIT_FP32 || dtype > CIT_FP16 || a.rows < 0 || row_blocks(a.rows) > INT32_MAX / 2) return true;
+  if (dtype < CIT_FP32 || dtype > CIT_FP16 || a.rows < 0 || a.rows > INT32_MAX / 2) return true;
   if (!(a.low >= 0.0f) || !(a.high >= 0.0f) || !(a.beta >= 0.0f)) return true;
   if (!a.rows) return false;
   if (!a.actions || !a.old || !a.adv) return true;
@@ -263,7 +461,9 @@ bool bad(const Policy& a, int dtype) {
 
 extern "C" {
 
-size_t cit_policy_loss_work_bytes(int64_t rows) { return rows > 0 ? (size_t)row_blocks(rows) * sizeof(double) : 0; }
+size_t cit_policy_loss_work_bytes(int64_t rows) {
+  return rows > 0 ? ((size_t)rows + SUM_BLOCKS) * sizeof(double) : 0;
+}
 
 int cit_policy_loss(const void* logits, int64_t ld, const void* ref, int64_t ld_ref, const uint8_t* mask,
                     int64_t ld_mask, const int64_t* offsets, int64_t total, int64_t rows, int width,
@@ -280,7 +480,15 @@ int cit_policy_loss(const void* logits, int64_t ld, const void* ref, int64_t ld_
     const int rc = run(a, dtype, stream);
     if (rc) return rc;
   }
-  hipLaunchKernelGGL(k_policy_sum, dim3(1), dim3(1024), 0, stream, a.part, rows ? row_blocks(rows) : 0, loss);
+  const int64_t parts =
+      rows ? row_blocks(rows, shape_of(width_of(rows, total, width, offsets != nullptr), dtype)) : 0;
+  if (parts > 64 * SUM_BLOCKS) {                     // one workgroup would be at it for longer than two launches take
+    double* part = a.part + rows;
+    hipLaunchKernelGGL(k_policy_sum, dim3(SUM_BLOCKS), dim3(1024), 0, stream, a.part, parts, part, nullptr);
+    hipLaunchKernelGGL(k_policy_sum, dim3(1), dim3(1024), 0, stream, part, (int64_t)SUM_BLOCKS, nullptr, loss);
+  } else {
+    hipLaunchKernelGGL(k_policy_sum, dim3(1), dim3(1024), 0, stream, a.part, parts, nullptr, loss);
+  }
   return launch_status();
 }
 

@@ -315,8 +315,15 @@ def policy_want(a, clip, beta):
             d = torch.where(ok, lp - (q - torch.logsumexp(q, 0)), 0.0)
             pq = torch.where(ok, torch.exp(q - torch.logsumexp(q, 0)), 0.0)
             kl = float((p * d).sum())
-            far = d.abs() >= 0.45
-            klt = float(((p - pq).abs() * (err + err_q)).sum()) + abs(kl) * (err + (n + 20) * U) \
+            # The kernel sums p f(x), f(x) = x + exp(-x) - 1, around x = d + L, L the difference of the log sums less
+            # that of the maxima, and takes L + exp(-L) - 1 off again, which is what the shift added:
+            # sum p f(d + L) = KL + L - 1 + exp(-L).  So its sum's error counts on KL + f(L), and an entry's own error
+            # (err, err_q in the exponents) moves its term by |p - q|, or by p + q where |x| >= 1/2.  What is taken off
+            # has the slope 1 - exp(-L) in the ratio of the two sums.
+            L = abs(float((l.max() - q.max()) - (torch.logsumexp(l, 0) - torch.logsumexp(q, 0)))) + 2e-4
+            shifted = math.exp(L) - L - 1                            # f(-L) >= f(L) for L > 0
+            far = d.abs() + L >= 0.5
+            klt = float(((p - pq).abs() * (err + err_q)).sum()) + (abs(kl) + shifted + math.exp(L) - 1) * (err + err_q + (n + 20) * U) \
                 + float((4 * U * (p * d.abs() + p + pq) + (err + err_q) * (p + pq))[far].sum())
             kls[i], tk[i] = kl, klt
         adv, ratio = float(a["adv"][i]), math.exp(float(lp[act]) - float(a["old"][i]))
@@ -481,7 +488,7 @@ def test_policy_entries_of_no_row():
     ga, gb = torch.autograd.grad(x.loss, la)[0], torch.autograd.grad(y.loss, lb)[0]
     assert torch.equal(gb[4:82], ga) and not bool(gb[:4].any()) and not bool(gb[82:].any())
     none = ops.policy_loss(lb, a["actions"][:0], a["old"][:0], a["adv"][:0], offsets=a["offsets"][:1])
-    assert float(none.loss) == 0.0 and none.logp.shape == (0,)
+    assert float(none.loss.detach()) == 0.0 and none.logp.shape == (0,)
     assert not bool(torch.autograd.grad(none.loss, lb)[0].any())
     assert float(ops.policy_loss(la.view(1, -1)[:0], a["actions"][:0], a["old"][:0], a["adv"][:0]).loss) == 0.0
 
