@@ -13,6 +13,13 @@
 // element type is the store.
 #include "cit_ops.h"
 
+#ifndef CIT_BIG_WAVES
+#define CIT_BIG_WAVES 2, 4, false
+#endif
+#ifndef CIT_MID_AHEAD
+#define CIT_MID_AHEAD true
+#endif
+
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -74,49 +81,103 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int n, int 
   static_cast<T*>(e.out)[m * e.ldo + n] = from_f<T>(v);
 }
 
-struct __attribute__((packed, aligned(2))) any_f4 { float v[4]; };
-
-// Four neighbouring columns of one row (count of them inside N).
+// Eight neighbouring columns of one row, from n on (those inside N).
 template <typename T>
-__device__ __forceinline__ void finish4(const Epilogue& e, int64_t m, int n, int N, f32x4 v, int split, int64_t M) {
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  Pack16<T> u[sizeof(T) / 2];
+#pragma unroll
+  for (int h = 0; h < (int)sizeof(T) / 2; h++) u[h].raw = load16(p + h * Pack16<T>::N);
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = to_f(u[i / Pack16<T>::N].e[i % Pack16<T>::N]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const T (&v)[8]) {
+  Pack16<T> u[sizeof(T) / 2];
+#pragma unroll
+  for (int i = 0; i < 8; i++) u[i / Pack16<T>::N].e[i % Pack16<T>::N] = v[i];
+#pragma unroll
+  for (int h = 0; h < (int)sizeof(T) / 2; h++) store16(p + h * Pack16<T>::N, u[h].raw);
+}
+
+template <typename T>
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n, int N, float (&v)[8], int split,
+                                        int64_t M) {
   if (e.part) {
     float* p = e.part + ((int64_t)split * M + m) * N + n;
-    if (n + 4 <= N) {
-      any_f4 o;
-      for (int i = 0; i < 4; i++) o.v[i] = v[i];
-      *reinterpret_cast<any_f4*>(p) = o;
+    if (n + 8 <= N) {
+      store8<float>(p, v);
     } else {
-      for (int i = 0; n + i < N; i++) p[i] = v[i];
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (n + i < N) p[i] = v[i];
     }
     return;
   }
-  struct __attribute__((packed, aligned(2))) row4 { T v[4]; };
-  if (n + 4 > N) {
-    for (int i = 0; n + i < N; i++) finish<T>(e, m, n + i, N, v[i]);
+  if (n + 8 > N) {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (n + i < N) finish<T>(e, m, n + i, N, v[i]);
     return;
   }
+  float t[8];
+  T o[8];
   if (e.bias) {
-    const row4 b = *reinterpret_cast<const row4*>(static_cast<const T*>(e.bias) + n);
+    load8<T>(static_cast<const T*>(e.bias) + n, t);
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] += to_f((T)b.v[i]);
+    for (int i = 0; i < 8; i++) v[i] += t[i];
   }
   if (e.z) {
-    row4 z;
 #pragma unroll
-    for (int i = 0; i < 4; i++) z.v[i] = keep_z<T>(v[i]);
-    *reinterpret_cast<row4*>(static_cast<T*>(e.z) + m * N + n) = z;
+    for (int i = 0; i < 8; i++) o[i] = keep_z<T>(v[i]);
+    store8<T>(static_cast<T*>(e.z) + m * N + n, o);
   }
+  if (e.act != ACT_NONE) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = act_fwd(e.act, v[i]);
+    for (int i = 0; i < 8; i++) v[i] = act_fwd(e.act, v[i]);
+  }
   if (e.res) {
-    const row4 r = *reinterpret_cast<const row4*>(static_cast<const T*>(e.res) + m * e.ldr + n);
+    load8<T>(static_cast<const T*>(e.res) + m * e.ldr + n, t);
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] += to_f((T)r.v[i]);
+    for (int i = 0; i < 8; i++) v[i] += t[i];
   }
-  row4 o;
 #pragma unroll
-  for (int i = 0; i < 4; i++) o.v[i] = from_f<T>(v[i]);
-  *reinterpret_cast<row4*>(static_cast<T*>(e.out) + m * e.ldo + n) = o;
+  for (int i = 0; i < 8; i++) o[i] = from_f<T>(v[i]);
+  store8<T>(static_cast<T*>(e.out) + m * e.ldo + n, o);
+}
+
+// A wave's sums, TM x TN blocks of 16 x 16 from (m0, n0) on, through its own
+// `bytes` of LDS so that rows leave in whole lines: a lane holds 4 columns of
+// one row (a 16-byte chunk; chunks permuted by the row against bank conflicts) and
+// writes out 8.  B went into the products as the instruction's rows, hence the
+// neighbouring columns.
+template <typename T, int TM, int TN, int BYTES>
+__device__ __forceinline__ void write_out(const Epilogue& e, const f32x4 (&acc)[TM][TN], char* lds, int m0, int n0,
+                                          int M, int N, int split) {
+  constexpr int ROW = TN * 64, CHUNKS = TN * 4;                        // bytes and chunks of a row
+  constexpr int FIT = BYTES / (16 * ROW), PER = FIT < TM ? FIT : TM;   // row blocks of a pass
+  static_assert(PER >= 1, "a row block fits");
+  const int l = threadIdx.x & 63;
+#pragma unroll
+  for (int i0 = 0; i0 < TM; i0 += PER) {
+#pragma unroll
+    for (int i = i0; i < i0 + PER && i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) {
+        const int r = (i - i0) * 16 + (l & 15), c = j * 4 + (l >> 4);
+        *reinterpret_cast<f32x4*>(lds + r * ROW + ((c ^ (r & (CHUNKS - 1))) << 4)) = acc[i][j];
+      }
+    const int rows = (TM - i0 < PER ? TM - i0 : PER) * 16;
+    for (int k = l; k < rows * (CHUNKS / 2); k += 64) {
+      const int r = k / (CHUNKS / 2), c = k % (CHUNKS / 2) * 2, x = r & (CHUNKS - 1);
+      const int m = m0 + i0 * 16 + r, n = n0 + c * 4;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(lds + r * ROW + ((c ^ x) << 4));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(lds + r * ROW + (((c + 1) ^ x) << 4));
+      if (m < M && n < N) {
+        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        finish8<T>(e, m, n, N, v, split, M);
+      }
+    }
+  }
 }
 
 // ---- operand tiles ------------------------------------------------------------
@@ -310,17 +371,182 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, 
     cur ^= 1;
   }
 
-  // B went in as the instruction's rows, so a lane holds 4 neighbouring n of one m.
-  const int l = threadIdx.x & 63;
+  constexpr int SHARE = (BM + BN) * 256 / (WM * WN);
+  write_out<T, TM, TN, SHARE>(e, acc, &lds[0][0] + w * SHARE, m0 + wm, n0 + wn, M, N, split);
+}
+
+// ---- the tile kernel with direct loads --------------------------------------------
+//
+// The same product for matrices whose rows start on 16 bytes (and, ks, whose
+// columns are whole chunks): global memory goes straight to LDS
+// (global_load_lds_dwordx4), so a tile costs no registers and no LDS write
+// instructions.  The chunk permutation of Tile is applied to the address each
+// lane reads, since a wave's 64 chunks land side by side.
+//
+// Two tiles of LDS, two k steps a tile, and two sets of fragments, so that the
+// matrix cores never wait for a load that was asked for in the same step:
+//
+//   read step 1 of tile t      multiply step 0 of tile t
+//   --- tile t + 1 has arrived, every wave has read tile t ---
+//   ask for tile t + 2 in tile t's place
+//   read step 0 of tile t + 1  multiply step 1 of tile t
+
+typedef const __attribute__((address_space(1))) void* global_ptr;
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+// One thread's share of a tile, asked for but not waited for.  Rows (ks:
+// chunks) past the edge repeat the last one; nothing of them is stored.
+template <typename T, bool KS, int R, int THREADS>
+struct Direct {
+  typedef Tile<T, KS, R> L;
+  static constexpr int PER = L::CHUNKS / THREADS;
+  const char* base;              // the next tile's first row, the same for all lanes
+  uint32_t off[PER];             // this thread's chunks behind it
+  int64_t step;                  // bytes to the tile after it
+
+  __device__ __forceinline__ void start(const Mat& a, int r0, int k0) {
 #pragma unroll
-  for (int i = 0; i < TM; i++) {
-    const int m = m0 + wm + i * 16 + (l & 15);
+    for (int i = 0; i < PER; i++) {
+      int row, c;
+      L::from(i * THREADS + (int)threadIdx.x, row, c);
+      int64_t at;
+      if (KS) {
+        int col = r0 + c * L::E;
+        if (col + L::E > a.cols) col = a.cols - L::E;
+        at = row * a.ld + (col - r0);
+      } else {
+        int r = row;
+        if (r0 + r >= a.rows) r = a.rows - 1 - r0;
+        at = r * a.ld + c * L::E;
+      }
+      off[i] = (uint32_t)(at * (int64_t)sizeof(T));
+    }
+    base = static_cast<const char*>(a.p) + (KS ? k0 * a.ld + r0 : r0 * a.ld + k0) * (int64_t)sizeof(T);
+    step = KS ? a.ld * BK<T> * (int64_t)sizeof(T) : 128;
+  }
+  __device__ __forceinline__ void next(char* lds) {
+    char* to = lds + (__builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63) << 4);   // the wave's place; lane i lands 16 i behind it
 #pragma unroll
-    for (int j = 0; j < TN; j++) {
-      const int n = n0 + wn + j * 16 + (l >> 4) * 4;
-      if (m < M && n < N) finish4<T>(e, m, n, N, acc[i][j], split, M);
+    for (int i = 0; i < PER; i++)
+      __builtin_amdgcn_global_load_lds((global_ptr)(base + off[i]), (lds_ptr)(to + i * THREADS * 16), 16, 0, 0);
+    base += step;
+  }
+};
+
+// Workgroup `b` of `n` runs on XCD b % 8: each XCD takes a run of neighbouring
+// tiles, in columns of 4 tile rows, so that what its L2 holds of A and B is
+// shared by its 32 compute units.
+__device__ __forceinline__ void place(int b, int n, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int per = n / 8, rest = n % 8, x = b & 7;
+  const int t = x * per + (x < rest ? x : rest) + (b >> 3);
+  constexpr int GROUP = 4;
+  const int wide = GROUP * tiles_n, g = t / wide, first = g * GROUP;
+  const int rows = tiles_m - first < GROUP ? tiles_m - first : GROUP;
+  tm = first + (t - g * wide) % rows;
+  tn = (t - g * wide) / rows;
+}
+
+template <typename T, bool AKS, bool BKS, int BM, int BN, int WM, int WN, bool AHEAD>
+__global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilogue e, int M, int N, int K, int tiles_m,
+                                                             int tiles_n, int k_per_split) {
+  constexpr int THREADS = WM * WN * 64;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int STEPS = 2;
+  // four arrays, not one: the compiler then sees that a load under way into one does not concern reads of another
+  __shared__ __attribute__((aligned(16))) char a0[BM * 128], b0[BN * 128], a1[BM * 128], b1[BN * 128];
+
+  int tm, tn;
+  place(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
+  const int split = blockIdx.y, m0 = tm * BM, n0 = tn * BN;
+  const int kb = split * k_per_split, ke = min(K, kb + k_per_split);
+  const int whole = (ke - kb) / BK<T>;
+  const int w = threadIdx.x >> 6;
+  const int wm = (w / WN) * (BM / WM), wn = (w % WN) * (BN / WN);
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  Direct<T, AKS, BM, THREADS> da;
+  Direct<T, BKS, BN, THREADS> db;
+  da.start(A, m0, kb);
+  db.start(B, n0, kb);
+  auto ask = [&](int t, char* la, char* lb) {
+    if (t < whole) {
+      da.next(la);
+      db.next(lb);
+    }
+  };
+  u32x4 fa[AHEAD ? 2 : 1][TM], fb[AHEAD ? 2 : 1][TN];
+  auto read = [&](int s, const char* la, const char* lb) {
+#pragma unroll
+    for (int i = 0; i < TM; i++) fa[AHEAD ? s : 0][i] = frag<T, AKS, BM>(la, wm + i * 16, s);
+#pragma unroll
+    for (int j = 0; j < TN; j++) fb[AHEAD ? s : 0][j] = frag<T, BKS, BN>(lb, wn + j * 16, s);
+  };
+  auto multiply = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[i][j] = mma(fb[AHEAD ? s : 0][j], fa[AHEAD ? s : 0][i], acc[i][j], T{});
+  };
+  auto tile = [&](int t, char* la, char* lb, char* na, char* nb) {
+    if (AHEAD) {
+      read(1, la, lb);
+      multiply(0);
+      __syncthreads();
+      ask(t + 2, la, lb);
+      if (t + 1 < whole) read(0, na, nb);
+      multiply(1);
+    } else {
+      ask(t + 1, na, nb);
+      read(0, la, lb);
+      multiply(0);
+      read(1, la, lb);
+      multiply(1);
+      __syncthreads();
+    }
+  };
+  ask(0, a0, b0);
+  __syncthreads();
+  if (AHEAD) {
+    ask(1, a1, b1);
+    if (whole) read(0, a0, b0);
+  }
+  for (int t = 0; t < whole; t += 2) {
+    tile(t, a0, b0, a1, b1);
+    if (t + 1 < whole) tile(t + 1, a1, b1, a0, b0);
+  }
+  if (kb + whole * BK<T> < ke) {
+    // the reduction ends inside a tile: that one through registers, zeros behind the end
+    Mat a = A, b = B;
+    if (AKS) a.rows = ke; else a.cols = ke;
+    if (BKS) b.rows = ke; else b.cols = ke;
+    __syncthreads();
+    {
+      Stage<T, AKS, BM, THREADS> sa;
+      sa.load(a, m0, kb + whole * BK<T>);
+      sa.store(a0);
+    }
+    {
+      Stage<T, BKS, BN, THREADS> sb;
+      sb.load(b, n0, kb + whole * BK<T>);
+      sb.store(b0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) {
+      read(s, a0, b0);
+      multiply(s);
     }
   }
+
+  __syncthreads();
+  static_assert(BM == BN && WM * WN % 4 == 0, "the waves share the four arrays evenly");
+  constexpr int EACH = WM * WN / 4, SHARE = BM * 128 / EACH;
+  char* mine = w / EACH == 0 ? a0 : w / EACH == 1 ? b0 : w / EACH == 2 ? a1 : b1;
+  write_out<T, TM, TN, SHARE>(e, acc, mine + (w % EACH) * SHARE, m0 + wm, n0 + wn, M, N, split);
 }
 
 // The splits' sums in their order, then the epilogue.
@@ -398,21 +624,61 @@ Plan plan_tiles(int M, int N, int K, int bm, int bn, int bk) {
 
 int elt(int dtype) { return dtype == CIT_FP32 ? 4 : 2; }
 
+enum { TILE_64, TILE_128, TILE_256 };
+
+// The tile of a product of aligned operands.
+int tile_of(int M, int N, int es) {
+  if (es == 2 && (int64_t)cdiv(M, 256) * cdiv(N, 256) >= 128) return TILE_256;
+  if ((int64_t)cdiv(M, 128) * cdiv(N, 128) >= 128) return TILE_128;
+  return TILE_64;
+}
+Plan plan_of(int tile, int M, int N, int K, int bk) {
+  const int t = tile == TILE_256 ? 256 : tile == TILE_128 ? 128 : 64;
+  return plan_tiles(M, N, K, t, t, bk);
+}
+
+// Room for split sums, whatever the operands' alignment makes of the tile.
 int64_t product_work(int M, int N, int K, int dtype) {
   if (M <= 0 || N <= 0) return 0;
-  const Plan p = plan_tiles(M, N, K, 64, 64, 128 / elt(dtype));
-  return p.splits > 1 ? align256((int64_t)p.splits * M * N * 4) : 0;
+  int64_t most = 0;
+  for (int tile : {(int)TILE_64, tile_of(M, N, elt(dtype))}) {
+    const Plan p = plan_of(tile, M, N, K, 128 / elt(dtype));
+    if (p.splits > 1 && p.splits > most) most = p.splits;
+  }
+  return align256(most * M * N * 4);
+}
+
+template <typename T>
+bool direct(const Mat& a, bool ks) {
+  if (((uintptr_t)a.p & 15) || (a.ld * (int64_t)sizeof(T)) % 16) return false;
+  if (a.ld * (int64_t)sizeof(T) >= 1 << 23) return false;             // a tile's rows within 31 bits of its first
+  return !ks || a.cols % (16 / (int)sizeof(T)) == 0;
+}
+
+template <typename T, bool AKS, bool BKS, int TILE, int WM, int WN, bool AHEAD>
+void launch_direct(const Mat& A, const Mat& B, const Epilogue& e, int M, int N, int K, const Plan& p,
+                   hipStream_t stream) {
+  hipLaunchKernelGGL((k_gemm_direct<T, AKS, BKS, TILE, TILE, WM, WN, AHEAD>), dim3(p.tiles_m * p.tiles_n, p.splits),
+                     dim3(WM * WN * 64), 0, stream, A, B, e, M, N, K, p.tiles_m, p.tiles_n, p.k_per);
 }
 
 template <typename T, bool AKS, bool BKS>
 int product(Mat A, Mat B, Epilogue e, int M, int N, int K, void* work, hipStream_t stream) {
-  const Plan p = plan_tiles(M, N, K, 64, 64, BK<T>);
+  const bool d = K > 0 && direct<T>(A, AKS) && direct<T>(B, BKS);
+  const int tile = d ? tile_of(M, N, sizeof(T)) : TILE_64;
+  const Plan p = plan_of(tile, M, N, K, BK<T>);
   if (p.splits > 1) e.part = static_cast<float*>(work);
-  hipLaunchKernelGGL((k_gemm<T, AKS, BKS, 64, 64, 2, 2>), dim3(p.tiles_m * p.tiles_n, p.splits), dim3(256), 0, stream,
-                     A, B, e, M, N, K, p.tiles_n, p.k_per);
-  if (p.splits > 1)
-    hipLaunchKernelGGL((k_join<T>), dim3(cdiv((int64_t)M * N, 256) < 4096 ? cdiv((int64_t)M * N, 256) : 4096), dim3(256), 0, stream, e, (int64_t)M, N,
-                       p.splits);
+  if (!d)
+    hipLaunchKernelGGL((k_gemm<T, AKS, BKS, 64, 64, 2, 2>), dim3(p.tiles_m * p.tiles_n, p.splits), dim3(256), 0, stream,
+                       A, B, e, M, N, K, p.tiles_n, p.k_per);
+  else if (tile == TILE_64) launch_direct<T, AKS, BKS, 64, 2, 2, true>(A, B, e, M, N, K, p, stream);
+  else if (tile == TILE_128) launch_direct<T, AKS, BKS, 128, 2, 2, CIT_MID_AHEAD>(A, B, e, M, N, K, p, stream);
+  else if constexpr (sizeof(T) == 2) launch_direct<T, AKS, BKS, 256, CIT_BIG_WAVES>(A, B, e, M, N, K, p, stream);
+  if (p.splits > 1) {
+    const int64_t blocks = ((int64_t)M * N + 255) / 256;
+    hipLaunchKernelGGL((k_join<T>), dim3(blocks < 4096 ? (unsigned)blocks : 4096), dim3(256), 0, stream, e, (int64_t)M,
+                       N, p.splits);
+  }
   return launch_status();
 }
 
