@@ -13,13 +13,6 @@
 // element type is the store.
 #include "cit_ops.h"
 
-#ifndef CIT_BIG_WAVES
-#define CIT_BIG_WAVES 2, 4, false
-#endif
-#ifndef CIT_MID_AHEAD
-#define CIT_MID_AHEAD true
-#endif
-
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -28,19 +21,55 @@ typedef short s16x4 __attribute__((__vector_size__(8)));
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
 
+// Phi(z) = erfc(-z / sqrt(2)) / 2 and exp(-z^2 / 2).  fp32 takes the library's erfc
+// (no cancellation at z < 0).  For 16-bit results it is Abramowitz and
+// Stegun's 7.1.26, off by at most 0.75e-7 absolute, whose exponential gelu's
+// derivative needs anyhow: a fifth of the instructions.
+template <typename T>
+__device__ __forceinline__ void normal_cdf(float z, float& cdf, float& e) {
+  if (sizeof(T) == 4) {
+    e = expf(-0.5f * z * z);
+    cdf = 0.5f * erfcf(-z * 0.70710678118654752f);
+    return;
+  }
+  e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(x, 0.3275911f, 1.0f));
+  float p = fmaf(t, 1.061405429f, -1.453152027f);
+  p = fmaf(t, p, 1.421413741f);
+  p = fmaf(t, p, -0.284496736f);
+  p = fmaf(t, p, 0.254829592f);
+  const float tail = 0.5f * p * t * e;
+  cdf = z < 0.0f ? tail : 1.0f - tail;
+}
+template <typename T>
+__device__ __forceinline__ float sigmoid(float z) {
+  if (sizeof(T) == 4) return 1.0f / (1.0f + expf(-z));
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+}
+
+template <typename T>
 __device__ __forceinline__ float act_fwd(int act, float z) {
   if (act == ACT_RELU) return z < 0.0f ? 0.0f : z;                  // NaN stays
-  if (act == ACT_GELU) return 0.5f * z * erfcf(-z * 0.70710678118654752f);   // erfc: no cancellation at z < 0
-  if (act == ACT_SILU) return z / (1.0f + expf(-z));
+  if (act == ACT_GELU) {
+    float cdf, e;
+    normal_cdf<T>(z, cdf, e);
+    return z * cdf;
+  }
+  if (act == ACT_SILU) return z * sigmoid<T>(z);
   return z;
 }
+template <typename T>
 __device__ __forceinline__ float act_grad(int act, float z) {
   if (act == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  if (act == ACT_GELU)
-    return 0.5f * erfcf(-z * 0.70710678118654752f) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+  if (act == ACT_GELU) {
+    float cdf, e;
+    normal_cdf<T>(z, cdf, e);
+    return fmaf(z * 0.39894228040143268f, e, cdf);
+  }
   if (act == ACT_SILU) {
-    const float s = 1.0f / (1.0f + expf(-z));
-    return s * (1.0f + z * (1.0f - s));
+    const float s = sigmoid<T>(z);
+    return s * fmaf(z, 1.0f - s, 1.0f);
   }
   return 1.0f;
 }
@@ -76,7 +105,7 @@ template <typename T>
 __device__ __forceinline__ void finish(const Epilogue& e, int64_t m, int n, int N, float v) {
   if (e.bias) v += to_f(static_cast<const T*>(e.bias)[n]);
   if (e.z) static_cast<T*>(e.z)[m * N + n] = keep_z<T>(v);
-  v = act_fwd(e.act, v);
+  v = act_fwd<T>(e.act, v);
   if (e.res) v += to_f(static_cast<const T*>(e.res)[m * e.ldr + n]);
   static_cast<T*>(e.out)[m * e.ldo + n] = from_f<T>(v);
 }
@@ -133,7 +162,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n, int
   }
   if (e.act != ACT_NONE) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = act_fwd(e.act, v[i]);
+    for (int i = 0; i < 8; i++) v[i] = act_fwd<T>(e.act, v[i]);
   }
   if (e.res) {
     load8<T>(static_cast<const T*>(e.res) + m * e.ldr + n, t);
@@ -563,39 +592,75 @@ __global__ __launch_bounds__(256) void k_join(Epilogue e, int64_t M, int N, int 
 
 // ---- dz and db --------------------------------------------------------------------
 //
-// Block (column block, row share): 64 columns of the share's rows, 4 waves down
-// the rows.  dz = dy act'(z) rounded once to the element type (the matrix
-// cores' input), its column sums taken before that rounding.
+// Workgroup (column block, row share): 16 lanes across 8 columns each, 16 rows
+// down, over the share's rows.  dz = dy act'(z) rounded once to the element
+// type (the matrix cores' input), its column sums taken before that rounding.
+// Bound by memory: dy and z read, dz written.
+
+#define DZ_COLUMNS 128
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_dz(const T* dy, int64_t ldy, const T* z, T* dz, float* db, int M, int N,
-                                            int act, int rows_per) {
-  __shared__ float sums[4][64];
-  const int n = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+__global__ __launch_bounds__(256) void k_dz(const T* dy, int64_t ldy, const T* z, T* dz, T* db, float* part, int M,
+                                            int N, int act, int rows_per) {
+  __shared__ float sums[16][DZ_COLUMNS + 4];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+  const int n = blockIdx.x * DZ_COLUMNS + x * 8;
   const int mb = blockIdx.y * rows_per, me = min(M, mb + rows_per);
-  float s = 0.0f;
-  if (n < N)
-    for (int m = mb + w; m < me; m += 4) {
-      float v = to_f(dy[(int64_t)m * ldy + n]);
-      if (act != ACT_NONE) v *= act_grad(act, to_f(z[(int64_t)m * N + n]));
-      s += v;
-      if (dz) dz[(int64_t)m * N + n] = from_f<T>(v);
+  float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (n + 8 <= N) {
+#pragma unroll 2
+    for (int m = mb + y; m < me; m += 16) {
+      float v[8], u[8];
+      load8<T>(dy + m * ldy + n, v);
+      if (act != ACT_NONE) {
+        load8<T>(z + (int64_t)m * N + n, u);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= act_grad<T>(act, u[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) s[i] += v[i];
+      if (dz) {
+        T o[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = from_f<T>(v[i]);
+        store8<T>(dz + (int64_t)m * N + n, o);
+      }
     }
-  if (!db) return;
-  sums[w][threadIdx.x & 63] = s;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (n + i < N)
+        for (int m = mb + y; m < me; m += 16) {
+          float v = to_f(dy[m * ldy + n + i]);
+          if (act != ACT_NONE) v *= act_grad<T>(act, to_f(z[(int64_t)m * N + n + i]));
+          s[i] += v;
+          if (dz) dz[(int64_t)m * N + n + i] = from_f<T>(v);
+        }
+  }
+  if (!db && !part) return;
+#pragma unroll
+  for (int i = 0; i < 8; i++) sums[y][x * 8 + i] = s[i];
   __syncthreads();
-  if (w == 0 && n < N)
-    db[(int64_t)blockIdx.y * N + n] =
-        (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
+  const int c = blockIdx.x * DZ_COLUMNS + threadIdx.x;
+  if (threadIdx.x >= DZ_COLUMNS || c >= N) return;
+  float t = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) t += sums[i][threadIdx.x];
+  if (part) part[(int64_t)blockIdx.y * N + c] = t;
+  else db[c] = from_f<T>(t);
 }
 
+// The shares' column sums: 4 waves over the shares, in a fixed order.
 template <typename T>
 __global__ __launch_bounds__(256) void k_db(const float* part, T* db, int N, int shares) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
+  __shared__ float sums[4][64];
+  const int x = threadIdx.x & 63, w = threadIdx.x >> 6, n = blockIdx.x * 64 + x;
   float s = 0.0f;
-  for (int i = 0; i < shares; i++) s += part[(int64_t)i * N + n];
-  db[n] = from_f<T>(s);
+  if (n < N)
+    for (int i = w; i < shares; i += 4) s += part[(int64_t)i * N + n];
+  sums[w][x] = s;
+  __syncthreads();
+  if (w == 0 && n < N) db[n] = from_f<T>((sums[0][x] + sums[1][x]) + (sums[2][x] + sums[3][x]));
 }
 
 // ---- host side ---------------------------------------------------------------------
@@ -672,8 +737,8 @@ int product(Mat A, Mat B, Epilogue e, int M, int N, int K, void* work, hipStream
     hipLaunchKernelGGL((k_gemm<T, AKS, BKS, 64, 64, 2, 2>), dim3(p.tiles_m * p.tiles_n, p.splits), dim3(256), 0, stream,
                        A, B, e, M, N, K, p.tiles_n, p.k_per);
   else if (tile == TILE_64) launch_direct<T, AKS, BKS, 64, 2, 2, true>(A, B, e, M, N, K, p, stream);
-  else if (tile == TILE_128) launch_direct<T, AKS, BKS, 128, 2, 2, CIT_MID_AHEAD>(A, B, e, M, N, K, p, stream);
-  else if constexpr (sizeof(T) == 2) launch_direct<T, AKS, BKS, 256, CIT_BIG_WAVES>(A, B, e, M, N, K, p, stream);
+  else if (tile == TILE_128) launch_direct<T, AKS, BKS, 128, 2, 2, true>(A, B, e, M, N, K, p, stream);
+  else if constexpr (sizeof(T) == 2) launch_direct<T, AKS, BKS, 256, 2, 4, false>(A, B, e, M, N, K, p, stream);
   if (p.splits > 1) {
     const int64_t blocks = ((int64_t)M * N + 255) / 256;
     hipLaunchKernelGGL((k_join<T>), dim3(blocks < 4096 ? (unsigned)blocks : 4096), dim3(256), 0, stream, e, (int64_t)M,
@@ -682,13 +747,13 @@ int product(Mat A, Mat B, Epilogue e, int M, int N, int K, void* work, hipStream
   return launch_status();
 }
 
+// Rows of a share: about 4 workgroups for each compute unit, at least 64 rows each.
 int dz_rows(int M, int N) {
-  const int columns = cdiv(N, 64);
-  int shares = cdiv(1024, columns);
+  int shares = cdiv(1024, cdiv(N, DZ_COLUMNS));
   const int most = cdiv(M, 64);
   if (shares > most) shares = most;
-  if (shares > 256) shares = 256;
-  return cdiv(M, shares);
+  if (shares < 1) shares = 1;
+  return cdiv(cdiv(M, shares), 16) * 16;
 }
 
 template <typename T>
@@ -709,15 +774,15 @@ int backward(const void* dy, int64_t ldy, const void* z, const void* x, int64_t 
     dz = reinterpret_cast<T*>(work);
     work += align256((int64_t)M * N * sizeof(T));
   }
-  if (db) {
+  if (db && shares > 1) {
     sums = reinterpret_cast<float*>(work);
     work += align256((int64_t)shares * N * 4);
   }
   if (dz || db) {
-    hipLaunchKernelGGL((k_dz<T>), dim3(cdiv(N, 64), shares), dim3(256), 0, stream, d, ldy, static_cast<const T*>(z), dz,
-                       sums, M, N, act, rows);
-    if (db)
-      hipLaunchKernelGGL((k_db<T>), dim3(cdiv(N, 256)), dim3(256), 0, stream, sums, static_cast<T*>(db), N, shares);
+    hipLaunchKernelGGL((k_dz<T>), dim3(cdiv(N, DZ_COLUMNS), shares), dim3(256), 0, stream, d, ldy,
+                       static_cast<const T*>(z), dz, static_cast<T*>(db), sums, M, N, act, rows);
+    if (sums)
+      hipLaunchKernelGGL((k_db<T>), dim3(cdiv(N, 64)), dim3(256), 0, stream, sums, static_cast<T*>(db), N, shares);
   }
   if (dz) d = dz, ldd = N;
   int rc = 0;
