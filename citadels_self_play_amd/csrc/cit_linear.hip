@@ -11,6 +11,8 @@
 // transposed copy is ever written.  Sums are fp32 in the matrix cores'
 // accumulators from the first product to the epilogue; the one rounding to the
 // element type is the store.
+#include <type_traits>
+
 #include "cit_ops.h"
 
 namespace {
@@ -227,7 +229,7 @@ struct Tile {
 
   __device__ static __forceinline__ int swz(int row) {
     if (!KS) return row & 7;
-    return sizeof(T) == 2 ? (row & 3) << 1 : ((row >> 2) & 3) << 2;
+    return (sizeof(T) == 2 ? (row & 3) << 1 : ((row >> 2) & 3) << 2) & (CPR - 1);
   }
   // Byte offset of the 16-byte chunk c of tile row `row`.
   __device__ static __forceinline__ int at(int row, int c) { return (row * CPR + (c ^ swz(row))) << 4; }
@@ -239,11 +241,12 @@ struct Tile {
   }
 };
 
-// A matrix of `rows` x `cols` elements, ld elements apart.
+// A matrix of `rows` x `cols` elements, ld elements apart; of each row `edge`
+// elements may be read (more than cols in a padded copy).
 struct Mat {
   const void* p;
   int64_t ld;
-  int rows, cols;
+  int rows, cols, edge;
 };
 
 // 16 bytes of row r from column c on, zero outside the matrix: any alignment.
@@ -265,24 +268,36 @@ __device__ __forceinline__ u32x4 fetch(const Mat& a, int r, int c) {
   return v.raw;
 }
 
-// Loads of one thread for one tile, through registers (THREADS threads).
-template <typename T, bool KS, int R, int THREADS>
+// Loads of thread `me` of THREADS for one tile, through registers.  DZ: the
+// operand is dy act'(z), made on the way (rounded to the type, as k_dz does).
+template <typename T, bool KS, int R, int THREADS, bool DZ = false>
 struct Stage {
   typedef Tile<T, KS, R> L;
   static constexpr int PER = L::CHUNKS / THREADS;
-  u32x4 v[PER];
-  __device__ __forceinline__ void load(const Mat& a, int r0, int k0) {
+  u32x4 v[PER], u[DZ ? PER : 1];
+  __device__ __forceinline__ void load(const Mat& a, int r0, int k0, int me, const Mat* z = nullptr) {
 #pragma unroll
     for (int i = 0; i < PER; i++) {
       int row, c;
-      L::from(i * THREADS + (int)threadIdx.x, row, c);
-      v[i] = KS ? fetch<T>(a, k0 + row, r0 + c * L::E) : fetch<T>(a, r0 + row, k0 + c * L::E);
+      L::from(i * THREADS + me, row, c);
+      const int y = KS ? k0 + row : r0 + row, x = KS ? r0 + c * L::E : k0 + c * L::E;
+      v[i] = fetch<T>(a, y, x);
+      if (DZ) u[i] = fetch<T>(*z, y, x);
     }
   }
-  __device__ __forceinline__ void store(char* lds) const {
+  __device__ __forceinline__ void store(char* lds, int me, int act = ACT_NONE) const {
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-      *reinterpret_cast<u32x4*>(lds + ((i * THREADS + (int)threadIdx.x) << 4)) = v[i];
+    for (int i = 0; i < PER; i++) {
+      Pack16<T> p;
+      p.raw = v[i];
+      if (DZ) {
+        Pack16<T> q;
+        q.raw = u[i];
+#pragma unroll
+        for (int k = 0; k < L::E; k++) p.e[k] = from_f<T>(to_f(p.e[k]) * act_grad<T>(act, to_f(q.e[k])));
+      }
+      *reinterpret_cast<u32x4*>(lds + ((i * THREADS + me) << 4)) = p.raw;
+    }
   }
 };
 
@@ -366,17 +381,17 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, 
 
   Stage<T, AKS, BM, THREADS> sa;
   Stage<T, BKS, BN, THREADS> sb;
-  sa.load(a, m0, kb);
-  sb.load(b, n0, kb);
-  sa.store(lds[0]);
-  sb.store(lds[0] + BM * 128);
+  sa.load(a, m0, kb, threadIdx.x);
+  sb.load(b, n0, kb, threadIdx.x);
+  sa.store(lds[0], threadIdx.x);
+  sb.store(lds[0] + BM * 128, threadIdx.x);
   __syncthreads();
   int cur = 0;
   for (int k = kb; k < ke; k += BK<T>) {
     const bool more = k + BK<T> < ke;
     if (more) {
-      sa.load(a, m0, k + BK<T>);
-      sb.load(b, n0, k + BK<T>);
+      sa.load(a, m0, k + BK<T>, threadIdx.x);
+      sb.load(b, n0, k + BK<T>, threadIdx.x);
     }
     const char* la = lds[cur];
     const char* lb = lds[cur] + BM * 128;
@@ -393,8 +408,8 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, 
         for (int j = 0; j < TN; j++) acc[i][j] = mma(fb[j], fa[i], acc[i][j], T{});
     }
     if (more) {
-      sa.store(lds[cur ^ 1]);
-      sb.store(lds[cur ^ 1] + BM * 128);
+      sa.store(lds[cur ^ 1], threadIdx.x);
+      sb.store(lds[cur ^ 1] + BM * 128, threadIdx.x);
     }
     __syncthreads();
     cur ^= 1;
@@ -412,13 +427,17 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, 
 // instructions.  The chunk permutation of Tile is applied to the address each
 // lane reads, since a wave's 64 chunks land side by side.
 //
-// Two tiles of LDS, two k steps a tile, and two sets of fragments, so that the
-// matrix cores never wait for a load that was asked for in the same step:
+// STAGES tiles of LDS, all but one of them under way while the last is worked
+// on, two k steps a tile, and (AHEAD) two sets of fragments, so that the matrix
+// cores never wait for a load that was asked for in the same step:
 //
 //   read step 1 of tile t      multiply step 0 of tile t
 //   --- tile t + 1 has arrived, every wave has read tile t ---
-//   ask for tile t + 2 in tile t's place
+//   ask for tile t + STAGES in tile t's place
 //   read step 0 of tile t + 1  multiply step 1 of tile t
+//
+// A tile takes about 0.9 us to arrive and a 64 x 64 one 0.1 us to multiply:
+// where there are not enough workgroups to hide that, four stages do.
 
 typedef const __attribute__((address_space(1))) void* global_ptr;
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -441,7 +460,7 @@ struct Direct {
       int64_t at;
       if (KS) {
         int col = r0 + c * L::E;
-        if (col + L::E > a.cols) col = a.cols - L::E;
+        if (col + L::E > a.edge) col = a.edge - L::E;
         at = row * a.ld + (col - r0);
       } else {
         int r = row;
@@ -475,14 +494,26 @@ __device__ __forceinline__ void place(int b, int n, int tiles_m, int tiles_n, in
   tn = (t - g * wide) / rows;
 }
 
-template <typename T, bool AKS, bool BKS, int BM, int BN, int WM, int WN, bool AHEAD>
+// Until all but N of this wave's loads to LDS have landed and its reads of LDS
+// are done, then until every wave is here.  (A plain barrier would wait for all
+// loads, the ones for later tiles too.)
+template <int N>
+__device__ __forceinline__ void arrive() {
+  static_assert(N < 64, "the counter's field");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);      // lgkmcnt 0; the builtin, since the compiler counts along
+  asm volatile("s_barrier" ::: "memory");
+}
+
+template <typename T, bool AKS, bool BKS, int BM, int BN, int WM, int WN, int STAGES, bool AHEAD>
 __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilogue e, int M, int N, int K, int tiles_m,
                                                              int tiles_n, int k_per_split) {
   constexpr int THREADS = WM * WN * 64;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int STEPS = 2;
-  // four arrays, not one: the compiler then sees that a load under way into one does not concern reads of another
-  __shared__ __attribute__((aligned(16))) char a0[BM * 128], b0[BN * 128], a1[BM * 128], b1[BN * 128];
+  constexpr int STEPS = 2, BYTES = (BM + BN) * 128;
+  // an array a stage, not one: the compiler then sees that loads under way into one do not concern reads of another
+  __shared__ __attribute__((aligned(16))) char s0[BYTES], s1[BYTES], s2[STAGES > 2 ? BYTES : 16],
+      s3[STAGES > 3 ? BYTES : 16];
 
   int tm, tn;
   place(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
@@ -499,54 +530,74 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilo
 
   Direct<T, AKS, BM, THREADS> da;
   Direct<T, BKS, BN, THREADS> db;
+  constexpr int LOADS = decltype(da)::PER + decltype(db)::PER;         // a tile's, for each wave
   da.start(A, m0, kb);
   db.start(B, n0, kb);
-  auto ask = [&](int t, char* la, char* lb) {
+  auto ask = [&](int t, char* to) __attribute__((always_inline)) {
     if (t < whole) {
-      da.next(la);
-      db.next(lb);
+      da.next(to);
+      db.next(to + BM * 128);
     }
   };
   u32x4 fa[AHEAD ? 2 : 1][TM], fb[AHEAD ? 2 : 1][TN];
-  auto read = [&](int s, const char* la, const char* lb) {
+  auto read = [&](int s, const char* from) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < TM; i++) fa[AHEAD ? s : 0][i] = frag<T, AKS, BM>(la, wm + i * 16, s);
+    for (int i = 0; i < TM; i++) fa[AHEAD ? s : 0][i] = frag<T, AKS, BM>(from, wm + i * 16, s);
 #pragma unroll
-    for (int j = 0; j < TN; j++) fb[AHEAD ? s : 0][j] = frag<T, BKS, BN>(lb, wn + j * 16, s);
+    for (int j = 0; j < TN; j++) fb[AHEAD ? s : 0][j] = frag<T, BKS, BN>(from + BM * 128, wn + j * 16, s);
   };
-  auto multiply = [&](int s) {
+  auto multiply = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < TM; i++)
 #pragma unroll
-      for (int j = 0; j < TN; j++) acc[i][j] = mma(fb[AHEAD ? s : 0][j], fa[AHEAD ? s : 0][i], acc[i][j], T{});
+      for (int j = 0; j < TN; j++)
+        acc[i][j] = mma(fb[AHEAD ? s : 0][j], fa[AHEAD ? s : 0][i], acc[i][j], T{});
   };
-  auto tile = [&](int t, char* la, char* lb, char* na, char* nb) {
+  // tile t in `here`, the one after it in `next`; `steady`: there is a tile t + STAGES
+  auto tile = [&](auto steady, int t, char* here, char* next) __attribute__((always_inline)) {
     if (AHEAD) {
-      read(1, la, lb);
+      read(1, here);
       multiply(0);
-      __syncthreads();
-      ask(t + 2, la, lb);
-      if (t + 1 < whole) read(0, na, nb);
+      // tiles t + 1 .. t + STAGES - 1 are under way, near the end fewer
+      if (STAGES == 2) __syncthreads();
+      else if (steady.value || t + STAGES <= whole) arrive<(STAGES - 2) * LOADS>();
+      else arrive<0>();
+      if (steady.value || t + STAGES < whole) {
+        da.next(here);
+        db.next(here + BM * 128);
+      }
+      if (steady.value || t + 1 < whole) read(0, next);
       multiply(1);
     } else {
-      ask(t + 1, na, nb);
-      read(0, la, lb);
+      static_assert(AHEAD || STAGES == 2, "one tile ahead");
+      ask(t + 1, next);
+      read(0, here);
       multiply(0);
-      read(1, la, lb);
+      read(1, here);
       multiply(1);
       __syncthreads();
     }
   };
-  ask(0, a0, b0);
-  __syncthreads();
+  auto round = [&](auto steady, int t) __attribute__((always_inline)) {
+    tile(steady, t, s0, s1);
+    if (steady.value || t + 1 < whole) tile(steady, t + 1, s1, STAGES == 2 ? s0 : s2);
+    if (STAGES > 2 && (steady.value || t + 2 < whole)) tile(steady, t + 2, s2, STAGES == 3 ? s0 : s3);
+    if (STAGES > 3 && (steady.value || t + 3 < whole)) tile(steady, t + 3, s3, s0);
+  };
+  ask(0, s0);
   if (AHEAD) {
-    ask(1, a1, b1);
-    if (whole) read(0, a0, b0);
+    ask(1, s1);
+    if (STAGES > 2) ask(2, s2);
+    if (STAGES > 3) ask(3, s3);
+    if (whole >= STAGES) arrive<(STAGES - 1) * LOADS>();
+    else arrive<0>();
+    if (whole) read(0, s0);
+  } else {
+    __syncthreads();
   }
-  for (int t = 0; t < whole; t += 2) {
-    tile(t, a0, b0, a1, b1);
-    if (t + 1 < whole) tile(t + 1, a1, b1, a0, b0);
-  }
+  int t = 0;
+  for (; STAGES > 2 && t + 2 * STAGES <= whole; t += STAGES) round(std::true_type{}, t);    // without a branch
+  for (; t < whole; t += STAGES) round(std::false_type{}, t);
   if (kb + whole * BK<T> < ke) {
     // the reduction ends inside a tile: that one through registers, zeros behind the end
     Mat a = A, b = B;
@@ -555,27 +606,162 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilo
     __syncthreads();
     {
       Stage<T, AKS, BM, THREADS> sa;
-      sa.load(a, m0, kb + whole * BK<T>);
-      sa.store(a0);
+      sa.load(a, m0, kb + whole * BK<T>, threadIdx.x);
+      sa.store(s0, threadIdx.x);
     }
     {
       Stage<T, BKS, BN, THREADS> sb;
-      sb.load(b, n0, kb + whole * BK<T>);
-      sb.store(b0);
+      sb.load(b, n0, kb + whole * BK<T>, threadIdx.x);
+      sb.store(s0 + BM * 128, threadIdx.x);
     }
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < STEPS; s++) {
-      read(s, a0, b0);
+      read(s, s0);
       multiply(s);
     }
   }
 
   __syncthreads();
-  static_assert(BM == BN && WM * WN % 4 == 0, "the waves share the four arrays evenly");
-  constexpr int EACH = WM * WN / 4, SHARE = BM * 128 / EACH;
-  char* mine = w / EACH == 0 ? a0 : w / EACH == 1 ? b0 : w / EACH == 2 ? a1 : b1;
+  static_assert(WM * WN % 2 == 0, "the waves share two stages evenly");
+  constexpr int EACH = WM * WN / 2, SHARE = BYTES / EACH;
+  char* mine = w < EACH ? s0 : s1;
   write_out<T, TM, TN, SHARE>(e, acc, mine + (w % EACH) * SHARE, m0 + wm, n0 + wn, M, N, split);
+}
+
+// ---- few outputs --------------------------------------------------------------------
+//
+// 32 x 32 outputs by 8 waves that share out the reduction, k tile by k tile:
+// each wave stages its own tiles in its own 8 KB of LDS (no barrier until the
+// end), and the 8 partial sums meet in LDS in the waves' order.  For layers too
+// small to fill the chip with larger tiles, and for a few rows against a wide
+// weight, whose bytes are then what there is to do.
+
+#define SMALL_WAVES 8
+#define SMALL_LDS (SMALL_WAVES * 64 * 128)
+
+template <typename T, bool AKS, bool BKS, bool DZ>
+__device__ __forceinline__ void small_tile(const Mat& A, const Mat* Z, const Mat& B, const Epilogue& e, int act, int M, int N, int K,
+                           int m0, int n0, int split, int k_per_split, char* lds) {
+  const int kb = split * k_per_split, ke = min(K, kb + k_per_split);
+  Mat a = A, b = B;
+  if (AKS) a.rows = ke; else a.cols = ke;
+  if (BKS) b.rows = ke; else b.cols = ke;
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  char* la = lds + w * (64 * 128);
+  char* lb = la + 32 * 128;
+  f32x4 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 4; i++) acc[i >> 1][i & 1] = f32x4{0, 0, 0, 0};
+  Stage<T, AKS, 32, 64, DZ> sa;
+  Stage<T, BKS, 32, 64> sb;
+  int k = kb + w * BK<T>;
+  if (k < ke) {
+    sa.load(a, m0, k, l, Z);
+    sb.load(b, n0, k, l);
+  }
+  for (; k < ke; k += SMALL_WAVES * BK<T>) {
+    sa.store(la, l, act);
+    sb.store(lb, l);
+    if (k + SMALL_WAVES * BK<T> < ke) {
+      sa.load(a, m0, k + SMALL_WAVES * BK<T>, l, Z);
+      sb.load(b, n0, k + SMALL_WAVES * BK<T>, l);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      u32x4 fa[2], fb[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        fa[i] = frag<T, AKS, 32>(la, i * 16, s);
+        fb[i] = frag<T, BKS, 32>(lb, i * 16, s);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[i >> 1][i & 1] = mma(fb[i & 1], fa[i >> 1], acc[i >> 1][i & 1], T{});
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  // [wave][row][chunk of 4 columns, permuted by the row]
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int r = i * 16 + (l & 15), c = j * 4 + (l >> 4);
+      *reinterpret_cast<f32x4*>(la + r * 128 + ((c ^ (r & 7)) << 4)) = acc[i][j];
+    }
+  __syncthreads();
+  if (threadIdx.x >= 128) return;
+  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 2, m = m0 + r, n = n0 + c * 4;
+  if (m >= M || n >= N) return;
+  f32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < SMALL_WAVES; i++) {
+    const char* p = lds + i * (64 * 128) + r * 128;
+    lo += *reinterpret_cast<const f32x4*>(p + ((c ^ (r & 7)) << 4));
+    hi += *reinterpret_cast<const f32x4*>(p + (((c + 1) ^ (r & 7)) << 4));
+  }
+  float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  finish8<T>(e, m, n, N, v, split, M);
+}
+
+template <typename T, bool AKS, bool BKS>
+__global__ __launch_bounds__(SMALL_WAVES * 64, 4) void k_gemm_small(Mat A, Mat B, Epilogue e, int M, int N, int K,
+                                                                 int tiles_n, int k_per_split) {
+  __shared__ __attribute__((aligned(16))) char lds[SMALL_LDS];
+  const int tile = blockIdx.x;
+  small_tile<T, AKS, BKS, false>(A, nullptr, B, e, ACT_NONE, M, N, K, tile / tiles_n * 32, tile % tiles_n * 32,
+                                 blockIdx.y, k_per_split, lds);
+}
+
+// A small layer's whole backward pass in one launch: workgroups for the tiles of
+// dx, then those of dw, then 16 columns each of db; dz is made from dy and z
+// wherever it is read.
+template <typename T>
+__global__ __launch_bounds__(SMALL_WAVES * 64, 4) void k_backward_small(Mat dy, Mat z, Mat x, Mat w, T* dx, T* dw, T* db,
+                                                                     int act, int M, int N, int K, int dx_tiles,
+                                                                     int dw_tiles) {
+  __shared__ __attribute__((aligned(16))) char lds[SMALL_LDS];
+  const int tiles_k = (K + 31) / 32;
+  int b = blockIdx.x;
+  Epilogue e = {};
+  e.ldo = K;
+  if (b < dx_tiles) {
+    e.out = dx;
+    const int m0 = b / tiles_k * 32, n0 = b % tiles_k * 32;
+    if (act == ACT_NONE) small_tile<T, false, true, false>(dy, &z, w, e, act, M, K, N, m0, n0, 0, N, lds);
+    else small_tile<T, false, true, true>(dy, &z, w, e, act, M, K, N, m0, n0, 0, N, lds);
+    return;
+  }
+  b -= dx_tiles;
+  if (b < dw_tiles) {
+    e.out = dw;
+    const int m0 = b / tiles_k * 32, n0 = b % tiles_k * 32;
+    if (act == ACT_NONE) small_tile<T, true, true, false>(dy, &z, x, e, act, N, K, M, m0, n0, 0, M, lds);
+    else small_tile<T, true, true, true>(dy, &z, x, e, act, N, K, M, m0, n0, 0, M, lds);
+    return;
+  }
+  b -= dw_tiles;
+  // 32 rows of 16 columns at a time, then 32 partial sums a column
+  const int c = threadIdx.x & 15, y = threadIdx.x >> 4, n = b * 16 + c;
+  float s = 0.0f;
+  if (n < N)
+    for (int m = y; m < M; m += SMALL_WAVES * 4) {
+      float v = to_f(static_cast<const T*>(dy.p)[m * dy.ld + n]);
+      if (act != ACT_NONE) v *= act_grad<T>(act, to_f(static_cast<const T*>(z.p)[m * z.ld + n]));
+      s += v;
+    }
+  float* sums = reinterpret_cast<float*>(lds);
+  sums[y * 16 + c] = s;
+  __syncthreads();
+  if (y || n >= N) return;
+  float t = 0.0f;
+#pragma unroll
+  for (int i = 0; i < SMALL_WAVES * 4; i++) t += sums[i * 16 + c];
+  db[n] = from_f<T>(t);
 }
 
 // The splits' sums in their order, then the epilogue.
@@ -600,8 +786,8 @@ __global__ __launch_bounds__(256) void k_join(Epilogue e, int64_t M, int N, int 
 #define DZ_COLUMNS 128
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_dz(const T* dy, int64_t ldy, const T* z, T* dz, T* db, float* part, int M,
-                                            int N, int act, int rows_per) {
+__global__ __launch_bounds__(256) void k_dz(const T* dy, int64_t ldy, const T* z, T* dz, int64_t ldd, T* db, float* part,
+                                            int M, int N, int act, int rows_per) {
   __shared__ float sums[16][DZ_COLUMNS + 4];
   const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
   const int n = blockIdx.x * DZ_COLUMNS + x * 8;
@@ -623,7 +809,7 @@ __global__ __launch_bounds__(256) void k_dz(const T* dy, int64_t ldy, const T* z
         T o[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) o[i] = from_f<T>(v[i]);
-        store8<T>(dz + (int64_t)m * N + n, o);
+        store8<T>(dz + m * ldd + n, o);
       }
     }
   } else {
@@ -634,7 +820,7 @@ __global__ __launch_bounds__(256) void k_dz(const T* dy, int64_t ldy, const T* z
           float v = to_f(dy[m * ldy + n + i]);
           if (act != ACT_NONE) v *= act_grad<T>(act, to_f(z[(int64_t)m * N + n + i]));
           s[i] += v;
-          if (dz) dz[(int64_t)m * N + n + i] = from_f<T>(v);
+          if (dz) dz[m * ldd + n + i] = from_f<T>(v);
         }
   }
   if (!db && !part) return;
@@ -663,82 +849,124 @@ __global__ __launch_bounds__(256) void k_db(const float* part, T* db, int N, int
   if (w == 0 && n < N) db[n] = from_f<T>((sums[0][x] + sums[1][x]) + (sums[2][x] + sums[3][x]));
 }
 
+// ---- padded copies -----------------------------------------------------------------
+//
+// Rows that do not start on 16 bytes cost the tile kernel guarded loads through
+// registers.  The backward products, which read them down the rows, are
+// faster over copies with padded rows (bf16 3000 x 1001 x 999: dw 95 -> 42 us);
+// the forward product is not (22 us, 29 with copies).
+
+struct Copies {
+  Mat from[2];
+  void* to[2];
+  int64_t ld[2];                 // of the copies, a whole number of chunks
+};
+
+// A wave a row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_pack(Copies c) {
+  constexpr int E = 16 / sizeof(T);
+  const int64_t all = (int64_t)c.from[0].rows + c.from[1].rows;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < all; r += (int64_t)gridDim.x * 4) {
+    const int w = r >= c.from[0].rows;
+    const int row = (int)(w ? r - c.from[0].rows : r);
+    T* to = static_cast<T*>(c.to[w]) + row * c.ld[w];
+#pragma unroll 2
+    for (int at = (threadIdx.x & 63) * E; at < c.ld[w]; at += 64 * E)
+      *reinterpret_cast<u32x4*>(to + at) = fetch<T>(c.from[w], row, at);
+  }
+}
+
 // ---- host side ---------------------------------------------------------------------
 
 int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 struct Plan {
-  int tiles_m, tiles_n, splits, k_per;
+  int tile, tiles_m, tiles_n, splits, k_per;
+  bool deep;                     // four stages instead of two
 };
 
-Plan plan_tiles(int M, int N, int K, int bm, int bn, int bk) {
+int elt(int dtype) { return dtype == CIT_FP32 ? 4 : 2; }
+
+enum { TILE_32, TILE_64, TILE_128, TILE_256 };
+
+// Outputs for 32 x 32 tiles: a few rows or columns, or less than a 64 x 64 tile for each compute unit.  Measured,
+// forward, 32 against 64: bf16 1 x 4096 x 16384 34 / 46 us, 512 x 1024 x 1024 6.7 / 7.8, 2048 x 512 x 512 8.4 / 5.6
+// (that one has 256 tiles); fp32 1 x 4096 x 16384 68 / 262 us, 512 x 1024 x 1024 17 / 21, 2048 x 512 x 512 19 / 14.
+bool small(int M, int N) { return M <= 32 || N <= 32 || (int64_t)cdiv(M, 64) * cdiv(N, 64) < 256; }
+
+// The tile of a product whose operands take direct loads: the largest of which there are enough (a tile's loads
+// are what the L2s deliver, about 10 TB/s, and fall with its side).  Measured, 64 / 128 / 256, us:
+// bf16 M x N x K 8192 x 4096 x 4096 380 / 264 / 232; 4096 x 4096 x 2048 (256 of 256) 104 / 70 / 60;
+// 4096 x 2048 x 4096 (128 of 256, 512 of 128) 92 / 62 / 92; 2048^3 (256 of 128) 29 / 24;
+// 3000 x 999 x 1001 (192 of 128) 29 / 33; fp32 2048^3 137 / 134, 3000 x 999 x 1001 71 / 92.
+int direct_tile(int M, int N, int es) {
+  if (es == 2 && (int64_t)cdiv(M, 256) * cdiv(N, 256) >= 192) return TILE_256;
+  if ((int64_t)cdiv(M, 128) * cdiv(N, 128) >= 208) return TILE_128;
+  return TILE_64;
+}
+
+Plan plan(int M, int N, int K, int es, bool aligned) {
   Plan p;
-  p.tiles_m = cdiv(M, bm);
-  p.tiles_n = cdiv(N, bn);
+  p.tile = small(M, N) ? TILE_32 : aligned ? direct_tile(M, N, es) : TILE_64;
+  const int t = 32 << p.tile, bk = 128 / es, kt = cdiv(K, bk);
+  p.tiles_m = cdiv(M, t);
+  p.tiles_n = cdiv(N, t);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  // fewer tiles than half the compute units: the reduction is shared out too, in shares of at least 4 k tiles
-  int want = tiles < 128 ? (int)(256 / tiles) : 1;
-  const int kt = cdiv(K, bk);
-  want = want < kt / 4 ? want : kt / 4;
+  p.deep = p.tile == TILE_128 && tiles <= 256;   // one workgroup on a compute unit: 2048^3 bf16 31 -> 25 us
+  int want = 1;
+  // A few small tiles over a long reduction: the launch shares it out too, at least 4 k tiles for each wave (fp32
+  // 4096 x 418 x 512: dw 39 -> 34 us).
+  if (p.tile == TILE_32 && tiles < 256) {
+    want = (int)(512 / tiles);
+    if (want > kt / (SMALL_WAVES * 4)) want = kt / (SMALL_WAVES * 4);
+  }
   if (want < 1) want = 1;
   p.k_per = cdiv(kt, want) * bk;
   p.splits = K > 0 ? cdiv(K, p.k_per) : 1;
   return p;
 }
-
-int elt(int dtype) { return dtype == CIT_FP32 ? 4 : 2; }
-
-enum { TILE_64, TILE_128, TILE_256 };
-
-// The tile of a product of aligned operands.
-int tile_of(int M, int N, int es) {
-  if (es == 2 && (int64_t)cdiv(M, 256) * cdiv(N, 256) >= 128) return TILE_256;
-  if ((int64_t)cdiv(M, 128) * cdiv(N, 128) >= 128) return TILE_128;
-  return TILE_64;
-}
-Plan plan_of(int tile, int M, int N, int K, int bk) {
-  const int t = tile == TILE_256 ? 256 : tile == TILE_128 ? 128 : 64;
-  return plan_tiles(M, N, K, t, t, bk);
+int64_t split_bytes(int M, int N, int K, int es) {
+  if (!small(M, N)) return 0;
+  const Plan p = plan(M, N, K, es, false);
+  return p.splits > 1 ? align256((int64_t)p.splits * M * N * 4) : 0;
 }
 
-// Room for split sums, whatever the operands' alignment makes of the tile.
-int64_t product_work(int M, int N, int K, int dtype) {
-  if (M <= 0 || N <= 0) return 0;
-  int64_t most = 0;
-  for (int tile : {(int)TILE_64, tile_of(M, N, elt(dtype))}) {
-    const Plan p = plan_of(tile, M, N, K, 128 / elt(dtype));
-    if (p.splits > 1 && p.splits > most) most = p.splits;
-  }
-  return align256(most * M * N * 4);
+bool aligned(const void* p, int64_t ld, int es) {
+  // 31 bits reach a tile's rows from its first
+  return !((uintptr_t)p & 15) && (ld * es) % 16 == 0 && ld * es < 1 << 23;
 }
+bool direct(const Mat& a, bool ks, int es) { return aligned(a.p, a.ld, es) && (!ks || a.edge % (16 / es) == 0); }
 
-template <typename T>
-bool direct(const Mat& a, bool ks) {
-  if (((uintptr_t)a.p & 15) || (a.ld * (int64_t)sizeof(T)) % 16) return false;
-  if (a.ld * (int64_t)sizeof(T) >= 1 << 23) return false;             // a tile's rows within 31 bits of its first
-  return !ks || a.cols % (16 / (int)sizeof(T)) == 0;
-}
+int64_t padded(int cols, int es) { return ((int64_t)cols * es + 15) / 16 * 16 / es; }
 
-template <typename T, bool AKS, bool BKS, int TILE, int WM, int WN, bool AHEAD>
+// Whether the backward pass copies unaligned operands of an M x N x K product first.
+bool worth_copies(int M, int N, int K) { return !small(M, N) && K >= 256; }
+
+template <typename T, bool AKS, bool BKS, int TILE, int WM, int WN, int STAGES, bool AHEAD>
 void launch_direct(const Mat& A, const Mat& B, const Epilogue& e, int M, int N, int K, const Plan& p,
                    hipStream_t stream) {
-  hipLaunchKernelGGL((k_gemm_direct<T, AKS, BKS, TILE, TILE, WM, WN, AHEAD>), dim3(p.tiles_m * p.tiles_n, p.splits),
+  hipLaunchKernelGGL((k_gemm_direct<T, AKS, BKS, TILE, TILE, WM, WN, STAGES, AHEAD>), dim3(p.tiles_m * p.tiles_n, p.splits),
                      dim3(WM * WN * 64), 0, stream, A, B, e, M, N, K, p.tiles_m, p.tiles_n, p.k_per);
 }
 
 template <typename T, bool AKS, bool BKS>
 int product(Mat A, Mat B, Epilogue e, int M, int N, int K, void* work, hipStream_t stream) {
-  const bool d = K > 0 && direct<T>(A, AKS) && direct<T>(B, BKS);
-  const int tile = d ? tile_of(M, N, sizeof(T)) : TILE_64;
-  const Plan p = plan_of(tile, M, N, K, BK<T>);
+  const bool d = K > 0 && direct(A, AKS, sizeof(T)) && direct(B, BKS, sizeof(T));
+  const Plan p = plan(M, N, K, sizeof(T), d);
+  const dim3 grid(p.tiles_m * p.tiles_n, p.splits);
   if (p.splits > 1) e.part = static_cast<float*>(work);
-  if (!d)
-    hipLaunchKernelGGL((k_gemm<T, AKS, BKS, 64, 64, 2, 2>), dim3(p.tiles_m * p.tiles_n, p.splits), dim3(256), 0, stream,
-                       A, B, e, M, N, K, p.tiles_n, p.k_per);
-  else if (tile == TILE_64) launch_direct<T, AKS, BKS, 64, 2, 2, true>(A, B, e, M, N, K, p, stream);
-  else if (tile == TILE_128) launch_direct<T, AKS, BKS, 128, 2, 2, true>(A, B, e, M, N, K, p, stream);
-  else if constexpr (sizeof(T) == 2) launch_direct<T, AKS, BKS, 256, 2, 4, false>(A, B, e, M, N, K, p, stream);
+  if (p.tile == TILE_32)
+    hipLaunchKernelGGL((k_gemm_small<T, AKS, BKS>), grid, dim3(SMALL_WAVES * 64), 0, stream, A, B, e, M, N, K,
+                       p.tiles_n, p.k_per);
+  else if (!d)
+    hipLaunchKernelGGL((k_gemm<T, AKS, BKS, 64, 64, 2, 2>), grid, dim3(256), 0, stream, A, B, e, M, N, K, p.tiles_n,
+                       p.k_per);
+  else if (p.tile == TILE_64) launch_direct<T, AKS, BKS, 64, 2, 2, 2, true>(A, B, e, M, N, K, p, stream);
+  else if (p.tile == TILE_128 && p.deep) launch_direct<T, AKS, BKS, 128, 2, 2, 4, true>(A, B, e, M, N, K, p, stream);
+  else if (p.tile == TILE_128) launch_direct<T, AKS, BKS, 128, 2, 2, 2, true>(A, B, e, M, N, K, p, stream);
+  else if constexpr (sizeof(T) == 2) launch_direct<T, AKS, BKS, 256, 2, 4, 2, false>(A, B, e, M, N, K, p, stream);
   if (p.splits > 1) {
     const int64_t blocks = ((int64_t)M * N + 255) / 256;
     hipLaunchKernelGGL((k_join<T>), dim3(blocks < 4096 ? (unsigned)blocks : 4096), dim3(256), 0, stream, e, (int64_t)M,
@@ -756,47 +984,93 @@ int dz_rows(int M, int N) {
   return cdiv(cdiv(M, shares), 16) * 16;
 }
 
+// Whether the backward pass goes in one launch: both products small and neither reduction long (db's column sums
+// walk M rows, 32 at a time).  fp32 64 x 418 x 512: 14 us in one, 25 in five; 2048 x 512 x 256: 63 in one, 39 in five.
+bool one_launch(int M, int N, int K) { return K > 0 && small(M, K) && small(N, K) && M <= 512 && N <= 4096; }
+
+// The pieces of a workspace, in their order; bytes 0: not needed.
+struct Layout {
+  int64_t copy[2], dz, sums, split;
+  int64_t bytes() const { return copy[0] + copy[1] + dz + sums + split; }
+};
+
+Layout backward_layout(const void* x, int64_t ldx, const void* w, int64_t ldw, bool dx, bool dw, bool db, int M, int N,
+                       int K, int es, int act) {
+  Layout l = {};
+  if (M <= 0 || N <= 0 || one_launch(M, N, K)) return l;
+  if (K <= 0) dx = dw = false;
+  // dz in rows of its own; where there is no activation dy stands for it, unless its rows are off 16 bytes, which
+  // the size alone decides here
+  const bool big_x = dx && worth_copies(M, K, N), big_w = dw && worth_copies(N, K, M);
+  const bool odd = padded(N, es) != N;
+  if ((dx || dw) && (act != ACT_NONE || (odd && (big_x || big_w)))) l.dz = align256(M * padded(N, es) * es);
+  // the products' other operands are read down their rows: their width has to be whole chunks too
+  const bool odd_k = padded(K, es) != K;
+  if (big_w && (!aligned(x, ldx, es) || odd_k)) l.copy[0] = align256(M * padded(K, es) * es);
+  if (big_x && (!aligned(w, ldw, es) || odd_k)) l.copy[1] = align256(N * padded(K, es) * es);
+  if (db && cdiv(M, dz_rows(M, N)) > 1) l.sums = align256((int64_t)cdiv(M, dz_rows(M, N)) * N * 4);
+  const int64_t a = dx ? split_bytes(M, K, N, es) : 0, b = dw ? split_bytes(N, K, M, es) : 0;
+  l.split = a > b ? a : b;
+  return l;
+}
+
+// The copies a layout asks for, at `work`; x and w become them.
 template <typename T>
-int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const Epilogue& e, int M, int N, int K, void* work,
-            hipStream_t stream) {
-  return product<T, false, false>(Mat{x, ldx, M, K}, Mat{w, ldw, N, K}, e, M, N, K, work, stream);
+void make_copies(const Layout& l, Mat& x, Mat& w, char* work, hipStream_t stream) {
+  if (!l.copy[0] && !l.copy[1]) return;
+  Copies c = {};
+  for (int i = 0; i < 2; i++) {
+    Mat& m = i ? w : x;
+    if (!l.copy[i]) continue;
+    c.from[i] = m;
+    c.to[i] = work + (i ? l.copy[0] : 0);
+    c.ld[i] = padded(m.cols, sizeof(T));
+    m = Mat{c.to[i], c.ld[i], m.rows, m.cols, (int)c.ld[i]};
+  }
+  const int64_t blocks = ((int64_t)c.from[0].rows + c.from[1].rows + 3) / 4;
+  hipLaunchKernelGGL((k_pack<T>), dim3(blocks < 4096 ? (unsigned)blocks : 4096), dim3(256), 0, stream, c);
 }
 
 template <typename T>
-int backward(const void* dy, int64_t ldy, const void* z, const void* x, int64_t ldx, const void* w, int64_t ldw,
-             void* dx, void* dw, void* db, int M, int N, int K, int act, char* work, hipStream_t stream) {
-  const T* d = static_cast<const T*>(dy);
-  int64_t ldd = ldy;
-  const int rows = dz_rows(M, N), shares = cdiv(M, rows);
-  T* dz = nullptr;
-  float* sums = nullptr;
-  if (act != ACT_NONE && (dx || dw)) {
-    dz = reinterpret_cast<T*>(work);
-    work += align256((int64_t)M * N * sizeof(T));
+int backward(Mat dy, const void* z, Mat x, Mat w, void* dx, void* dw, void* db, int M, int N, int K, int act,
+             char* work, hipStream_t stream) {
+  if (one_launch(M, N, K)) {
+    const int dx_tiles = dx ? cdiv(M, 32) * cdiv(K, 32) : 0, dw_tiles = dw ? cdiv(N, 32) * cdiv(K, 32) : 0;
+    const int sums = db ? cdiv(N, 16) : 0;
+    if (dx_tiles + dw_tiles + sums)
+      hipLaunchKernelGGL((k_backward_small<T>), dim3(dx_tiles + dw_tiles + sums), dim3(SMALL_WAVES * 64), 0, stream, dy,
+                         Mat{z, N, M, N, N}, x, w, static_cast<T*>(dx), static_cast<T*>(dw), static_cast<T*>(db), act,
+                         M, N, K, dx_tiles, dw_tiles);
+    return launch_status();
   }
-  if (db && shares > 1) {
-    sums = reinterpret_cast<float*>(work);
-    work += align256((int64_t)shares * N * 4);
-  }
+  const Layout l =
+      backward_layout(x.p, x.ld, w.p, w.ld, dx != nullptr, dw != nullptr, db != nullptr, M, N, K, sizeof(T), act);
+  make_copies<T>(l, x, w, work, stream);
+  work += l.copy[0] + l.copy[1];
+  T* dz = l.dz ? reinterpret_cast<T*>(work) : nullptr;
+  float* sums = l.sums ? reinterpret_cast<float*>(work + l.dz) : nullptr;
+  const int64_t ldd = padded(N, sizeof(T));
+  const int rows = dz_rows(M, N);
   if (dz || db) {
-    hipLaunchKernelGGL((k_dz<T>), dim3(cdiv(N, DZ_COLUMNS), shares), dim3(256), 0, stream, d, ldy,
-                       static_cast<const T*>(z), dz, static_cast<T*>(db), sums, M, N, act, rows);
+    hipLaunchKernelGGL((k_dz<T>), dim3(cdiv(N, DZ_COLUMNS), cdiv(M, rows)), dim3(256), 0, stream,
+                       static_cast<const T*>(dy.p), dy.ld, static_cast<const T*>(z), dz, ldd, static_cast<T*>(db), sums,
+                       M, N, act, rows);
     if (sums)
-      hipLaunchKernelGGL((k_db<T>), dim3(cdiv(N, 64)), dim3(256), 0, stream, sums, static_cast<T*>(db), N, shares);
+      hipLaunchKernelGGL((k_db<T>), dim3(cdiv(N, 64)), dim3(256), 0, stream, sums, static_cast<T*>(db), N,
+                         cdiv(M, rows));
   }
-  if (dz) d = dz, ldd = N;
+  if (dz) dy = Mat{dz, ldd, M, N, (int)ldd};
+  work += l.dz + l.sums;
   int rc = 0;
+  Epilogue e = {};
+  e.ldo = K;
   if (dx && K > 0) {
-    Epilogue e = {};
     e.out = dx;
-    e.ldo = K;
-    rc = product<T, false, true>(Mat{d, ldd, M, N}, Mat{w, ldw, N, K}, e, M, K, N, work, stream);
+    rc = product<T, false, true>(dy, w, e, M, K, N, work, stream);
   }
   if (!rc && dw && K > 0) {
-    Epilogue e = {};
     e.out = dw;
-    e.ldo = K;
-    rc = product<T, true, true>(Mat{d, ldd, M, N}, Mat{x, ldx, M, K}, e, N, K, M, work, stream);
+    rc = product<T, true, true>(dy, x, e, N, K, M, work, stream);
   }
   return rc ? rc : launch_status();
 }
@@ -808,14 +1082,15 @@ bool bad_types(int dtype, int act) { return dtype < CIT_FP32 || dtype > CIT_FP16
 extern "C" {
 
 size_t cit_linear_forward_work_bytes(int M, int N, int K, int dtype) {
-  return bad_types(dtype, 0) ? 0 : (size_t)product_work(M, N, K, dtype);
+  return bad_types(dtype, 0) || M <= 0 || N <= 0 || K <= 0 ? 0 : (size_t)split_bytes(M, N, K, elt(dtype));
 }
 
-size_t cit_linear_backward_work_bytes(int M, int N, int K, int dtype, int act) {
-  if (bad_types(dtype, act) || M <= 0 || N <= 0 || K < 0) return 0;
-  const int64_t a = product_work(M, K, N, dtype), b = product_work(N, K, M, dtype);
-  const int64_t dz = act != ACT_NONE ? align256((int64_t)M * N * elt(dtype)) : 0;
-  return (size_t)(dz + align256((int64_t)cdiv(M, dz_rows(M, N)) * N * 4) + (a > b ? a : b));
+size_t cit_linear_backward_work_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* dx,
+                                      const void* dw, const void* db, int M, int N, int K, int dtype, int act) {
+  return bad_types(dtype, act) ? 0
+                               : (size_t)backward_layout(x, ldx, w, ldw, dx != nullptr, dw != nullptr, db != nullptr, M,
+                                                         N, K, elt(dtype), act)
+                                     .bytes();
 }
 
 int cit_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
@@ -828,22 +1103,25 @@ int cit_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
   if (need && (!work || work_bytes < need)) return -1;
   Epilogue e = {};
   e.bias = bias, e.res = residual, e.out = y, e.z = z, e.ldr = ldr, e.ldo = N, e.act = act;
-  if (dtype == CIT_FP32) return forward<float>(x, ldx, w, ldw, e, M, N, K, work, stream);
-  if (dtype == CIT_BF16) return forward<bf16_t>(x, ldx, w, ldw, e, M, N, K, work, stream);
-  return forward<fp16_t>(x, ldx, w, ldw, e, M, N, K, work, stream);
+  const Mat a = {x, ldx, M, K, K}, b = {w, ldw, N, K, K};
+  if (dtype == CIT_FP32) return product<float, false, false>(a, b, e, M, N, K, work, stream);
+  if (dtype == CIT_BF16) return product<bf16_t, false, false>(a, b, e, M, N, K, work, stream);
+  return product<fp16_t, false, false>(a, b, e, M, N, K, work, stream);
 }
 
 int cit_linear_backward(const void* dy, int64_t ldy, const void* z, const void* x, int64_t ldx, const void* w,
                         int64_t ldw, void* dx, void* dw, void* db, int M, int N, int K, int dtype, int act, void* work,
                         size_t work_bytes, hipStream_t stream) {
   if (M <= 0 || N <= 0 || K < 0 || bad_types(dtype, act)) return -1;
-  if (!dy || ldy < N || (act != ACT_NONE && !z) || (dx && (!w || ldw < K)) || (dw && (!x || ldx < K))) return -1;
-  const size_t need = cit_linear_backward_work_bytes(M, N, K, dtype, act);
+  if (!dy || ldy < N || (act != ACT_NONE && !z) || (dx && K && (!w || ldw < K)) || (dw && K && (!x || ldx < K)))
+    return -1;
+  const size_t need = cit_linear_backward_work_bytes(x, ldx, w, ldw, dx, dw, db, M, N, K, dtype, act);
   if (need && (!work || work_bytes < need)) return -1;
+  const Mat a = {dy, ldy, M, N, N}, b = {x, ldx, M, K, K}, c = {w, ldw, N, K, K};
   char* p = static_cast<char*>(work);
-  if (dtype == CIT_FP32) return backward<float>(dy, ldy, z, x, ldx, w, ldw, dx, dw, db, M, N, K, act, p, stream);
-  if (dtype == CIT_BF16) return backward<bf16_t>(dy, ldy, z, x, ldx, w, ldw, dx, dw, db, M, N, K, act, p, stream);
-  return backward<fp16_t>(dy, ldy, z, x, ldx, w, ldw, dx, dw, db, M, N, K, act, p, stream);
+  if (dtype == CIT_FP32) return backward<float>(a, z, b, c, dx, dw, db, M, N, K, act, p, stream);
+  if (dtype == CIT_BF16) return backward<bf16_t>(a, z, b, c, dx, dw, db, M, N, K, act, p, stream);
+  return backward<fp16_t>(a, z, b, c, dx, dw, db, M, N, K, act, p, stream);
 }
 
 }  // extern "C"

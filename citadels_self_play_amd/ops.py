@@ -9,8 +9,13 @@ kernels (csrc/cit_linear.hip, cit_policy.hip, cit_gradnorm.hip):
 
 Tensors are fp32, bf16 or fp16 on one GPU.  Every call runs on the current
 stream of its tensors' device, takes its workspace from torch's caching
-allocator, waits for nothing and can be captured into a HIP graph.  Wrong
-arguments raise ValueError before anything is launched.
+allocator and waits for nothing.  Calls can be captured into a HIP graph (a
+backward pass too, while no eager graph of the same leaves is alive: torch's
+autograd engine joins the two graphs' streams, whatever the operators).
+Wrong arguments raise ValueError before anything is launched.
+
+The checks are written out rather than shared: at a trainer's batch of 64 a
+call's time is the host's.
 """
 import collections
 import ctypes as C
@@ -24,80 +29,112 @@ from . import _lib
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 _MOST = 2 ** 31 - 1
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current = torch.cuda.current_device
+_empty, _empty_like = torch.empty, torch.empty_like
+_grad_on = torch.is_grad_enabled
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
-
-
-def _tensor(name, t, like=None):
-    _need(isinstance(t, torch.Tensor), "%s must be a tensor, not %s" % (name, type(t).__name__))
-    _need(t.layout == torch.strided, "%s must be a dense tensor" % name)
-    if like is not None:
-        _need(t.device == like.device, "%s is on %s, the first tensor on %s" % (name, t.device, like.device))
+def _same_place(first, **others):
+    """Every tensor a strided one on the first one's device, and that a GPU; None is left out."""
+    for name, t in others.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise ValueError("%s must be a tensor, not %s" % (name, type(t).__name__))
+        if t.layout != torch.strided:
+            raise ValueError("%s must be a dense tensor" % name)
+        if t.device != first.device:
+            raise ValueError("%s is on %s, the first tensor on %s" % (name, t.device, first.device))
 
 
 def _gpu(t):
-    _need(t.is_cuda, "tensors must be on the GPU (there is no CPU path), not on %s" % t.device)
+    if not t.is_cuda:
+        raise ValueError("tensors must be on the GPU (there is no CPU path), not on %s" % t.device)
 
 
-class _on:
-    """The tensors' device as the current one (nothing where it is already); gives the current stream's handle."""
-
-    def __init__(self, t):
-        self.device = t.device
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
+def _on(index, call, *args):
+    """call(*args, stream) with the device's current stream, and the device as the current one."""
+    if index == _current():
+        return call(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return call(*args, _raw_stream(index))
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _work(n, like):
-    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
-
-
 def _rows(t, width):
     """`t` [rows][width] with its entries side by side, and the elements between rows."""
-    if t.shape[0] == 1 and (width <= 1 or t.stride(1) == 1):
+    if t.is_contiguous():
         return t, width
-    if (width > 1 and t.stride(1) != 1) or t.stride(0) < width:
-        t = t.contiguous()
-    return t, max(width, t.stride(0))
+    if (width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width):
+        return t.contiguous(), width
+    return t, t.stride(0) if t.shape[0] > 1 else width
 
 
 # ---- linear ---------------------------------------------------------------------
 
 def _linear_forward(x, w, b, r, act, keep):
-    """(y, z): z is the pre-activation for the backward pass where `keep` asks for it."""
-    M, K, N = x.shape[0], x.shape[1], w.shape[0]
-    lib = _lib.load()
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    z = torch.empty_like(y) if keep else None
-    if not y.numel():
+    """(y, z) of x [M, K]: z is the pre-activation for the backward pass where `keep` asks for it."""
+    M, K = x.shape
+    N = w.shape[0]
+    y = _empty((M, N), dtype=x.dtype, device=x.device)
+    z = _empty_like(y) if keep else None
+    if not (M and N):
         return y, z
-    t = TYPES[x.dtype]
+    lib, t = _lib.load(), TYPES[x.dtype]
     x, ldx = _rows(x, K)
     w, ldw = _rows(w, K)
     ldr = N
     if r is not None:
         r, ldr = _rows(r, N)
-    with _on(x) as stream:
-        n = int(lib.cit_linear_forward_work_bytes(M, N, K, t))
-        work = _work(n, x)
-        _lib.check(lib.cit_linear_forward(x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(b), _ptr(r), ldr, y.data_ptr(),
-                                          _ptr(z), M, N, K, t, act, _ptr(work), n, stream), "cit_linear_forward")
+    px, pw = x.data_ptr(), w.data_ptr()
+    n = lib.cit_linear_forward_work_bytes(M, N, K, t)
+    work = _empty(n, dtype=torch.uint8, device=x.device) if n else None
+    rc = _on(x.get_device(), lib.cit_linear_forward, px, ldx, pw, ldw, _ptr(b), _ptr(r), ldr, y.data_ptr(), _ptr(z), M,
+             N, K, t, act, _ptr(work), n)
+    if rc:
+        _lib.check(rc, "cit_linear_forward")
     return y, z
+
+
+def _linear_backward(ctx, dy):
+    x, w, z = ctx.saved_tensors
+    nx, nw, nb, nr = ctx.needs_input_grad[:4]
+    shape, M, N, K, act = ctx.dims
+    dx = dw = db = None
+    if nx or nw or nb:
+        make = _empty if M and N else torch.zeros
+        kind = dict(dtype=dy.dtype, device=dy.device)
+        dx = make((M, K), **kind) if nx else None
+        dw = make((N, K), **kind) if nw else None
+        db = make(N, **kind) if nb else None
+        if M and N:
+            lib, t = _lib.load(), TYPES[dy.dtype]
+            d2, ldy = _rows(dy if dy.dim() == 2 else dy.reshape(M, N), N)
+            ldx = ldw = K
+            if nw:
+                x, ldx = _rows(x if x.dim() == 2 else x.reshape(M, K), K)
+            if nx:
+                w, ldw = _rows(w, K)
+            if z is not None and not z.is_contiguous():
+                z = z.contiguous()
+            px, pw = x.data_ptr() if nw else None, w.data_ptr() if nx else None
+            pdx, pdw, pdb = _ptr(dx), _ptr(dw), _ptr(db)
+            n = lib.cit_linear_backward_work_bytes(px, ldx, pw, ldw, pdx, pdw, pdb, M, N, K, t, act)
+            work = _empty(n, dtype=torch.uint8, device=dy.device) if n else None
+            rc = _on(dy.get_device(), lib.cit_linear_backward, d2.data_ptr(), ldy, _ptr(z), px, ldx, pw, ldw, pdx, pdw,
+                     pdb, M, N, K, t, act, _ptr(work), n)
+            if rc:
+                _lib.check(rc, "cit_linear_backward")
+        if nx and len(shape) != 2:
+            dx = dx.reshape(shape)
+    return dx, dw, db, dy if nr else None, None
+
+
+_linear_backward_once = once_differentiable(_linear_backward)
 
 
 class _Linear(torch.autograd.Function):
@@ -105,46 +142,24 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, w, b, r, act):
         # relu without a residual leaves its sign in y (fp16 aside, where a small y rounds to 0); other activations
         # need the pre-activation
-        own_y = act == ACTIVATIONS["relu"] and r is None and x.dtype != torch.float16
-        x2 = x.reshape(-1, w.shape[1]) if w.shape[1] else x.reshape(math.prod(x.shape[:-1]), 0)
-        y, z = _linear_forward(x2, w, b, None if r is None else r.reshape(x2.shape[0], w.shape[0]), act,
-                               act != ACTIVATIONS["none"] and not own_y)
-        out = y.reshape(x.shape[:-1] + (w.shape[0],))
-        ctx.act = act
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        ctx.save_for_backward(x if need_w else None, w if need_x else None, out if own_y else z)
-        ctx.dims = (x.shape, w.shape)
+        own_y = act == 1 and r is None and x.dtype != torch.float16
+        shape = x.shape
+        N, K = w.shape
+        x2 = x
+        if len(shape) != 2:
+            M = math.prod(shape[:-1])
+            x2 = x.reshape(M, K)
+            r = None if r is None else r.reshape(M, N)
+        y, z = _linear_forward(x2, w, b, r, act, act != 0 and not own_y)
+        out = y if x2 is x else y.reshape(shape[:-1] + (N,))
+        nx, nw = ctx.needs_input_grad[:2]
+        ctx.dims = (shape, x2.shape[0], N, K, act)
+        ctx.save_for_backward(x if nw else None, w if nx else None, out if own_y else z)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, w, z = ctx.saved_tensors
-        (xs, (N, K)), (nx, nw, nb, nr) = ctx.dims, ctx.needs_input_grad[:4]
-        M = math.prod(xs[:-1])
-        dx = dw = db = None
-        if nx or nw or nb:
-            make = torch.empty if M and N else torch.zeros
-            new = lambda *s: make(s, dtype=dy.dtype, device=dy.device)  # noqa: E731
-            dx, dw, db = new(M, K) if nx else None, new(N, K) if nw else None, new(N) if nb else None
-        if (nx or nw or nb) and M and N:
-            lib, t = _lib.load(), TYPES[dy.dtype]
-            d2, ldy = _rows(dy.reshape(M, N), N)
-            ldx = ldw = K
-            if nw:
-                x, ldx = _rows(x.reshape(M, K), K)
-            if nx:
-                w, ldw = _rows(w, K)
-            if z is not None:
-                z = z.reshape(M, N)
-                z = z if z.is_contiguous() else z.contiguous()
-            with _on(dy) as stream:
-                n = int(lib.cit_linear_backward_work_bytes(M, N, K, t, ctx.act))
-                work = _work(n, dy)
-                _lib.check(lib.cit_linear_backward(d2.data_ptr(), ldy, _ptr(z), _ptr(x) if nw else None, ldx,
-                                                   _ptr(w) if nx else None, ldw, _ptr(dx), _ptr(dw), _ptr(db), M, N, K,
-                                                   t, ctx.act, _ptr(work), n, stream), "cit_linear_backward")
-        return (dx.reshape(xs) if nx else None, dw, db, dy if nr else None, None)
+        return (_linear_backward_once if _grad_on() else _linear_backward)(ctx, dy)
 
 
 def linear(x, weight, bias=None, residual=None, activation="none"):
@@ -155,32 +170,43 @@ def linear(x, weight, bias=None, residual=None, activation="none"):
     Sums are fp32.  Differentiable in every tensor; under no_grad nothing is
     kept.  The gradient of the pre-activation is rounded to the type before the
     two products that use it (bias gradients are summed before that)."""
-    _tensor("x", x)
-    _need(x.dtype in TYPES, "x must be fp32, bf16 or fp16, not %s" % x.dtype)
-    _need(activation in ACTIVATIONS, "activation must be one of %s, not %r" % (sorted(ACTIVATIONS), activation))
-    _need(x.dim() >= 1, "x must be [..., K]")
-    _tensor("weight", weight, x)
-    _need(weight.dim() == 2 and weight.shape[1] == x.shape[-1],
-          "weight must be [N, %d] for x %s, not %s" % (x.shape[-1], tuple(x.shape), tuple(weight.shape)))
-    out = x.shape[:-1] + (weight.shape[0],)
-    for name, t, shape in (("bias", bias, (weight.shape[0],)), ("residual", residual, out)):
-        if t is not None:
-            _tensor(name, t, x)
-            _need(tuple(t.shape) == tuple(shape), "%s must be %s, not %s" % (name, tuple(shape), tuple(t.shape)))
-    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
-        _need(t is None or t.dtype == x.dtype, "%s is %s, x %s" % (name, t is not None and t.dtype, x.dtype))
-    M = math.prod(x.shape[:-1])
-    _need(max(M, x.shape[-1], weight.shape[0]) <= _MOST, "a dimension is over %d" % _MOST)
+    _same_place(x if isinstance(x, torch.Tensor) else torch.empty(0), x=x, weight=weight, bias=bias, residual=residual)
+    dt, shape, ws = x.dtype, x.shape, weight.shape
+    if dt not in TYPES:
+        raise ValueError("x must be fp32, bf16 or fp16, not %s" % dt)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError("activation must be one of %s, not %r" % (sorted(ACTIVATIONS), activation))
+    if not shape:
+        raise ValueError("x must be [..., K]")
+    if len(ws) != 2 or ws[1] != shape[-1]:
+        raise ValueError("weight must be [N, %d] for x %s, not %s" % (shape[-1], tuple(shape), tuple(ws)))
+    if weight.dtype != dt:
+        raise ValueError("weight is %s, x %s" % (weight.dtype, dt))
+    if bias is not None:
+        if bias.shape != ws[:1]:
+            raise ValueError("bias must be [%d], not %s" % (ws[0], tuple(bias.shape)))
+        if bias.dtype != dt:
+            raise ValueError("bias is %s, x %s" % (bias.dtype, dt))
+    if residual is not None:
+        if residual.shape != shape[:-1] + ws[:1]:
+            raise ValueError("residual must be %s, not %s" % (tuple(shape[:-1] + ws[:1]), tuple(residual.shape)))
+        if residual.dtype != dt:
+            raise ValueError("residual is %s, x %s" % (residual.dtype, dt))
     _gpu(x)
+    M = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+    if max(M, shape[-1], ws[0]) > _MOST:
+        raise ValueError("a dimension is over %d" % _MOST)
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    if _grad_on() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                       or (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, act)
-    y, _ = _linear_forward(x.reshape(M, x.shape[-1]), weight, bias,
-                           None if residual is None else residual.reshape(M, weight.shape[0]), act, False)
-    return y.reshape(out)
+    if len(shape) == 2:
+        return _linear_forward(x, weight, bias, residual, act, False)[0]
+    y = _linear_forward(x.reshape(M, ws[1]), weight, bias, None if residual is None else residual.reshape(M, ws[0]),
+                        act, False)[0]
+    return y.reshape(shape[:-1] + ws[:1])
 
 
 # ---- policy loss ------------------------------------------------------------------
@@ -189,7 +215,7 @@ PolicyLoss = collections.namedtuple("PolicyLoss", "loss logp kl")
 
 
 def _policy_args(logits, ref, mask, offsets, actions, old, adv, weights, low, high, beta):
-    rows = actions.shape[0]
+    """(tensors to keep, the entry points' common arguments)."""
     if offsets is None:
         width = logits.shape[1]
         logits, ld = _rows(logits, width)
@@ -200,30 +226,58 @@ def _policy_args(logits, ref, mask, offsets, actions, old, adv, weights, low, hi
         width = ld = ld_ref = ld_mask = 0
         total = logits.shape[0]
         logits, ref, mask = (None if t is None else t.contiguous() for t in (logits, ref, mask))
-    keep = (logits, ref, mask)
-    return keep, (_ptr(logits), ld, _ptr(ref), ld_ref, _ptr(mask), ld_mask, _ptr(offsets), total, rows, width,
-                  actions.data_ptr(), old.data_ptr(), adv.data_ptr(), _ptr(weights), low, high, beta,
-                  TYPES[logits.dtype])
+    return (logits, ref, mask), (logits.data_ptr(), ld, _ptr(ref), ld_ref, _ptr(mask), ld_mask, _ptr(offsets), total,
+                                 actions.shape[0], width, actions.data_ptr(), old.data_ptr(), adv.data_ptr(),
+                                 _ptr(weights), low, high, beta, TYPES[logits.dtype])
 
 
 def _policy_forward(given, want_grad):
-    logits, actions = given[0], given[4]
-    lib = _lib.load()
-    dev, rows = logits.device, actions.shape[0]
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    """(loss, logp, kl, gradient for an upstream gradient of 1)."""
+    logits, rows = given[0], given[4].shape[0]
+    lib, dev = _lib.load(), logits.device
+    loss = _empty((), dtype=torch.float32, device=dev)
+    logp = _empty(rows, dtype=torch.float32, device=dev)
+    kl = _empty(rows, dtype=torch.float32, device=dev)
     grad = None
     if want_grad:
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        grad = _empty(logits.shape, dtype=logits.dtype, device=dev)
         if not rows:
             grad.zero_()
-    with _on(logits) as stream:
-        keep, args = _policy_args(*given)
-        n = int(lib.cit_policy_loss_work_bytes(rows))
-        work = _work(n, logits)
-        _lib.check(lib.cit_policy_loss(*args, loss.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(), _ptr(grad),
-                                       _ptr(work), n, stream), "cit_policy_loss")
-    return loss, stats[0], stats[1], grad
+    n = lib.cit_policy_loss_work_bytes(rows)
+    work = _empty(n, dtype=torch.uint8, device=dev) if n else None
+    keep, args = _policy_args(*given)
+    rc = _on(logits.get_device(), lib.cit_policy_loss, *args, loss.data_ptr(), logp.data_ptr(), kl.data_ptr(),
+             _ptr(grad), _ptr(work), n)
+    if rc:
+        _lib.check(rc, "cit_policy_loss")
+    return loss, logp, kl, grad
+
+
+def _policy_backward(ctx, up):
+    given = ctx.saved_tensors + ctx.scalars
+    logits = given[0]
+    try:
+        grad, captured = ctx.held.pop()
+    except IndexError:                           # a second backward pass: the first one's gradient is its owner's
+        grad = None
+    # a graph replayed on its own may find the forward pass's gradient used up
+    ready = grad is not None and (captured or not torch.cuda.is_current_stream_capturing())
+    if grad is None:
+        grad = _empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if not given[4].shape[0]:
+        return (grad.zero_(),) + (None,) * 10
+    if up.dtype != torch.float32:
+        up = up.float()
+    lib = _lib.load()
+    keep, args = _policy_args(*given)
+    rc = _on(logits.get_device(), lib.cit_policy_loss_backward, *args, up.data_ptr(), 1 if ready else 0,
+             grad.data_ptr())
+    if rc:
+        _lib.check(rc, "cit_policy_loss_backward")
+    return (grad,) + (None,) * 10
+
+
+_policy_backward_once = once_differentiable(_policy_backward)
 
 
 class _PolicyLoss(torch.autograd.Function):
@@ -234,35 +288,35 @@ class _PolicyLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, *given):
-        loss, logp, kl, grad = _policy_forward(given, ctx.needs_input_grad[0])
+        loss, logp, kl, grad = _policy_forward(given, True)
         ctx.mark_non_differentiable(logp, kl)
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(*given[:8])
         ctx.scalars = given[8:]
         ctx.held = [(grad, torch.cuda.is_current_stream_capturing())]
         return loss, logp, kl
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, up, _logp, _kl):
-        given = ctx.saved_tensors + ctx.scalars
-        logits, rows = given[0], given[4].shape[0]
-        try:
-            grad, captured = ctx.held.pop()
-        except IndexError:                       # a second backward pass: the first one's gradient is its owner's
-            grad = None
-        # a graph replayed on its own may find the forward pass's gradient used up
-        fresh = grad is None or (torch.cuda.is_current_stream_capturing() and not captured)
-        if grad is None:
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        if not rows:
-            return (grad.zero_(),) + (None,) * 10
-        up = up.to(torch.float32).contiguous()
-        lib = _lib.load()
-        with _on(logits) as stream:
-            keep, args = _policy_args(*given)
-            _lib.check(lib.cit_policy_loss_backward(*args, up.data_ptr(), 0 if fresh else 1, grad.data_ptr(), stream),
-                       "cit_policy_loss_backward")
-        return (grad,) + (None,) * 10
+        if up is None:
+            return (None,) * 11
+        return (_policy_backward_once if _grad_on() else _policy_backward)(ctx, up)
+
+
+def _f32(name, t, N):
+    if t.shape != (N,) or not t.dtype.is_floating_point:
+        raise ValueError("%s must be [%d] floating point numbers" % (name, N))
+    if t.dtype != torch.float32:
+        t = t.float()
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.detach() if t.requires_grad else t
+
+
+def _whole(t):
+    if t.dtype != torch.int64:
+        t = t.long()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def policy_loss(logits, actions, old_logp, advantages, *, ref_logits=None, offsets=None, mask=None, weights=None,
@@ -283,94 +337,116 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logits=None, offse
     a gradient.  Rows of weight 0 are not read, rows with no legal entry (or
     nothing over -inf) count nothing: both give logp 0, kl 0 and a gradient of 0.
     A masked action has rho 0; an action outside its row, or offsets that
-    leave the list, give NaN.  KL is infinite where p_ref is 0 and p is not."""
-    _tensor("logits", logits)
-    _need(logits.dtype in TYPES, "logits must be fp32, bf16 or fp16, not %s" % logits.dtype)
-    _need(logits.dim() == (2 if offsets is None else 1),
-          "logits must be [N, width], or one list with offsets, not %s" % (tuple(logits.shape),))
+    leave the list, give NaN.  KL is infinite where p_ref is 0 and p is not, and
+    NaN where the reference leaves nothing of a row."""
+    _same_place(logits if isinstance(logits, torch.Tensor) else torch.empty(0), logits=logits, actions=actions,
+                old_logp=old_logp, advantages=advantages, ref_logits=ref_logits, offsets=offsets, mask=mask,
+                weights=weights)
+    dt, shape = logits.dtype, logits.shape
+    if dt not in TYPES:
+        raise ValueError("logits must be fp32, bf16 or fp16, not %s" % dt)
+    if len(shape) != (2 if offsets is None else 1):
+        raise ValueError("logits must be [N, width], or one list with offsets, not %s" % (tuple(shape),))
     low, high = (clip, clip) if isinstance(clip, (int, float)) else clip
     low, high, kl_coef = float(low), float(high), float(kl_coef)
-    _need(low >= 0 and high >= 0, "clip must be two numbers >= 0, not %r" % (clip,))
-    _need(0 <= kl_coef < math.inf, "kl_coef must be a finite number >= 0, not %r" % kl_coef)
-    _need(kl_coef == 0 or ref_logits is not None, "a KL term needs ref_logits")
-    _tensor("actions", actions, logits)
-    _need(actions.dim() == 1 and actions.dtype in (torch.int64, torch.int32), "actions must be [N] whole numbers")
+    if not (low >= 0 and high >= 0):
+        raise ValueError("clip must be two numbers >= 0, not %r" % (clip,))
+    if not 0 <= kl_coef < math.inf:
+        raise ValueError("kl_coef must be a finite number >= 0, not %r" % kl_coef)
+    if kl_coef and ref_logits is None:
+        raise ValueError("a KL term needs ref_logits")
+    if actions.dim() != 1 or actions.dtype not in (torch.int64, torch.int32):
+        raise ValueError("actions must be [N] whole numbers")
     N = actions.shape[0]
     if offsets is None:
-        _need(logits.shape[0] == N, "%d rows of logits, %d actions" % (logits.shape[0], N))
-        _need(logits.shape[1] <= _MOST, "a row is over %d entries" % _MOST)
+        if shape[0] != N:
+            raise ValueError("%d rows of logits, %d actions" % (shape[0], N))
+        if shape[1] > _MOST:
+            raise ValueError("a row is over %d entries" % _MOST)
     else:
-        _tensor("offsets", offsets, logits)
-        _need(offsets.dim() == 1 and offsets.dtype in (torch.int64, torch.int32) and offsets.shape[0] == N + 1,
-              "offsets must be [N + 1] whole numbers for %d actions" % N)
-    for name, t in (("old_logp", old_logp), ("advantages", advantages), ("weights", weights)):
-        if t is not None:
-            _tensor(name, t, logits)
-            _need(t.shape == (N,) and t.dtype.is_floating_point, "%s must be [N] floating point numbers" % name)
-    if ref_logits is not None:
-        _tensor("ref_logits", ref_logits, logits)
-        _need(ref_logits.shape == logits.shape and ref_logits.dtype == logits.dtype,
-              "ref_logits must be as logits (%s %s)" % (logits.dtype, tuple(logits.shape)))
-    if mask is not None:
-        _tensor("mask", mask, logits)
-        _need(mask.shape == logits.shape and mask.dtype == torch.bool,
-              "mask must be bool and as logits %s" % (tuple(logits.shape),))
+        if offsets.dtype not in (torch.int64, torch.int32) or offsets.shape != (N + 1,):
+            raise ValueError("offsets must be [N + 1] whole numbers for %d actions" % N)
+        offsets = _whole(offsets)
+    old_logp, advantages = _f32("old_logp", old_logp, N), _f32("advantages", advantages, N)
+    if weights is not None:
+        weights = _f32("weights", weights, N)
+    if ref_logits is not None and (ref_logits.shape != shape or ref_logits.dtype != dt):
+        raise ValueError("ref_logits must be as logits (%s %s)" % (dt, tuple(shape)))
+    if mask is not None and (mask.shape != shape or mask.dtype != torch.bool):
+        raise ValueError("mask must be bool and as logits %s" % (tuple(shape),))
     _gpu(logits)
-    f32 = lambda t: None if t is None else t.detach().to(torch.float32).contiguous()  # noqa: E731
-    given = (logits, None if ref_logits is None else ref_logits.detach(), mask,
-             None if offsets is None else offsets.to(torch.int64).contiguous(),
-             actions.to(torch.int64).contiguous(), f32(old_logp), f32(advantages), f32(weights), low, high, kl_coef)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if ref_logits is not None and ref_logits.requires_grad:
+        ref_logits = ref_logits.detach()
+    given = (logits, ref_logits, mask, offsets, _whole(actions), old_logp, advantages, weights, low, high, kl_coef)
+    if logits.requires_grad and _grad_on():
         return PolicyLoss(*_PolicyLoss.apply(*given))
     return PolicyLoss(*_policy_forward(given, False)[:3])
 
 
 # ---- gradient norm ------------------------------------------------------------------
 
+def _spans(tensors, kind):
+    return [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), kind) for t in tensors if t.numel()]
+
+
 def _overlap(outs, others=()):
     """Whether a tensor of `outs` shares memory with another one of them or with one of `others`."""
-    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), k) for k, ts in ((1, outs), (0, others))
-             for t in ts if t.numel()]
+    spans = _spans(outs, 1) + _spans(others, 0) if others else _spans(outs, 1)
+    spans.sort()
     end = [0, 0]                                 # of the spans of others and of outs so far
-    for a, b, k in sorted(spans):
+    for a, b, k in spans:
         if a < end[1] or (k and a < end[0]):
             return True
-        end[k] = max(end[k], b)
+        if b > end[k]:
+            end[k] = b
     return False
 
 
-def _listed(grads):
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    for t in grads:
-        _tensor("a gradient", t, grads[0])
-        _need(t.dtype in TYPES, "gradients must be fp32, bf16 or fp16, not %s" % t.dtype)
-    return [t.detach() for t in grads]
+def _listed(tensors, what):
+    """(the list, their type codes, whether all are contiguous)."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    codes, flat = [], True
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise ValueError("%s must be a tensor, not %s" % (what, type(t).__name__))
+        if t.layout != torch.strided:
+            raise ValueError("%s must be a dense tensor" % what)
+        c = TYPES.get(t.dtype)
+        if c is None:
+            raise ValueError("%ss must be fp32, bf16 or fp16, not %s" % (what, t.dtype))
+        if t.get_device() != tensors[0].get_device():
+            raise ValueError("%s is on %s, the first on %s" % (what, t.device, tensors[0].device))
+        codes.append(c)
+        flat = flat and t.is_contiguous()
+    return tensors, codes, flat
 
 
-def _norm(flat, max_norm=math.inf, outs=None):
+def _norm(flat, codes, max_norm=math.inf, outs=None, out_codes=None):
     """cit_clip_grad_norm over contiguous tensors (outs: None, `flat` itself or as many others)."""
     _gpu(flat[0])
     lib, n = _lib.load(), len(flat)
-    norm = torch.empty((), dtype=torch.float32, device=flat[0].device)
-    ptrs = (C.c_void_p * n)(*[t.data_ptr() for t in flat])
+    norm = _empty((), dtype=torch.float32, device=flat[0].device)
+    array = C.c_void_p * n
+    ptrs = array(*[t.data_ptr() for t in flat])
     sizes = (C.c_int64 * n)(*[t.numel() for t in flat])
-    types = (C.c_int32 * n)(*[TYPES[t.dtype] for t in flat])
+    types = (C.c_int32 * n)(*codes)
     to, to_types = (None, None) if outs is None else (ptrs, types)
     if outs is not None and outs is not flat:
-        to = (C.c_void_p * n)(*[t.data_ptr() for t in outs])
-        to_types = (C.c_int32 * n)(*[TYPES[t.dtype] for t in outs])
-    with _on(norm) as stream:
-        size = int(lib.cit_clip_grad_norm_work_bytes(n))
-        work = _work(size, norm)
-        _lib.check(lib.cit_clip_grad_norm(ptrs, to, sizes, types, to_types, n, max_norm, norm.data_ptr(),
-                                          work.data_ptr(), size, stream), "cit_clip_grad_norm")
+        to = array(*[t.data_ptr() for t in outs])
+        to_types = (C.c_int32 * n)(*out_codes)
+    size = lib.cit_clip_grad_norm_work_bytes(n)
+    work = _empty(size, dtype=torch.uint8, device=norm.device)
+    rc = _on(norm.get_device(), lib.cit_clip_grad_norm, ptrs, to, sizes, types, to_types, n, max_norm, norm.data_ptr(),
+             work.data_ptr(), size)
+    if rc:
+        _lib.check(rc, "cit_clip_grad_norm")
     return norm
 
 
 def grad_norm(grads):
     """sqrt of the sum of all squares of a list of gradients (fp32 scalar on the device; no tensors: 0)."""
-    grads = _listed(grads)
-    return _norm([t.contiguous() for t in grads]) if grads else torch.zeros(())
+    grads, codes, _ = _listed(grads, "a gradient")
+    return _norm([t.detach().contiguous() for t in grads], codes) if grads else torch.zeros(())
 
 
 def clip_grad_norm(grads, max_norm, out=None, error_if_nonfinite=False):
@@ -383,32 +459,38 @@ def clip_grad_norm(grads, max_norm, out=None, error_if_nonfinite=False):
     clip_grad_norm_ does; error_if_nonfinite waits for the norm and raises
     RuntimeError before anything is scaled."""
     max_norm = float(max_norm)
-    _need(max_norm >= 0, "max_norm must be a number >= 0, not %r" % max_norm)
-    grads = _listed(grads)
-    flat = [t if t.is_contiguous() else t.contiguous() for t in grads]
+    if not max_norm >= 0:
+        raise ValueError("max_norm must be a number >= 0, not %r" % max_norm)
+    grads, codes, contiguous = _listed(grads, "a gradient")
+    flat = grads if contiguous else [t.detach().contiguous() for t in grads]
+    out_codes = codes
     if out is None:
         outs = flat
-        _need(all(s > 0 or n <= 1 for t in grads if not t.is_contiguous() for n, s in zip(t.shape, t.stride())),
-              "a gradient whose elements share memory cannot be clipped in place: give out=")
+        if not contiguous and any(s == 0 and n > 1 for t in grads for n, s in zip(t.shape, t.stride())):
+            raise ValueError("a gradient whose elements share memory cannot be clipped in place: give out=")
         at = [t.data_ptr() for t in grads if t.numel()]
-        _need(len(set(at)) == len(at) and not _overlap(flat), "a gradient is listed twice, or two share memory")
+        if len(set(at)) != len(at) or _overlap(flat):
+            raise ValueError("a gradient is listed twice, or two share memory")
     else:
-        outs = [t.detach() for t in ([out] if isinstance(out, torch.Tensor) else out)]
-        _need(len(outs) == len(grads), "%d gradients, %d tensors in out" % (len(grads), len(outs)))
-        for g, o in zip(grads, outs):
-            _tensor("an out tensor", o, g)
-            _need(o.shape == g.shape and o.dtype in (g.dtype, torch.float32) and o.is_contiguous(),
-                  "an out tensor must be contiguous, of its gradient's shape, and of its type or fp32")
-        _need(not _overlap(outs, [f for f, o in zip(flat, outs) if f.data_ptr() != o.data_ptr() or f.dtype != o.dtype]),
-              "out tensors share memory with one another or with other gradients")
+        outs, out_codes, contiguous_out = _listed(out, "an out tensor")
+        if len(outs) != len(grads):
+            raise ValueError("%d gradients, %d tensors in out" % (len(grads), len(outs)))
+        for g, o, c, d in zip(grads, outs, codes, out_codes):
+            if o.shape != g.shape or (d != c and d != 0) or not contiguous_out or o.get_device() != g.get_device():
+                raise ValueError("an out tensor must be contiguous, of its gradient's shape and device, and of its "
+                                 "type or fp32")
+        if _overlap(outs, [f for f, o, c, d in zip(flat, outs, codes, out_codes)
+                           if f.data_ptr() != o.data_ptr() or c != d]):
+            raise ValueError("out tensors share memory with one another or with other gradients")
     if not grads:
         return torch.zeros(())
-    if error_if_nonfinite and not math.isfinite(float(_norm(flat))):
+    if error_if_nonfinite and not math.isfinite(float(_norm(flat, codes))):
         raise RuntimeError("the gradients' global norm is not finite: nothing was clipped")
-    norm = _norm(flat, max_norm, outs)
+    norm = _norm(flat, codes, max_norm, outs, out_codes)
     torch.autograd.graph.increment_version(outs)
-    if out is None:
-        for t, c in zip(grads, flat):
-            if c.data_ptr() != t.data_ptr():
-                t.copy_(c)
+    if flat is not grads and out is None:
+        with torch.no_grad():
+            for t, c in zip(grads, flat):
+                if c.data_ptr() != t.data_ptr():
+                    t.copy_(c)
     return norm

@@ -413,12 +413,14 @@ int cit_cfr_targets(void* pool, int B, int node_cap, int edge_cap, const int32_t
  * in fp32.  z [M][N] (may be NULL) receives the pre-activation for the
  * backward pass in the element type (a finite value stays finite, a nonzero one nonzero).
  * cit_linear_backward: from dy [M][N] (and z; relu without a residual may give y
- * for z; act none ignores it) dx [M][K], dw [N][K] and db [N], each unless NULL. */
+ * for z; act none ignores it) dx [M][K], dw [N][K] and db [N], each unless NULL.
+ * Its workspace is for these very matrices (their alignment counts). */
 size_t cit_linear_forward_work_bytes(int M, int N, int K, int dtype);
 int cit_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
                        int64_t ldr, void* y, void* z, int M, int N, int K, int dtype, int act, void* work,
                        size_t work_bytes, hipStream_t stream);
-size_t cit_linear_backward_work_bytes(int M, int N, int K, int dtype, int act);
+size_t cit_linear_backward_work_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* dx,
+                                      const void* dw, const void* db, int M, int N, int K, int dtype, int act);
 int cit_linear_backward(const void* dy, int64_t ldy, const void* z, const void* x, int64_t ldx, const void* w,
                         int64_t ldw, void* dx, void* dw, void* db, int M, int N, int K, int dtype, int act, void* work,
                         size_t work_bytes, hipStream_t stream);

@@ -490,7 +490,7 @@ def test_policy_entries_of_no_row():
     none = ops.policy_loss(lb, a["actions"][:0], a["old"][:0], a["adv"][:0], offsets=a["offsets"][:1])
     assert float(none.loss.detach()) == 0.0 and none.logp.shape == (0,)
     assert not bool(torch.autograd.grad(none.loss, lb)[0].any())
-    assert float(ops.policy_loss(la.view(1, -1)[:0], a["actions"][:0], a["old"][:0], a["adv"][:0]).loss) == 0.0
+    assert float(ops.policy_loss(la.detach().view(1, -1)[:0], a["actions"][:0], a["old"][:0], a["adv"][:0]).loss) == 0.0
 
 
 def test_policy_strides_and_types():

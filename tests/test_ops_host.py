@@ -108,10 +108,10 @@ def test_entry_points_refuse(lib):
     assert fw(p, 8, p, 8, None, None, 0, None, None, 4, 4, 8, 0, 0, None, 0, None) == -1
     assert fw(p, 8, p, 8, None, None, 0, p, None, -1, 4, 8, 0, 0, None, 0, None) == -1
     assert fw(None, 8, None, 8, None, None, 0, None, None, 0, 4, 8, 0, 0, None, 0, None) == 0
-    need = lib.cit_linear_backward_work_bytes(4, 4, 8, 1, 1)
+    need = lib.cit_linear_backward_work_bytes(p, 4000, p, 4000, p, p, p, 4000, 4000, 4000, 1, 1)
     assert need > 0
     bw = lib.cit_linear_backward
-    assert bw(p, 4, p, p, 8, p, 8, p, p, p, 4, 4, 8, 1, 1, p, need - 1, None) == -1
+    assert bw(p, 4000, p, p, 4000, p, 4000, p, p, p, 4000, 4000, 4000, 1, 1, p, need - 1, None) == -1
     assert bw(p, 4, None, p, 8, p, 8, p, p, p, 4, 4, 8, 1, 1, p, need, None) == -1
     assert bw(p, 3, p, p, 8, p, 8, p, p, p, 4, 4, 8, 1, 1, p, need, None) == -1
     pl = lib.cit_policy_loss
