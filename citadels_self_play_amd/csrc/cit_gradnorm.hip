@@ -32,25 +32,39 @@ __device__ __forceinline__ int tensor_of(const GradList& g, int c) {
   return lo;
 }
 
+// Four loads of 16 bytes at a time: 4e8 bf16 elements in 4 launches of 45 us each, 4.4 TB/s (one load at a time: 2.8).
 template <typename T>
 __device__ __forceinline__ double sum_squares(const T* p, int64_t n) {
-  constexpr int E = 16 / sizeof(T);
-  double s = 0.0;
+  constexpr int E = 16 / sizeof(T), U = 4;
+  double s[U] = {0.0, 0.0, 0.0, 0.0};
   const int64_t whole = n / E;
-  for (int64_t i = threadIdx.x; i < whole; i += 256) {
+  int64_t i = threadIdx.x;
+  for (; i + (U - 1) * 256 < whole; i += U * 256) {
+    Pack16<T> v[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) v[u].raw = load16(p + (i + u * 256) * E);
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int j = 0; j < E; j++) {
+        const double d = (double)to_f(v[u].e[j]);
+        s[u] = fma(d, d, s[u]);
+      }
+  }
+  for (; i < whole; i += 256) {
     Pack16<T> v;
     v.raw = load16(p + i * E);
 #pragma unroll
     for (int j = 0; j < E; j++) {
       const double d = (double)to_f(v.e[j]);
-      s = fma(d, d, s);
+      s[0] = fma(d, d, s[0]);
     }
   }
-  for (int64_t i = whole * E + threadIdx.x; i < n; i += 256) {
+  for (i = whole * E + threadIdx.x; i < n; i += 256) {
     const double d = (double)to_f(p[i]);
-    s = fma(d, d, s);
+    s[1] = fma(d, d, s[1]);
   }
-  return s;
+  return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 __global__ __launch_bounds__(256) void k_sum_squares(GradList g, double* part) {
@@ -72,43 +86,71 @@ __global__ __launch_bounds__(256) void k_sum_squares(GradList g, double* part) {
   if (threadIdx.x == 0) part[blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
 
-// work: [0] the factor (fp32), then the partial sums.
-__global__ __launch_bounds__(1024) void k_norm(const double* part, int count, double max_norm, float* norm,
-                                               float* factor) {
-  __shared__ double sums[16];
+// The norm and the factor from the partial sums, the same in every workgroup that asks (THREADS threads, all of them).
+template <int THREADS>
+__device__ __forceinline__ double norm_of(const double* part, int count, double (&sums)[THREADS / 64]) {
   double s = 0.0;
-  for (int i = threadIdx.x; i < count; i += 1024) s += part[i];
+  for (int i = threadIdx.x; i < count; i += THREADS) s += part[i];
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x) return;
   s = 0.0;
-  for (int i = 0; i < 16; i++) s += sums[i];
-  const double n = sqrt(s);
-  *norm = (float)n;
+  for (int i = 0; i < THREADS / 64; i++) s += sums[i];
+  return sqrt(s);
+}
+__device__ __forceinline__ float factor_of(double n, double max_norm) {
   const double c = max_norm / (n + 1e-6);
-  *factor = max_norm == INFINITY || c >= 1.0 ? 1.0f : (float)c;        // a NaN norm makes NaN gradients
+  return max_norm == INFINITY || c >= 1.0 ? 1.0f : (float)c;           // a NaN norm makes NaN gradients
 }
 
+// work: [0] the factor (fp32), [2] on the partial sums.
+__global__ __launch_bounds__(1024) void k_norm(const double* part, int count, double max_norm, float* norm,
+                                               float* factor) {
+  __shared__ double sums[16];
+  const double n = norm_of<1024>(part, count, sums);
+  if (threadIdx.x) return;
+  *norm = (float)n;
+  *factor = factor_of(n, max_norm);
+}
+
+// A lane writes 16 neighbouring bytes and reads what they are made of, four times over: 4e8 bf16 elements to fp32 in
+// 4 launches of 121 us each, 5.0 TB/s, what a copy reaches (16 bytes read and 32 written a lane: 3.4).  Scaling the
+// last tensors first, for what the cache before memory still holds of them, changed nothing.
 template <typename T, typename O>
 __device__ __forceinline__ void scale(const T* p, O* o, int64_t n, float c) {
-  constexpr int E = 16 / sizeof(T), EO = 16 / sizeof(O), W = E > EO ? E : EO;   // elements of a step
+  constexpr int W = 16 / sizeof(O), U = 4;
+  struct __attribute__((packed, aligned(2))) In { T e[W]; };
   const int64_t whole = n / W;
-  for (int64_t i = threadIdx.x; i < whole; i += 256) {
-    Pack16<T> v[W / E];
-    Pack16<O> r[W / EO];
+  auto write = [&](int64_t i, const In& v) {
+    Pack16<O> r;
 #pragma unroll
-    for (int k = 0; k < W / E; k++) v[k].raw = load16(p + i * W + k * E);
+    for (int j = 0; j < W; j++) r.e[j] = from_f<O>(to_f((T)v.e[j]) * c);
+    store16(o + i * W, r.raw);
+  };
+  int64_t i = threadIdx.x;
+  for (; i + (U - 1) * 256 < whole; i += U * 256) {
+    In v[U];
 #pragma unroll
-    for (int j = 0; j < W; j++) r[j / EO].e[j % EO] = from_f<O>(to_f(v[j / E].e[j % E]) * c);
+    for (int u = 0; u < U; u++) v[u] = *reinterpret_cast<const In*>(p + (i + u * 256) * W);
 #pragma unroll
-    for (int k = 0; k < W / EO; k++) store16(o + i * W + k * EO, r[k].raw);
+    for (int u = 0; u < U; u++) write(i + u * 256, v[u]);
   }
-  for (int64_t i = whole * W + threadIdx.x; i < n; i += 256) o[i] = from_f<O>(to_f(p[i]) * c);
+  for (; i < whole; i += 256) write(i, *reinterpret_cast<const In*>(p + i * W));
+  for (i = whole * W + threadIdx.x; i < n; i += 256) o[i] = from_f<O>(to_f(p[i]) * c);
 }
 
-__global__ __launch_bounds__(256) void k_scale(GradList g, const float* factor) {
-  const float f = *factor;
+// `parts` > 0: every workgroup works the norm out of that many partial sums itself, which saves a launch.
+__global__ __launch_bounds__(256) void k_scale(GradList g, const float* factor, const double* part, int parts,
+                                               double max_norm, float* norm) {
+  __shared__ double sums[4];
+  float f;
+  if (parts) {
+    const double n = norm_of<256>(part, parts, sums);
+    f = factor_of(n, max_norm);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+  } else {
+    f = *factor;
+  }
   const int chunks = g.first[g.count];
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
     const int t = tensor_of(g, c);
@@ -141,25 +183,30 @@ int cit_clip_grad_norm(const void* const* grads, void* const* out, const int64_t
   if (tensors && (!grads || !sizes || !types || (out && !out_types))) return -1;
   if (out && !(max_norm >= 0.0)) return -1;
   int64_t total = 0;
+  int count = 0;
   for (int t = 0; t < tensors; t++) {
     if (sizes[t] < 0 || sizes[t] > (int64_t)1 << 48 || (sizes[t] && !grads[t])) return -1;
     if (types[t] < CIT_FP32 || types[t] > CIT_FP16) return -1;
     if (out && ((sizes[t] && !out[t]) || (out_types[t] != types[t] && out_types[t] != CIT_FP32))) return -1;
     total += sizes[t];
+    count += sizes[t] > 0;
   }
-  // about GN_BLOCKS chunks in all: fewer leave compute units idle, more only add ends
-  int64_t chunk = (total / GN_BLOCKS + 2047) / 2048 * 2048;
+  const int lists_needed = count ? (count + GN_LIST - 1) / GN_LIST : 1;
+  const int each = (count + lists_needed - 1) / lists_needed;          // lists of equal length: none left with a few
+  // about 8 GN_BLOCKS chunks in all, so that each launch of a long list has enough workgroups
+  int64_t chunk = (total / (8 * GN_BLOCKS) + 2047) / 2048 * 2048;
   if (chunk < 2048) chunk = 2048;
   if (chunk > (int64_t)1 << 30) chunk = (int64_t)1 << 30;
   float* factor = static_cast<float*>(work);
   double* part = static_cast<double*>(work) + 2;
+  int parts = 0, lists = 0;
+  bool own_norm = false;                             // the scaling workgroups take the norm from the partial sums
   for (int pass = 0; pass < (out ? 2 : 1); pass++) {
-    int parts = 0;
     for (int t = 0; t < tensors;) {
       GradList g;
       g.count = 0, g.chunk = (int32_t)chunk;
       int64_t chunks = 0;
-      for (; t < tensors && g.count < GN_LIST; t++) {
+      for (; t < tensors && g.count < each; t++) {
         if (!sizes[t]) continue;
         const int64_t more = (sizes[t] + chunk - 1) / chunk;
         if (chunks + more > INT32_MAX / 2) return -1;
@@ -172,12 +219,21 @@ int cit_clip_grad_norm(const void* const* grads, void* const* out, const int64_t
       if (!g.count) continue;
       g.first[g.count] = (int32_t)chunks;
       const int blocks = chunks < GN_BLOCKS ? (int)chunks : GN_BLOCKS;
-      if (pass == 0) hipLaunchKernelGGL(k_sum_squares, dim3(blocks), dim3(256), 0, stream, g, part + parts);
-      else hipLaunchKernelGGL(k_scale, dim3(blocks), dim3(256), 0, stream, g, factor);
-      parts += blocks;
+      if (pass == 0) {
+        hipLaunchKernelGGL(k_sum_squares, dim3(blocks), dim3(256), 0, stream, g, part + parts);
+        parts += blocks;
+        lists++;
+      } else {
+        hipLaunchKernelGGL(k_scale, dim3(blocks), dim3(256), 0, stream, g, factor, part, own_norm ? parts : 0, max_norm,
+                           norm);
+      }
     }
-    if (pass == 0)
-      hipLaunchKernelGGL(k_norm, dim3(1), dim3(1024), 0, stream, part, parts, out ? max_norm : INFINITY, norm, factor);
+    if (pass == 0) {
+      own_norm = out && lists == 1 && parts <= 1024;
+      if (!own_norm)
+        hipLaunchKernelGGL(k_norm, dim3(1), dim3(1024), 0, stream, part, parts, out ? max_norm : INFINITY, norm,
+                           factor);
+    }
   }
   return launch_status();
 }

@@ -653,19 +653,21 @@ __device__ __forceinline__ void small_tile(const Mat& A, const Mat* Z, const Mat
   f32x4 acc[2][2];
 #pragma unroll
   for (int i = 0; i < 4; i++) acc[i >> 1][i & 1] = f32x4{0, 0, 0, 0};
+  // the next tile's loads are under way while this one is at work; two tiles ahead spilled registers and gained nothing
   Stage<T, AKS, 32, 64, DZ> sa;
   Stage<T, BKS, 32, 64> sb;
+  constexpr int STEP = SMALL_WAVES * BK<T>;
   int k = kb + w * BK<T>;
   if (k < ke) {
     sa.load(a, m0, k, l, Z);
     sb.load(b, n0, k, l);
   }
-  for (; k < ke; k += SMALL_WAVES * BK<T>) {
+  for (; k < ke; k += STEP) {
     sa.store(la, l, act);
     sb.store(lb, l);
-    if (k + SMALL_WAVES * BK<T> < ke) {
-      sa.load(a, m0, k + SMALL_WAVES * BK<T>, l, Z);
-      sb.load(b, n0, k + SMALL_WAVES * BK<T>, l);
+    if (k + STEP < ke) {
+      sa.load(a, m0, k + STEP, l, Z);
+      sb.load(b, n0, k + STEP, l);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -717,136 +719,54 @@ __global__ __launch_bounds__(SMALL_WAVES * 64, 4) void k_gemm_small(Mat A, Mat B
                                  blockIdx.y, k_per_split, lds);
 }
 
-// A small layer's whole backward pass in one launch: workgroups for the tiles of
-// dx, then those of dw, then 16 columns each of db; dz is made from dy and z
-// wherever it is read.
+// A small layer's whole backward pass in one launch: workgroups for 4 columns
+// each of db, then the tiles of dw (the long ones first), then those of dx; dz
+// is made from dy and z wherever it is read.
 template <typename T>
 __global__ __launch_bounds__(SMALL_WAVES * 64, 4) void k_backward_small(Mat dy, Mat z, Mat x, Mat w, T* dx, T* dw, T* db,
-                                                                     int act, int M, int N, int K, int dx_tiles,
+                                                                     int act, int M, int N, int K, int sums,
                                                                      int dw_tiles) {
   __shared__ __attribute__((aligned(16))) char lds[SMALL_LDS];
   const int tiles_k = (K + 31) / 32;
   int b = blockIdx.x;
-  Epilogue e = {};
-  e.ldo = K;
-  if (b < dx_tiles) {
+  if (b >= sums) {
+    b -= sums;
+    Epilogue e = {};
+    e.ldo = K;
+    if (b < dw_tiles) {
+      e.out = dw;
+      const int m0 = b / tiles_k * 32, n0 = b % tiles_k * 32;
+      if (act == ACT_NONE) small_tile<T, true, true, false>(dy, &z, x, e, act, N, K, M, m0, n0, 0, M, lds);
+      else small_tile<T, true, true, true>(dy, &z, x, e, act, N, K, M, m0, n0, 0, M, lds);
+      return;
+    }
+    b -= dw_tiles;
     e.out = dx;
     const int m0 = b / tiles_k * 32, n0 = b % tiles_k * 32;
     if (act == ACT_NONE) small_tile<T, false, true, false>(dy, &z, w, e, act, M, K, N, m0, n0, 0, N, lds);
     else small_tile<T, false, true, true>(dy, &z, w, e, act, M, K, N, m0, n0, 0, N, lds);
     return;
   }
-  b -= dx_tiles;
-  if (b < dw_tiles) {
-    e.out = dw;
-    const int m0 = b / tiles_k * 32, n0 = b % tiles_k * 32;
-    if (act == ACT_NONE) small_tile<T, true, true, false>(dy, &z, x, e, act, N, K, M, m0, n0, 0, M, lds);
-    else small_tile<T, true, true, true>(dy, &z, x, e, act, N, K, M, m0, n0, 0, M, lds);
-    return;
-  }
-  b -= dw_tiles;
-  // 32 rows of 16 columns at a time, then 32 partial sums a column
-  const int c = threadIdx.x & 15, y = threadIdx.x >> 4, n = b * 16 + c;
+  // 128 rows of 4 columns at a time, then the 16 rows of a wave, then the waves
+  const int c = threadIdx.x & 3, n = b * 4 + c;
   float s = 0.0f;
   if (n < N)
-    for (int m = y; m < M; m += SMALL_WAVES * 4) {
+#pragma unroll 4
+    for (int m = threadIdx.x >> 2; m < M; m += SMALL_WAVES * 16) {
       float v = to_f(static_cast<const T*>(dy.p)[m * dy.ld + n]);
       if (act != ACT_NONE) v *= act_grad<T>(act, to_f(static_cast<const T*>(z.p)[m * z.ld + n]));
       s += v;
     }
-  float* sums = reinterpret_cast<float*>(lds);
-  sums[y * 16 + c] = s;
+#pragma unroll
+  for (int d = 4; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
+  float* part = reinterpret_cast<float*>(lds);
+  if ((threadIdx.x & 63) < 4) part[(threadIdx.x >> 6) * 4 + c] = s;
   __syncthreads();
-  if (y || n >= N) return;
+  if (threadIdx.x >= 4 || n >= N) return;
   float t = 0.0f;
 #pragma unroll
-  for (int i = 0; i < SMALL_WAVES * 4; i++) t += sums[i * 16 + c];
+  for (int i = 0; i < SMALL_WAVES; i++) t += part[i * 4 + c];
   db[n] = from_f<T>(t);
-}
-
-// The splits' sums in their order, then the epilogue.
-template <typename T>
-__global__ __launch_bounds__(256) void k_join(Epilogue e, int64_t M, int N, int splits) {
-  const int64_t count = M * N;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-    float v = 0.0f;
-    for (int s = 0; s < splits; s++) v += e.part[s * count + i];
-    const int64_t m = i / N;
-    finish<T>(e, m, (int)(i - m * N), N, v);
-  }
-}
-
-// ---- dz and db --------------------------------------------------------------------
-//
-// Workgroup (column block, row share): 16 lanes across 8 columns each, 16 rows
-// down, over the share's rows.  dz = dy act'(z) rounded once to the element
-// type (the matrix cores' input), its column sums taken before that rounding.
-// Bound by memory: dy and z read, dz written.
-
-#define DZ_COLUMNS 128
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_dz(const T* dy, int64_t ldy, const T* z, T* dz, int64_t ldd, T* db, float* part,
-                                            int M, int N, int act, int rows_per) {
-  __shared__ float sums[16][DZ_COLUMNS + 4];
-  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-  const int n = blockIdx.x * DZ_COLUMNS + x * 8;
-  const int mb = blockIdx.y * rows_per, me = min(M, mb + rows_per);
-  float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (n + 8 <= N) {
-#pragma unroll 2
-    for (int m = mb + y; m < me; m += 16) {
-      float v[8], u[8];
-      load8<T>(dy + m * ldy + n, v);
-      if (act != ACT_NONE) {
-        load8<T>(z + (int64_t)m * N + n, u);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= act_grad<T>(act, u[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; i++) s[i] += v[i];
-      if (dz) {
-        T o[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = from_f<T>(v[i]);
-        store8<T>(dz + m * ldd + n, o);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (n + i < N)
-        for (int m = mb + y; m < me; m += 16) {
-          float v = to_f(dy[m * ldy + n + i]);
-          if (act != ACT_NONE) v *= act_grad<T>(act, to_f(z[(int64_t)m * N + n + i]));
-          s[i] += v;
-          if (dz) dz[m * ldd + n + i] = from_f<T>(v);
-        }
-  }
-  if (!db && !part) return;
-#pragma unroll
-  for (int i = 0; i < 8; i++) sums[y][x * 8 + i] = s[i];
-  __syncthreads();
-  const int c = blockIdx.x * DZ_COLUMNS + threadIdx.x;
-  if (threadIdx.x >= DZ_COLUMNS || c >= N) return;
-  float t = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; i++) t += sums[i][threadIdx.x];
-  if (part) part[(int64_t)blockIdx.y * N + c] = t;
-  else db[c] = from_f<T>(t);
-}
-
-// The shares' column sums: 4 waves over the shares, in a fixed order.
-template <typename T>
-__global__ __launch_bounds__(256) void k_db(const float* part, T* db, int N, int shares) {
-  __shared__ float sums[4][64];
-  const int x = threadIdx.x & 63, w = threadIdx.x >> 6, n = blockIdx.x * 64 + x;
-  float s = 0.0f;
-  if (n < N)
-    for (int i = w; i < shares; i += 4) s += part[(int64_t)i * N + n];
-  sums[w][x] = s;
-  __syncthreads();
-  if (w == 0 && n < N) db[n] = from_f<T>((sums[0][x] + sums[1][x]) + (sums[2][x] + sums[3][x]));
 }
 
 // ---- padded copies -----------------------------------------------------------------
@@ -984,9 +904,15 @@ int dz_rows(int M, int N) {
   return cdiv(cdiv(M, shares), 16) * 16;
 }
 
-// Whether the backward pass goes in one launch: both products small and neither reduction long (db's column sums
-// walk M rows, 32 at a time).  fp32 64 x 418 x 512: 14 us in one, 25 in five; 2048 x 512 x 256: 63 in one, 39 in five.
-bool one_launch(int M, int N, int K) { return K > 0 && small(M, K) && small(N, K) && M <= 512 && N <= 4096; }
+// Whether the backward pass goes in one launch, where act' is worked out again by every 32 columns of K: cells of
+// that work, and rows for the column sums to walk.  One launch against five, us: fp32 relu 64 x 418 x 512 8.5 / 15,
+// 2048 x 512 x 256 25 / 32, 512 x 1024 x 1024 (34e6 cells) 42 / 41; fp32 gelu (erfc) 512 x 418 x 512 (7e6) 23 / 25,
+// 1024 x 418 x 512 (14e6) 40 / 36; bf16 gelu 2048 x 418 x 512 (27e6) 30 / 35, 512 x 1024 x 1024 33 / 22.
+bool one_launch(int M, int N, int K, int es, int act) {
+  if (K <= 0 || M > 2048 || N > 4096) return false;
+  const int64_t k = cdiv(K, 32), cells = (int64_t)M * N * k;
+  return cdiv(M, 32) * k <= 1024 && cdiv(N, 32) * k <= 1024 && cells <= (es == 4 && act > ACT_RELU ? 8 << 20 : 30 << 20);
+}
 
 // The pieces of a workspace, in their order; bytes 0: not needed.
 struct Layout {
@@ -997,7 +923,7 @@ struct Layout {
 Layout backward_layout(const void* x, int64_t ldx, const void* w, int64_t ldw, bool dx, bool dw, bool db, int M, int N,
                        int K, int es, int act) {
   Layout l = {};
-  if (M <= 0 || N <= 0 || one_launch(M, N, K)) return l;
+  if (M <= 0 || N <= 0 || one_launch(M, N, K, es, act)) return l;
   if (K <= 0) dx = dw = false;
   // dz in rows of its own; where there is no activation dy stands for it, unless its rows are off 16 bytes, which
   // the size alone decides here
@@ -1034,13 +960,13 @@ void make_copies(const Layout& l, Mat& x, Mat& w, char* work, hipStream_t stream
 template <typename T>
 int backward(Mat dy, const void* z, Mat x, Mat w, void* dx, void* dw, void* db, int M, int N, int K, int act,
              char* work, hipStream_t stream) {
-  if (one_launch(M, N, K)) {
+  if (one_launch(M, N, K, sizeof(T), act)) {
     const int dx_tiles = dx ? cdiv(M, 32) * cdiv(K, 32) : 0, dw_tiles = dw ? cdiv(N, 32) * cdiv(K, 32) : 0;
-    const int sums = db ? cdiv(N, 16) : 0;
+    const int sums = db ? cdiv(N, 4) : 0;
     if (dx_tiles + dw_tiles + sums)
       hipLaunchKernelGGL((k_backward_small<T>), dim3(dx_tiles + dw_tiles + sums), dim3(SMALL_WAVES * 64), 0, stream, dy,
                          Mat{z, N, M, N, N}, x, w, static_cast<T*>(dx), static_cast<T*>(dw), static_cast<T*>(db), act,
-                         M, N, K, dx_tiles, dw_tiles);
+                         M, N, K, sums, dw_tiles);
     return launch_status();
   }
   const Layout l =

@@ -172,9 +172,17 @@ __device__ __forceinline__ Pack<T, E> load_pack(const T* row, const uint8_t* ok,
     for (int i = 0; i < E; i++) v.set(i, j + i < len ? to_f(row[j + i]) : -INFINITY);
   }
   if (ok) {                      // illegal entries are -inf from here on
+    if (E > 1 && j + E <= len) {
+      struct __attribute__((packed, aligned(1))) Bytes { uint8_t b[E]; };
+      const Bytes m = *reinterpret_cast<const Bytes*>(ok + j);
 #pragma unroll
-    for (int i = 0; i < E; i++)
-      if (j + i < len && !ok[j + i]) v.set(i, -INFINITY);
+      for (int i = 0; i < E; i++)
+        if (!m.b[i]) v.set(i, -INFINITY);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i++)
+        if (j + i < len && !ok[j + i]) v.set(i, -INFINITY);
+    }
   }
   return v;
 }

@@ -385,59 +385,53 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logits=None, offse
 
 # ---- gradient norm ------------------------------------------------------------------
 
-def _spans(tensors, kind):
-    return [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), kind) for t in tensors if t.numel()]
-
-
-def _overlap(outs, others=()):
-    """Whether a tensor of `outs` shares memory with another one of them or with one of `others`."""
-    spans = _spans(outs, 1) + _spans(others, 0) if others else _spans(outs, 1)
-    spans.sort()
-    end = [0, 0]                                 # of the spans of others and of outs so far
-    for a, b, k in spans:
-        if a < end[1] or (k and a < end[0]):
-            return True
-        if b > end[k]:
-            end[k] = b
-    return False
-
-
 def _listed(tensors, what):
-    """(the list, their type codes, whether all are contiguous)."""
+    """(the list, its type codes, whether all are contiguous)."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    codes, flat = [], True
-    for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise ValueError("%s must be a tensor, not %s" % (what, type(t).__name__))
-        if t.layout != torch.strided:
+    if not all(isinstance(t, torch.Tensor) for t in tensors):
+        raise ValueError("%s must be a tensor" % what)
+    kinds = {(t.dtype, t.get_device(), t.layout) for t in tensors}
+    for dt, device, layout in kinds:
+        if layout != torch.strided:
             raise ValueError("%s must be a dense tensor" % what)
-        c = TYPES.get(t.dtype)
-        if c is None:
-            raise ValueError("%ss must be fp32, bf16 or fp16, not %s" % (what, t.dtype))
-        if t.get_device() != tensors[0].get_device():
-            raise ValueError("%s is on %s, the first on %s" % (what, t.device, tensors[0].device))
-        codes.append(c)
-        flat = flat and t.is_contiguous()
-    return tensors, codes, flat
+        if dt not in TYPES:
+            raise ValueError("%ss must be fp32, bf16 or fp16, not %s" % (what, dt))
+        if device != tensors[0].get_device():
+            raise ValueError("%ss must be on one device" % what)
+    if len(kinds) == 1:
+        codes = [TYPES[tensors[0].dtype]] * len(tensors)
+    else:
+        codes = [TYPES[t.dtype] for t in tensors]
+    return tensors, codes, all(t.is_contiguous() for t in tensors)
 
 
-def _norm(flat, codes, max_norm=math.inf, outs=None, out_codes=None):
-    """cit_clip_grad_norm over contiguous tensors (outs: None, `flat` itself or as many others)."""
-    _gpu(flat[0])
-    lib, n = _lib.load(), len(flat)
-    norm = _empty((), dtype=torch.float32, device=flat[0].device)
-    array = C.c_void_p * n
-    ptrs = array(*[t.data_ptr() for t in flat])
-    sizes = (C.c_int64 * n)(*[t.numel() for t in flat])
-    types = (C.c_int32 * n)(*codes)
-    to, to_types = (None, None) if outs is None else (ptrs, types)
-    if outs is not None and outs is not flat:
-        to = array(*[t.data_ptr() for t in outs])
-        to_types = (C.c_int32 * n)(*out_codes)
+def _addresses(tensors, codes):
+    """(addresses, element counts, (start, end) of those that are not empty)."""
+    ptrs, sizes = [t.data_ptr() for t in tensors], [t.numel() for t in tensors]
+    return ptrs, sizes, [(p, p + n * (2 if c else 4)) for p, n, c in zip(ptrs, sizes, codes) if n]
+
+
+def _disjoint(spans):
+    end = 0
+    for a, b in sorted(spans):
+        if a < end:
+            return False
+        end = b
+    return True
+
+
+def _norm(like, codes, ptrs, sizes, max_norm=math.inf, to=None, to_codes=None):
+    """cit_clip_grad_norm over contiguous tensors at `ptrs`, into those at `to` (None: the norm alone)."""
+    _gpu(like)
+    lib, n = _lib.load(), len(ptrs)
+    norm = _empty((), dtype=torch.float32, device=like.device)
+    pointers, types = C.c_void_p * n, C.c_int32 * n
+    grads, kinds = pointers(*ptrs), types(*codes)
+    outs, out_kinds = (None, None) if to is None else (grads, kinds) if to is ptrs else (pointers(*to), types(*to_codes))
     size = lib.cit_clip_grad_norm_work_bytes(n)
-    work = _empty(size, dtype=torch.uint8, device=norm.device)
-    rc = _on(norm.get_device(), lib.cit_clip_grad_norm, ptrs, to, sizes, types, to_types, n, max_norm, norm.data_ptr(),
-             work.data_ptr(), size)
+    work = _empty(size, dtype=torch.uint8, device=like.device)
+    rc = _on(like.get_device(), lib.cit_clip_grad_norm, grads, outs, (C.c_int64 * n)(*sizes), kinds, out_kinds, n,
+             max_norm, norm.data_ptr(), work.data_ptr(), size)
     if rc:
         _lib.check(rc, "cit_clip_grad_norm")
     return norm
@@ -445,8 +439,11 @@ def _norm(flat, codes, max_norm=math.inf, outs=None, out_codes=None):
 
 def grad_norm(grads):
     """sqrt of the sum of all squares of a list of gradients (fp32 scalar on the device; no tensors: 0)."""
-    grads, codes, _ = _listed(grads, "a gradient")
-    return _norm([t.detach().contiguous() for t in grads], codes) if grads else torch.zeros(())
+    grads, codes, contiguous = _listed(grads, "a gradient")
+    if not grads:
+        return torch.zeros(())
+    flat = grads if contiguous else [t.detach().contiguous() for t in grads]
+    return _norm(flat[0], codes, *_addresses(flat, codes)[:2])
 
 
 def clip_grad_norm(grads, max_norm, out=None, error_if_nonfinite=False):
@@ -463,30 +460,35 @@ def clip_grad_norm(grads, max_norm, out=None, error_if_nonfinite=False):
         raise ValueError("max_norm must be a number >= 0, not %r" % max_norm)
     grads, codes, contiguous = _listed(grads, "a gradient")
     flat = grads if contiguous else [t.detach().contiguous() for t in grads]
-    out_codes = codes
+    ptrs, sizes, spans = _addresses(flat, codes)
     if out is None:
-        outs = flat
+        outs, to, to_codes = flat, ptrs, codes
         if not contiguous and any(s == 0 and n > 1 for t in grads for n, s in zip(t.shape, t.stride())):
             raise ValueError("a gradient whose elements share memory cannot be clipped in place: give out=")
         at = [t.data_ptr() for t in grads if t.numel()]
-        if len(set(at)) != len(at) or _overlap(flat):
+        if not _disjoint(spans) or len(set(at)) != len(at):
             raise ValueError("a gradient is listed twice, or two share memory")
     else:
-        outs, out_codes, contiguous_out = _listed(out, "an out tensor")
+        outs, to_codes, contiguous_out = _listed(out, "an out tensor")
         if len(outs) != len(grads):
             raise ValueError("%d gradients, %d tensors in out" % (len(grads), len(outs)))
-        for g, o, c, d in zip(grads, outs, codes, out_codes):
-            if o.shape != g.shape or (d != c and d != 0) or not contiguous_out or o.get_device() != g.get_device():
-                raise ValueError("an out tensor must be contiguous, of its gradient's shape and device, and of its "
-                                 "type or fp32")
-        if _overlap(outs, [f for f, o, c, d in zip(flat, outs, codes, out_codes)
-                           if f.data_ptr() != o.data_ptr() or c != d]):
-            raise ValueError("out tensors share memory with one another or with other gradients")
+        if not contiguous_out or any(o.shape != g.shape for g, o in zip(grads, outs)) or \
+                any(d != c and d for c, d in zip(codes, to_codes)):
+            raise ValueError("an out tensor must be contiguous, of its gradient's shape, and of its type or fp32")
+        if outs and outs[0].get_device() != grads[0].get_device():
+            raise ValueError("out tensors must be on the gradients' device")
+        to, _, out_spans = _addresses(outs, to_codes)
+        if not _disjoint(out_spans + spans):
+            # gradients may share memory among themselves, and one may be its own out tensor
+            alone = [(f, c) for f, p, o, c, d in zip(flat, ptrs, to, codes, to_codes) if p != o or c != d]
+            alone = _addresses([f for f, _ in alone], [c for _, c in alone])[2]
+            if not _disjoint(out_spans) or any(not _disjoint(out_spans + [s]) for s in alone):
+                raise ValueError("out tensors share memory with one another or with other gradients")
     if not grads:
         return torch.zeros(())
-    if error_if_nonfinite and not math.isfinite(float(_norm(flat, codes))):
+    if error_if_nonfinite and not math.isfinite(float(_norm(flat[0], codes, ptrs, sizes))):
         raise RuntimeError("the gradients' global norm is not finite: nothing was clipped")
-    norm = _norm(flat, codes, max_norm, outs, out_codes)
+    norm = _norm(flat[0], codes, ptrs, sizes, max_norm, to, to_codes)
     torch.autograd.graph.increment_version(outs)
     if flat is not grads and out is None:
         with torch.no_grad():

@@ -85,7 +85,8 @@ def test_clip_refuses():
         ((two, 1.0, [T(6), T(8)[::2]]), "an out tensor must be"),
         (([g, T(6)], 1.0, [T(6), g]), "share memory"),
         (([T(4), T(4)], 1.0, list(T(7).as_strided((2, 4), (3, 1)))), "share memory"),
-        (([T(6).half()], 1.0, [T(6).half().view(torch.float16), ]), "must be on the GPU"),
+        (([g, g], 1.0, [T(6), T(6)]), "must be on the GPU"),
+        (([g], 1.0, [g]), "must be on the GPU"),
         ((two, 1.0), "must be on the GPU"),
     ]:
         with pytest.raises(ValueError, match=says):
