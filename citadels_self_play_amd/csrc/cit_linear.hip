@@ -769,6 +769,91 @@ __global__ __launch_bounds__(SMALL_WAVES * 64, 4) void k_backward_small(Mat dy, 
   db[n] = from_f<T>(t);
 }
 
+// The splits' sums in their order, then the epilogue.
+template <typename T>
+__global__ __launch_bounds__(256) void k_join(Epilogue e, int64_t M, int N, int splits) {
+  const int64_t count = M * N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    float v = 0.0f;
+    for (int s = 0; s < splits; s++) v += e.part[s * count + i];
+    const int64_t m = i / N;
+    finish<T>(e, m, (int)(i - m * N), N, v);
+  }
+}
+
+// ---- dz and db --------------------------------------------------------------------
+//
+// Workgroup (column block, row share): 16 lanes across 8 columns each, 16 rows
+// down, over the share's rows.  dz = dy act'(z) rounded once to the element
+// type (the matrix cores' input), its column sums taken before that rounding.
+// Bound by memory: dy and z read, dz written.
+
+#define DZ_COLUMNS 128
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_dz(const T* dy, int64_t ldy, const T* z, T* dz, int64_t ldd, T* db, float* part,
+                                            int M, int N, int act, int rows_per) {
+  __shared__ float sums[16][DZ_COLUMNS + 4];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+  const int n = blockIdx.x * DZ_COLUMNS + x * 8;
+  const int mb = blockIdx.y * rows_per, me = min(M, mb + rows_per);
+  float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (n + 8 <= N) {
+#pragma unroll 2
+    for (int m = mb + y; m < me; m += 16) {
+      float v[8], u[8];
+      load8<T>(dy + m * ldy + n, v);
+      if (act != ACT_NONE) {
+        load8<T>(z + (int64_t)m * N + n, u);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= act_grad<T>(act, u[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) s[i] += v[i];
+      if (dz) {
+        T o[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = from_f<T>(v[i]);
+        store8<T>(dz + m * ldd + n, o);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (n + i < N)
+        for (int m = mb + y; m < me; m += 16) {
+          float v = to_f(dy[m * ldy + n + i]);
+          if (act != ACT_NONE) v *= act_grad<T>(act, to_f(z[(int64_t)m * N + n + i]));
+          s[i] += v;
+          if (dz) dz[m * ldd + n + i] = from_f<T>(v);
+        }
+  }
+  if (!db && !part) return;
+#pragma unroll
+  for (int i = 0; i < 8; i++) sums[y][x * 8 + i] = s[i];
+  __syncthreads();
+  const int c = blockIdx.x * DZ_COLUMNS + threadIdx.x;
+  if (threadIdx.x >= DZ_COLUMNS || c >= N) return;
+  float t = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) t += sums[i][threadIdx.x];
+  if (part) part[(int64_t)blockIdx.y * N + c] = t;
+  else db[c] = from_f<T>(t);
+}
+
+// The shares' column sums: 4 waves over the shares, in a fixed order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_db(const float* part, T* db, int N, int shares) {
+  __shared__ float sums[4][64];
+  const int x = threadIdx.x & 63, w = threadIdx.x >> 6, n = blockIdx.x * 64 + x;
+  float s = 0.0f;
+  if (n < N)
+    for (int i = w; i < shares; i += 4) s += part[(int64_t)i * N + n];
+  sums[w][x] = s;
+  __syncthreads();
+  if (w == 0 && n < N) db[n] = from_f<T>((sums[0][x] + sums[1][x]) + (sums[2][x] + sums[3][x]));
+}
+
 // ---- padded copies -----------------------------------------------------------------
 //
 // Rows that do not start on 16 bytes cost the tile kernel guarded loads through
@@ -911,7 +996,7 @@ int dz_rows(int M, int N) {
 bool one_launch(int M, int N, int K, int es, int act) {
   if (K <= 0 || M > 2048 || N > 4096) return false;
   const int64_t k = cdiv(K, 32), cells = (int64_t)M * N * k;
-  return cdiv(M, 32) * k <= 1024 && cdiv(N, 32) * k <= 1024 && cells <= (es == 4 && act > ACT_RELU ? 8 << 20 : 30 << 20);
+  return cdiv(M, 32) * k <= 1024 && cdiv(N, 32) * k <= 1024 && cells <= (es == 4 && act > ACT_RELU ? 7 << 20 : 30 << 20);
 }
 
 // The pieces of a workspace, in their order; bytes 0: not needed.
