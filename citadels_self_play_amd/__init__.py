@@ -11,6 +11,8 @@ resident in HBM; this package is the host side:
                 `CFRNode`, the run_utils functions) over single device lanes;
 * `selfplay`  - one-process-per-GPU drivers (configs 3-5, RCCL pooling);
 * `models` / `train` - ValueOnlyNN and its trainer;
+* `ops`       - linear layer, policy loss and gradient clipping as HIP kernels
+                with gradients, at any size in fp32 / bf16 / fp16;
 * `train_from_scratch`, `compare_to_random`, `generate_test_data` - the
   reference's entry points.
 

@@ -526,7 +526,8 @@ class GameBatch:
         models.ValueNet.  fused (auto: PRED_FUSED): one launch, each tree
         evaluating its leaves in its own kernel (rounds = 0); otherwise leaf rows
         of all suspended trees are evaluated in one MFMA launch per round.
-        Both search bitwise the same trees.  Trees that outgrow their pool are
+        Both search bitwise the same trees.  Nets of a hidden size other than 512
+        are evaluated in rounds (fused auto is then False).  Trees that outgrow their pool are
         searched again with a 4x pool (as cfr_decide).  Returns (chosen, stats
         [B,5], rounds).
 
@@ -543,7 +544,9 @@ class GameBatch:
         if not hasattr(self, "np_mt"):
             self.seed_numpy()
         snap = self._snapshot() if max_retries > 0 else None
-        F = PRED_FUSED if fused == "auto" else bool(fused)
+        if fused not in ("auto", False, 0) and net.wave is None:
+            raise ValueError("leaves in the search kernel need a ValueOnlyNN(418, 512); use fused=False for other nets")
+        F = PRED_FUSED and net.wave is not None if fused == "auto" else bool(fused)
         G = (PRED_GROUPS if self.B >= PRED_GROUP_MIN else 1) if groups == "auto" else max(1, min(int(groups), self.B))
         if F:
             self._groups = None
@@ -607,6 +610,9 @@ class GameBatch:
 
     def _pred_leaves(self, net):
         P = self._pred
+        if net.packed is None:                 # a net without built-in sizes: layer by layer
+            P["probs"].copy_(net.forward(P["feat"]))
+            return
         if P.get("work") is None:
             P["work"] = net.workspace(self.B)
         _lib.check(self.lib.cit_mlp_forward_packed(_ptr(P["feat"]), self.B, net.packed.data_ptr(), _ptr(P["probs"]),

@@ -229,6 +229,11 @@ def main(argv=None):
     ap.add_argument("--phases", type=int, default=5)
     ap.add_argument("--epochs", type=int, default=1000)
     ap.add_argument("--batch-size", type=int, default=2048)
+    ap.add_argument("--max-grad-norm", type=float, default=None,
+                    help="clip each training step's gradients to this global norm (ops.clip_grad_norm; off by default, "
+                         "as in the reference)")
+    ap.add_argument("--fused-linear", action="store_true",
+                    help="train with the layers' products and gradients as ops.linear instead of torch's")
     ap.add_argument("--val", default="validation_targets.pkl", help="generate_test_data output")
     ap.add_argument("--out", default=".")
     ap.add_argument("--seed", type=int, default=0)
@@ -277,7 +282,8 @@ def selfplay_train(feat, value, val, args, lr, folder, dev):
     from .train import train_node_value_only
     return train_node_value_only((feat, value), val, epochs=args.epochs, lr=lr, hidden_size=512,
                                  gamma=0.8851980333411889, batch_size=args.batch_size, device=dev,
-                                 parent_folder=folder)
+                                 parent_folder=folder, max_grad_norm=getattr(args, "max_grad_norm", None),
+                                 fused=getattr(args, "fused_linear", False))
 
 
 if __name__ == "__main__":
