@@ -75,11 +75,11 @@ _SIGS = {
     "cit_linear_forward": ([vp, i64, vp, i64, vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, vp, u64, vp], i32),
     "cit_linear_backward_work_bytes": ([vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32], u64),
     "cit_linear_backward": ([vp, i64, vp, vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, vp, u64, vp], i32),
-    "cit_policy_loss_work_bytes": ([i64], u64),
+    "cit_policy_loss_work_bytes": ([i64, i32, i32], u64),
     "cit_policy_loss": ([vp, i64, vp, i64, vp, i64, vp, i64, i64, i32, vp, vp, vp, vp, f32, f32, f32, i32, vp, vp, vp,
                          vp, vp, u64, vp], i32),
     "cit_policy_loss_backward": ([vp, i64, vp, i64, vp, i64, vp, i64, i64, i32, vp, vp, vp, vp, f32, f32, f32, i32,
-                                  vp, i32, vp, vp], i32),
+                                  vp, i32, vp, vp, u64, vp], i32),
     "cit_clip_grad_norm_work_bytes": ([i32], u64),
     "cit_clip_grad_norm": ([vp, vp, vp, vp, vp, i32, C.c_double, vp, vp, u64, vp], i32),
 }

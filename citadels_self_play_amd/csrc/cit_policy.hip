@@ -36,6 +36,17 @@ struct Policy {
   void* grad;                    // null: no gradient
   const float* upstream;         // backward pass: the loss's gradient; null in the forward pass
   int32_t skip_one;              // backward pass: grad holds upstream = 1 already
+  // a few long rows in parts, a workgroup each: first their sums, then (join) the row's, then the gradient
+  int32_t parts, part_len, mode; // parts 1: whole rows, mode 0; else mode 1 sums, 2 gradient
+  float* part_sums;              // [rows][parts] PartSums
+  float* row_state;              // [rows] RowState
+};
+
+struct PartSums {                // maxima and sums of k_policy's pass 2 over one part
+  float m, mr, s, sr, f;
+};
+struct RowState {                // what the gradient needs of a row
+  float top, top_q, log2_s, L, dlogp, kl, live;
 };
 
 struct Row {
@@ -59,18 +70,19 @@ __device__ __forceinline__ Row row_of(const Policy& a, int64_t i) {
   return r;
 }
 
-// e (x + exp(-x) - 1) from e = exp(a), er = e exp(-x): the series where the three
-// cancel (to 2^-25 of the value at |x| < 1/2), er itself where e is 0.
+// e (x + exp(-x) - 1) from e and er = e exp(-x); where the three would cancel, x^2 e times
+// the Chebyshev interpolation of (x + exp(-x) - 1) / x^2 on |x| <= 1/2 (off by 2^-24).
 __device__ __forceinline__ float kl_term(float e, float er, float x) {
-  float s = 1.0f / 40320.0f;
-  s = fmaf(s, -x, 1.0f / 5040.0f);
-  s = fmaf(s, -x, 1.0f / 720.0f);
-  s = fmaf(s, -x, 1.0f / 120.0f);
-  s = fmaf(s, -x, 1.0f / 24.0f);
-  s = fmaf(s, -x, 1.0f / 6.0f);
-  s = fmaf(s, -x, 0.5f);
-  const float t = fabsf(x) < 0.5f ? e * (x * x * s) : fmaf(e, x - 1.0f, er);
-  return e == 0.0f ? er : t;
+  float s = -0.00019944873929489404f;
+  s = fmaf(s, x, 0.0013982185628265142f);
+  s = fmaf(s, x, -0.0083332359790802f);
+  s = fmaf(s, x, 0.04166579246520996f);
+  s = fmaf(s, x, -0.1666666716337204f);
+  s = fmaf(s, x, 0.5f);
+  // both sides worked out: as a branch a lane takes, either costs both and the exec mask's bookkeeping
+  const float near = x * x * s, far = x - 1.0f;
+  const bool close = fabsf(x) < 0.5f;
+  return fmaf(e, close ? near : far, close ? 0.0f : er);
 }
 
 // Sums and maxima over the G lanes that share a row: shuffles, and LDS between the waves of a wide row.
@@ -103,20 +115,29 @@ struct Lanes {
   }
 };
 
-// What a row's statistics say about the loss: from lse, the action's logit and kl.
+// What a row's statistics say about the loss: from the action's shifted logit
+// l = l_a - m, the sum s of exp(l_j - m), and kl.  The rows' values have either
+// sign and a batch's sum is smaller than they are, so they are worked out and
+// summed in 64 bits.  DOUBLE: the logarithm and exponential too, about 2,400
+// cycles of a wave, where a wave has several rows or a row several waves; a row
+// to a wave takes the 32-bit functions (65,536 x 1,000 bf16: 125 us, 145 with the
+// others).
 struct Verdict {
-  float logp, kl, dlogp, loss;
+  float logp, kl, dlogp;
+  double loss;
 };
 
-__device__ __forceinline__ Verdict judge(const Policy& a, int64_t i, float logp, float kl) {
+template <bool DOUBLE>
+__device__ __forceinline__ Verdict judge(const Policy& a, int64_t i, double l, double s, float kl) {
   Verdict v;
-  v.logp = logp, v.kl = kl;
-  const float adv = a.adv[i], ratio = expf(logp - a.old[i]);
-  const float free = ratio * adv;
-  const float clipped = ratio < 1.0f - a.low ? 1.0f - a.low : ratio > 1.0f + a.high ? 1.0f + a.high : ratio;
-  const float held = clipped * adv;
-  v.dlogp = free <= held ? -free : held < free ? 0.0f : NAN;
-  v.loss = (free <= held || free != free ? -free : -held) + (a.ref ? a.beta * kl : 0.0f);
+  const double logp = l - (DOUBLE ? log(s) : (double)logf((float)s));
+  const double adv = a.adv[i], past = logp - (double)a.old[i];
+  const double ratio = DOUBLE ? exp(past) : (double)expf((float)past);
+  const double low = 1.0 - (double)a.low, high = 1.0 + (double)a.high;
+  const double free = ratio * adv, held = (ratio < low ? low : ratio > high ? high : ratio) * adv;
+  v.logp = (float)logp, v.kl = kl;
+  v.dlogp = (float)(free <= held ? -free : held < free ? 0.0 : (double)NAN);
+  v.loss = (free <= held || free != free ? -free : -held) + (a.ref ? (double)a.beta * (double)kl : 0.0);
   return v;
 }
 
@@ -151,6 +172,20 @@ struct Pack {
     uint16_t h;
     __builtin_memcpy(&h, &v, 2);
     w[k >> 1] = k & 1 ? (w[k >> 1] & 0xffffu) | ((uint32_t)h << 16) : (w[k >> 1] & 0xffff0000u) | h;
+  }
+  // All of them at once: two 16-bit conversions are one instruction.
+  __device__ __forceinline__ void set_all(const float (&f)[E]) {
+    if (sizeof(T) == 4 || E == 1) {
+#pragma unroll
+      for (int k = 0; k < E; k++) set(k, f[k]);
+      return;
+    }
+    typedef T Two __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int k = 0; k + 1 < E; k += 2) {
+      const Two t = {from_f<T>(f[k]), from_f<T>(f[k + 1])};
+      __builtin_memcpy(&w[k >> 1], &t, 4);
+    }
   }
   // Not to be unpacked once for all passes: that doubles the registers a row takes.
   __device__ __forceinline__ void keep_packed() {
@@ -214,24 +249,39 @@ __device__ void clear_ends(const Policy& a, int block, int blocks) {
 }
 
 #define LOG2E 1.44269504088896341f
-#define LN2 0.693147180559945309f
+
+// exp(x), and exp(x - ln s) from log2 s.  FINE: to the last place, for short rows; over long ones what the product
+// x log2(e) is off by, |x| last places, averages out, and the instruction alone does (fp32 2,048 x 16,384: 93 us, 108).
+template <bool FINE>
+__device__ __forceinline__ float exp_of(float x) {
+  return FINE ? expf(x) : __builtin_amdgcn_exp2f(x * LOG2E);
+}
+template <bool FINE>
+__device__ __forceinline__ float exp_less(float x, float log2_s) {
+  return FINE ? expf(fmaf(log2_s, -0.693147180559945309f, x)) : __builtin_amdgcn_exp2f(fmaf(x, LOG2E, -log2_s));
+}
 
 // A row by G lanes, each with up to NV packs of E entries in registers, so that
 // the logits come from memory once; a longer row is read again in each pass.
 //
-//   pass 1  the maxima of l and of the reference r
-//   pass 2  with powers of two (v_exp_f32):  e = 2^(l log2(e) - m2), m2 a whole
-//           number; x = l - r - c0 and er = e exp(-x), c0 the difference of the
-//           maxima on a grid of log(2) / 4096 (m2 and c0's power of two exact: no
-//           error that all entries share).  s = sum e, sr = sum er, F = sum e (x + exp(-x) - 1):
-//           with eta = 1 - sr / s,  d = x - L, L = -log1p(-eta), and
+//   pass 1  the maxima m of l and mr of the reference r
+//   pass 2  e = exp(l - m), er = exp(r - mr) (a difference first, so
+//           that no error is shared by all entries and a type's lowest value is
+//           a number like others), x = (l - m) - (r - mr), hence er = e exp(-x).
+//           s = sum e, sr = sum er, F = sum e (x + exp(-x) - 1): with
+//           eta = 1 - sr / s,  d = x - L, L = -log1p(-eta), and
 //           KL = F / s + eta - L.  One pass gives KL without its cancellation.
-//   pass 3  the gradient: p = 2^(l log2(e) - log2(e) lse), one exp more
-template <typename T, int G, int NV, int E, bool REF>
-__global__ __launch_bounds__(G > 256 ? G : 256, G > 256 ? 4 : 2) void k_policy(Policy a, int row_blocks) {
+//   pass 3  the gradient: p = exp(l - m - log s), one exp more
+//
+// bf16 with a reference is bound by the vector units (about 50 operations an
+// entry, 12 of them the three exponentials), the others by memory.
+template <typename T, int G, int NV, int E, bool REF, bool PARTED>
+__global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 ? 4 : E > 1 && REF && !PARTED ? 5 : 2) void k_policy(Policy a, int row_blocks) {
   constexpr int THREADS = G > 256 ? G : 256, GROUPS = THREADS / G;
+  constexpr bool FINE = E == 1;
   __shared__ double sums[GROUPS];
   __shared__ float between[G > 64 ? G / 64 : 1][4];
+  __shared__ Verdict said;
   const float up = a.upstream ? *a.upstream : 1.0f;
   if (a.upstream && a.skip_one && up == 1.0f) return;
   if ((int)blockIdx.x >= row_blocks) {
@@ -239,19 +289,30 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 256 ? 4 : 2) void k_policy(P
     return;
   }
   const int lane = threadIdx.x % G;
-  const int64_t i = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G;
+  int64_t i = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G;
+  int part = 0;
+  if (PARTED) {
+    part = (int)(i % a.parts);
+    i /= a.parts;
+  }
   const Lanes<G> lanes{between};
   double counted = 0.0;
   if (i < a.rows) {              // the same for all lanes of a row: barriers inside are met by all of a wide row
-    const Row r = row_of(a, i);
+    Row r = row_of(a, i);
+    if (PARTED) {
+      const int skip = part * a.part_len;
+      r.at += skip, r.at_ref += skip, r.at_mask += skip, r.at_grad += skip;
+      r.len = r.len - skip < a.part_len ? r.len - skip : a.part_len;
+    }
     const float w = weight_of(a, i);
     const T* lrow = static_cast<const T*>(a.logits) + r.at;
     const T* qrow = REF ? static_cast<const T*>(a.ref) + r.at_ref : nullptr;
     const uint8_t* ok = a.mask ? a.mask + r.at_mask : nullptr;
     T* grow = a.grad ? static_cast<T*>(a.grad) + r.at_grad : nullptr;
-    Verdict v = {0.0f, 0.0f, 0.0f, 0.0f};
+    Verdict v = {0.0f, 0.0f, 0.0f, 0.0};
     bool live = w != 0.0f && !r.bad;
-    float lse2 = 0.0f, c0 = 0.0f, shift = 0.0f;
+    const float of_action = !PARTED && live ? action_logit<T>(a, r, i) : 0.0f;
+    float top = 0.0f, top_q = 0.0f, log2_s = 0.0f, L = 0.0f;
     const bool held = r.len <= G * NV * E;
     Pack<T, E> l[NV], q[NV];
     // f(j, l, q) for every pack of the row this lane has
@@ -272,7 +333,6 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 256 ? 4 : 2) void k_policy(P
       }
     };
     if (live) {
-      const float old_action = action_logit<T>(a, r, i);
       if (held) {
 #pragma unroll
         for (int n = 0; n < NV; n++) {
@@ -283,77 +343,99 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 256 ? 4 : 2) void k_policy(P
           }
         }
       }
-      float m[2] = {-INFINITY, -INFINITY};
-      visit([&](int, const Pack<T, E>& x, const Pack<T, E>& y) {
+    }
+    if (PARTED && a.mode == 2) {
+      const RowState* state = reinterpret_cast<const RowState*>(a.row_state) + i;
+      live = state->live != 0.0f;
+      top = state->top, top_q = state->top_q, log2_s = state->log2_s, L = state->L;
+      v.dlogp = state->dlogp, v.kl = state->kl;
+    } else if (live) {
+      float m[REF ? 2 : 1];
+      for (float& k : m) k = -INFINITY;
+      visit([&](int, const Pack<T, E>& x, const Pack<T, E>& y) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < E; k++) {
           m[0] = fmaxf(m[0], x.get(k));
-          if (REF) m[1] = fmaxf(m[1], y.get(k));
+          if (REF) m[REF ? 1 : 0] = fmaxf(m[REF ? 1 : 0], y.get(k));
         }
       });
-      lanes.template all<2, true>(m);
-      // Far from 0 (a type's lowest value as a mask) the scaled exponents would leave fp32: such a row is moved
-      // by its maximum first, which a softmax does not see.
-      shift = fabsf(m[0]) > 1e30f && fabsf(m[0]) < INFINITY ? m[0] : 0.0f;
-      const float shift_q = REF && fabsf(m[1]) > 1e30f && fabsf(m[1]) < INFINITY ? m[1] : 0.0f;
-      const float top = m[0] - shift, top_q = m[1] - shift_q;
-      const float m2 = top == -INFINITY ? 0.0f : ceilf(top * LOG2E);
-      float c2 = 0.0f;
-      if (REF) c2 = rintf((top - top_q) * (LOG2E * 4096.0f)) * (1.0f / 4096.0f);
-      if (!(fabsf(c2) < 1e30f)) c2 = 0.0f;
-      c0 = c2 * LN2 + shift - shift_q;
-      const float at_q = c2 - m2;
-      float t[3] = {0.0f, 0.0f, 0.0f};
-      visit([&](int, const Pack<T, E>& x, const Pack<T, E>& y) {
+      lanes.template all<REF ? 2 : 1, true>(m);
+      top = m[0] == -INFINITY ? 0.0f : m[0];
+      if (REF) top_q = m[REF ? 1 : 0] == -INFINITY ? 0.0f : m[REF ? 1 : 0];
+      float t[REF ? 3 : 1] = {};
+      visit([&](int, const Pack<T, E>& x, const Pack<T, E>& y) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < E; k++) {
-          const float lx = x.get(k) - shift;
-          const float e = __builtin_amdgcn_exp2f(fmaf(lx, LOG2E, -m2));
+          const float dl = x.get(k) - top;
+          const float e = exp_of<FINE>(dl);
           t[0] += e;
           if (REF) {
-            const float qx = y.get(k) - shift_q;
-            const float er = __builtin_amdgcn_exp2f(fmaf(qx, LOG2E, at_q));
-            t[1] += er;
-            t[2] += kl_term(e, er, lx - qx - c2 * LN2);
+            const float dr = y.get(k) - top_q;
+            const float er = exp_of<FINE>(dr);
+            t[REF ? 1 : 0] += er;
+            // an entry of no probability (l = -inf, and r perhaps too) is finite here: it counts er
+            t[REF ? 2 : 0] += kl_term(e, er, fmaxf(dl - dr, -200.0f));
           }
         }
       });
-      lanes.template all<3, false>(t);
+      lanes.template all<REF ? 3 : 1, false>(t);
+      if (PARTED && a.mode == 1) {
+        if (lane == 0)
+          reinterpret_cast<PartSums*>(a.part_sums)[i * a.parts + part] =
+              PartSums{m[0], m[REF ? 1 : 0], t[0], REF ? t[REF ? 1 : 0] : 0.0f, REF ? t[REF ? 2 : 0] : 0.0f};
+        return;
+      }
       live = !(t[0] == 0.0f);
       if (live) {
-        lse2 = m2 + __builtin_amdgcn_logf(t[0]);
+        log2_s = __builtin_amdgcn_logf(t[0]);
         float kl = 0.0f;
         if (REF) {
-          const float eta = (t[0] - t[1]) / t[0], L = -log1pf(-eta);
-          kl = t[2] / t[0] + (fabsf(eta) < 0.01f ? -eta * eta * fmaf(eta, fmaf(eta, 0.25f, 1.0f / 3.0f), 0.5f) : eta - L);
+          const float eta = (t[0] - t[REF ? 1 : 0]) / t[0];
+          L = -log1pf(-eta);
+          kl = t[REF ? 2 : 0] / t[0] + (fabsf(eta) < 0.01f ? -eta * eta * fmaf(eta, fmaf(eta, 0.25f, 1.0f / 3.0f), 0.5f) : eta - L);
           kl = kl < 0.0f ? 0.0f : kl;
-          c0 += L;               // d = l - r - c0 from here on
         }
-        v = judge(a, i, (old_action - shift) - lse2 * LN2, kl);
+        const double l_a = (double)of_action - top;
+        if (G > 64) {            // the first wave for all
+          if (threadIdx.x < 64) {
+            v = judge<true>(a, i, l_a, t[0], kl);
+            if (threadIdx.x == 0) said = v;
+          }
+          __syncthreads();
+          v = said;
+        } else {
+          v = judge<G != 64>(a, i, l_a, t[0], kl);
+        }
       }
     }
-    if (r.bad && w != 0.0f) v = {NAN, NAN, NAN, NAN};
-    if (!a.upstream && lane == 0) {
+    if (PARTED && a.mode == 1) return;
+    if (r.bad && w != 0.0f) v = {NAN, NAN, NAN, (double)NAN};
+    if (!a.upstream && !PARTED && lane == 0) {
       a.logp[i] = v.logp, a.kl[i] = v.kl;
-      counted = w != 0.0f ? (double)w * (double)v.loss : 0.0;
+      counted = w != 0.0f ? (double)w * v.loss : 0.0;
     }
     if (grow) {
-      const int64_t action = a.actions[i];
+      const int64_t action = PARTED ? a.actions[i] - (int64_t)part * a.part_len : a.actions[i];
       const float uw = up * w;
       if (live) {
         const float bw = REF ? uw * a.beta : 0.0f;
-        const float flat = -uw * v.dlogp - (bw != 0.0f ? bw * (c0 + v.kl) : 0.0f);   // p (bw (l - r) + flat)
-        visit([&](int j, const Pack<T, E>& x, const Pack<T, E>& y) {
-          Pack<T, E> g = x;
+        const float flat = -uw * v.dlogp - (bw != 0.0f ? bw * (L + v.kl) : 0.0f);    // p (bw x + flat)
+        auto prob = [&](float lx) __attribute__((always_inline)) {
+          return exp_less<FINE>(lx - top, log2_s);
+        };
+        // x within what times 0 is 0: an entry of no probability has no gradient
+        auto slope = [&](float lx, float qx) __attribute__((always_inline)) {
+          return REF ? fmaf(bw, fminf(fmaxf((lx - top) - (qx - top_q), -1e30f), 1e30f), flat) : flat;
+        };
+        visit([&](int j, const Pack<T, E>& x, const Pack<T, E>& y) __attribute__((always_inline)) {
+          Pack<T, E> g = {};
+          float o[E];
 #pragma unroll
           for (int k = 0; k < E; k++) {
             const float lx = x.get(k);
-            const float p = __builtin_amdgcn_exp2f(fmaf(lx - shift, LOG2E, -lse2));
-            float d = flat;
-            if (REF) d = bw != 0.0f ? fmaf(bw, lx - y.get(k), flat) : flat;
-            d = p == 0.0f ? flat : d;                // an entry of no probability: 0, not 0 times infinity
-            g.set(k, p * d);
+            o[k] = prob(lx) * slope(lx, REF ? y.get(k) : 0.0f);
           }
+          g.set_all(o);
           store_pack<T, E>(grow, j, r.len, g);
           if (action >= j && action < j + E && action < r.len) {
             // the chosen entry has uw dlogp besides; its lane has just stored the pack
@@ -365,9 +447,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 256 ? 4 : 2) void k_policy(P
                 lx = x.get(c);
                 if (REF) qx = y.get(c);
               }
-            const float p = __builtin_amdgcn_exp2f(fmaf(lx - shift, LOG2E, -lse2));
-            float d = REF && bw != 0.0f && p != 0.0f ? fmaf(bw, lx - qx, flat) : flat;
-            if (!(ok && !ok[action])) grow[action] = from_f<T>(fmaf(p, d, uw * v.dlogp));
+            if (!(ok && !ok[action])) grow[action] = from_f<T>(fmaf(prob(lx), slope(lx, qx), uw * v.dlogp));
           }
         });
       } else {
@@ -376,7 +456,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 256 ? 4 : 2) void k_policy(P
       }
     }
   }
-  if (a.upstream) return;
+  if (a.upstream || PARTED) return;
   if (lane == 0) sums[threadIdx.x / G] = counted;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -384,6 +464,58 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 256 ? 4 : 2) void k_policy(P
     for (int k = 0; k < GROUPS; k++) s += sums[k];
     a.part[blockIdx.x] = s;
   }
+}
+
+// The parts of a row together, a wave a row.  With a = exp(m_part - m) and the
+// shift of x, delta = (m_part - m) - (mr_part - mr):
+//   sum e (x + exp(-x) - 1) = a (F_part + delta (s_part - sr_part) + (delta + exp(-delta) - 1) sr_part)
+template <typename T>
+__global__ __launch_bounds__(64) void k_policy_join(Policy a) {
+  const float up = a.upstream ? *a.upstream : 1.0f;
+  if (a.upstream && a.skip_one && up == 1.0f) return;
+  const int64_t i = blockIdx.x;
+  const int lane = threadIdx.x;
+  const float w = weight_of(a, i);
+  const Row r = row_of(a, i);
+  const bool ref = a.ref != nullptr;
+  PartSums p = {-INFINITY, -INFINITY, 0.0f, 0.0f, 0.0f};
+  if (w != 0.0f && lane < a.parts) p = reinterpret_cast<const PartSums*>(a.part_sums)[i * a.parts + lane];
+  const float m = wave_max(p.m), mr = wave_max(p.mr);
+  const float top = m == -INFINITY ? 0.0f : m, top_q = !ref || mr == -INFINITY ? 0.0f : mr;
+  double s = 0.0, sr = 0.0, f = 0.0;
+  if (p.s != 0.0f) {                                 // NaN too
+    const double x = (double)p.m - top, y = exp(x);
+    s = y * p.s;
+    if (ref) {
+      const double delta = x - ((double)p.mr - top_q);
+      f = p.sr == 0.0f ? y * (p.f + delta * p.s)
+                       : y * (p.f + delta * ((double)p.s - p.sr) + (delta + expm1(-delta)) * p.sr);
+    }
+  }
+  if (ref && p.sr != 0.0f) {
+    sr = exp((double)p.mr - top_q) * p.sr;
+    if (p.s == 0.0f) f = sr;
+  }
+  s = wave_sum(s), sr = wave_sum(sr), f = wave_sum(f);
+  if (lane) return;
+  Verdict v = {0.0f, 0.0f, 0.0f, 0.0};
+  RowState state = {top, top_q, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  if (w != 0.0f && !(s == 0.0)) {
+    float kl = 0.0f;
+    if (ref) {
+      const double eta = (s - sr) / s, L = -log1p(-eta);
+      state.L = (float)L;
+      kl = (float)(f / s + (fabs(eta) < 1e-4 ? -eta * eta * (0.5 + eta / 3.0) : eta - L));
+      kl = kl < 0.0f ? 0.0f : kl;
+    }
+    state.log2_s = (float)log2(s);
+    v = judge<true>(a, i, (double)action_logit<T>(a, r, i) - top, s, kl);
+    state.dlogp = v.dlogp, state.kl = v.kl, state.live = 1.0f;
+  }
+  reinterpret_cast<RowState*>(a.row_state)[i] = state;
+  if (a.upstream) return;
+  a.logp[i] = v.logp, a.kl[i] = v.kl;
+  a.part[i] = w != 0.0f ? (double)w * v.loss : 0.0;
 }
 
 #define SUM_BLOCKS 256
@@ -427,17 +559,36 @@ int64_t row_blocks(int64_t rows, const Shape& s) {
   return (rows + groups - 1) / groups;
 }
 
-template <typename T, int G, int NV, int E>
+// Workgroups for each of a few long dense rows, 1 where the rows fill the chip or are short; parts of whole packs.
+// 8 rows of 131,072 bf16 entries, gradient included: 46 us whole, 25 in parts.
+int parts_of(int64_t rows, int width, bool ragged) {
+  if (ragged || rows > 128 || width < 16384) return 1;
+  int64_t parts = 512 / rows;
+  if (parts > 64) parts = 64;
+  const int most = (int)(((int64_t)width + 4095) / 4096);              // 4,096 entries are held by 256 lanes in any type
+  return parts < most ? (int)parts : most;
+}
+int part_len(int width, int parts) { return ((width - 1) / parts + 1 + 7) / 8 * 8; }
+
+template <typename T, int G, int NV, int E, bool PARTED = false>
 void launch_shape(const Policy& a, int64_t blocks, hipStream_t stream) {
   const int tail = a.grad && a.offsets ? 64 : 0;
   const dim3 grid((unsigned)(blocks + tail)), block(G > 256 ? G : 256);
-  if (a.ref) hipLaunchKernelGGL((k_policy<T, G, NV, E, true>), grid, block, 0, stream, a, (int)blocks);
-  else hipLaunchKernelGGL((k_policy<T, G, NV, E, false>), grid, block, 0, stream, a, (int)blocks);
+  if (a.ref) hipLaunchKernelGGL((k_policy<T, G, NV, E, true, PARTED>), grid, block, 0, stream, a, (int)blocks);
+  else hipLaunchKernelGGL((k_policy<T, G, NV, E, false, PARTED>), grid, block, 0, stream, a, (int)blocks);
 }
 
 template <typename T>
-int launch(const Policy& a, const Shape& s, hipStream_t stream) {
+int launch(Policy a, const Shape& s, hipStream_t stream) {
   constexpr int E = 16 / sizeof(T);
+  if (a.parts > 1) {
+    a.mode = 1;
+    launch_shape<T, 256, 4, E, true>(a, a.rows * a.parts, stream);
+    hipLaunchKernelGGL((k_policy_join<T>), dim3((unsigned)a.rows), dim3(64), 0, stream, a);
+    a.mode = 2;
+    if (a.grad) launch_shape<T, 256, 4, E, true>(a, a.rows * a.parts, stream);
+    return launch_status();
+  }
   const int64_t blocks = row_blocks(a.rows, s);
   if (s.lanes == 16) launch_shape<T, 16, 4, 1>(a, blocks, stream);
   else if (s.lanes == 64 && !s.packs) launch_shape<T, 64, 4, 1>(a, blocks, stream);
@@ -446,6 +597,18 @@ int launch(const Policy& a, const Shape& s, hipStream_t stream) {
   else if (s.lanes == 512) launch_shape<T, 512, 8, E>(a, blocks, stream);
   else launch_shape<T, 1024, 8, E>(a, blocks, stream);
   return launch_status();
+}
+
+// Sums and row states of rows in parts, at `work`.
+size_t part_bytes(int64_t rows, int parts) {
+  return parts > 1 ? (size_t)rows * (parts * sizeof(PartSums) + sizeof(RowState)) : 0;
+}
+void set_parts(Policy& a, void* work) {
+  a.parts = parts_of(a.rows, a.width, a.offsets != nullptr);
+  a.part_len = a.parts > 1 ? part_len(a.width, a.parts) : 0;
+  a.mode = 0;
+  a.part_sums = static_cast<float*>(work);
+  a.row_state = a.part_sums + (a.parts > 1 ? a.rows * a.parts * (int64_t)(sizeof(PartSums) / 4) : 0);
 }
 
 int run(const Policy& a, int dtype, hipStream_t stream) {
@@ -469,8 +632,9 @@ bool bad(const Policy& a, int dtype) {
 
 extern "C" {
 
-size_t cit_policy_loss_work_bytes(int64_t rows) {
-  return rows > 0 ? ((size_t)rows + SUM_BLOCKS) * sizeof(double) : 0;
+size_t cit_policy_loss_work_bytes(int64_t rows, int width, int ragged) {
+  if (rows <= 0 || (!ragged && width < 0)) return 0;
+  return ((size_t)rows + SUM_BLOCKS) * sizeof(double) + part_bytes(rows, parts_of(rows, width, ragged != 0));
 }
 
 int cit_policy_loss(const void* logits, int64_t ld, const void* ref, int64_t ld_ref, const uint8_t* mask,
@@ -482,14 +646,16 @@ int cit_policy_loss(const void* logits, int64_t ld, const void* ref, int64_t ld_
               width, low, high, kl_coef, rows > 0 ? (float)(1.0 / (double)rows) : 0.0f, logp, kl,
               static_cast<double*>(work), grad, nullptr, 0};
   if (bad(a, dtype) || !loss || (rows && (!logp || !kl))) return -1;
-  const size_t need = cit_policy_loss_work_bytes(rows);
+  const size_t need = cit_policy_loss_work_bytes(rows, width, offsets != nullptr);
   if (need && (!work || work_bytes < need)) return -1;
+  set_parts(a, a.part + rows + SUM_BLOCKS);
   if (rows) {
     const int rc = run(a, dtype, stream);
     if (rc) return rc;
   }
   const int64_t parts =
-      rows ? row_blocks(rows, shape_of(width_of(rows, total, width, offsets != nullptr), dtype)) : 0;
+      !rows ? 0
+            : a.parts > 1 ? rows : row_blocks(rows, shape_of(width_of(rows, total, width, offsets != nullptr), dtype));
   if (parts > 64 * SUM_BLOCKS) {                     // one workgroup would be at it for longer than two launches take
     double* part = a.part + rows;
     hipLaunchKernelGGL(k_policy_sum, dim3(SUM_BLOCKS), dim3(1024), 0, stream, a.part, parts, part, nullptr);
@@ -504,11 +670,15 @@ int cit_policy_loss_backward(const void* logits, int64_t ld, const void* ref, in
                              int64_t ld_mask, const int64_t* offsets, int64_t total, int64_t rows, int width,
                              const int64_t* actions, const float* old_logp, const float* advantages,
                              const float* weights, float low, float high, float kl_coef, int dtype,
-                             const float* upstream, int skip_one, void* grad, hipStream_t stream) {
+                             const float* upstream, int skip_one, void* grad, void* work, size_t work_bytes,
+                             hipStream_t stream) {
   Policy a = {logits, ref, mask, offsets, actions, old_logp, advantages, weights, ld, ld_ref, ld_mask, rows, total,
               width, low, high, kl_coef, rows > 0 ? (float)(1.0 / (double)rows) : 0.0f, nullptr, nullptr, nullptr,
               grad, upstream, skip_one};
   if (bad(a, dtype) || !upstream || (rows && !grad)) return -1;
+  const size_t need = part_bytes(rows, parts_of(rows, width, offsets != nullptr));
+  if (need && (!work || work_bytes < need)) return -1;
+  set_parts(a, work);
   return rows ? run(a, dtype, stream) : 0;
 }
 

@@ -243,9 +243,9 @@ def _policy_forward(given, want_grad):
         grad = _empty(logits.shape, dtype=logits.dtype, device=dev)
         if not rows:
             grad.zero_()
-    n = lib.cit_policy_loss_work_bytes(rows)
-    work = _empty(n, dtype=torch.uint8, device=dev) if n else None
     keep, args = _policy_args(*given)
+    n = lib.cit_policy_loss_work_bytes(rows, args[9], args[6] is not None)
+    work = _empty(n, dtype=torch.uint8, device=dev) if n else None
     rc = _on(logits.get_device(), lib.cit_policy_loss, *args, loss.data_ptr(), logp.data_ptr(), kl.data_ptr(),
              _ptr(grad), _ptr(work), n)
     if rc:
@@ -270,8 +270,10 @@ def _policy_backward(ctx, up):
         up = up.float()
     lib = _lib.load()
     keep, args = _policy_args(*given)
+    n = lib.cit_policy_loss_work_bytes(args[8], args[9], args[6] is not None)
+    work = _empty(n, dtype=torch.uint8, device=logits.device) if n else None
     rc = _on(logits.get_device(), lib.cit_policy_loss_backward, *args, up.data_ptr(), 1 if ready else 0,
-             grad.data_ptr())
+             grad.data_ptr(), _ptr(work), n)
     if rc:
         _lib.check(rc, "cit_policy_loss_backward")
     return (grad,) + (None,) * 10

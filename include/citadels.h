@@ -433,8 +433,9 @@ int cit_linear_backward(const void* dy, int64_t ldy, const void* z, const void* 
  * the gradient of the loss (dense rows without gaps; list entries of no
  * position get 0).  cit_policy_loss_backward writes the gradient times
  * upstream[0]; with skip_one, grad holds cit_policy_loss's and stays as it is
- * if that is 1. */
-size_t cit_policy_loss_work_bytes(int64_t rows);
+ * if that is 1.  Either workspace is of cit_policy_loss_work_bytes(rows, width,
+ * ragged: offsets given). */
+size_t cit_policy_loss_work_bytes(int64_t rows, int width, int ragged);
 int cit_policy_loss(const void* logits, int64_t ld, const void* ref, int64_t ld_ref, const uint8_t* mask,
                     int64_t ld_mask, const int64_t* offsets, int64_t total, int64_t rows, int width,
                     const int64_t* actions, const float* old_logp, const float* advantages, const float* weights,
@@ -444,7 +445,8 @@ int cit_policy_loss_backward(const void* logits, int64_t ld, const void* ref, in
                              int64_t ld_mask, const int64_t* offsets, int64_t total, int64_t rows, int width,
                              const int64_t* actions, const float* old_logp, const float* advantages,
                              const float* weights, float low, float high, float kl_coef, int dtype,
-                             const float* upstream, int skip_one, void* grad, hipStream_t stream);
+                             const float* upstream, int skip_one, void* grad, void* work, size_t work_bytes,
+                             hipStream_t stream);
 
 /* norm[0] = sqrt(sum of all squares) of `tensors` gradients (host arrays of
  * device pointers, element counts and types) and, unless out is NULL,

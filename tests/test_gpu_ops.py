@@ -411,19 +411,44 @@ def test_policy_rows_that_count_nothing(dtype):
     got, grad = check_policy(a)
     assert got.logp[1:5].tolist() == [0.0] * 4 and got.kl[1:5].tolist() == [0.0] * 4
     assert not bool(grad[off[1]:off[5]].any())
-    # the same rows as a table
-    b = policy_rows(None, DT[dtype], dense=(4, 2000))
-    b["mask"] = torch.ones_like(b["logits"], dtype=torch.bool)
-    b["mask"][0] = False
-    b["logits"][1] = -math.inf
-    b["logits"][2] = math.nan
-    b["weights"][2] = 0.0
-    got, grad = check_policy(b)
-    assert not bool(grad[:3].any()) and got.logp[:3].tolist() == [0.0] * 3
+    # the same rows as a table, one that a workgroup a row takes and one whose rows are taken in parts
+    for width in (2000, 20000):
+        b = policy_rows(None, DT[dtype], dense=(4, width))
+        b["mask"] = torch.ones_like(b["logits"], dtype=torch.bool)
+        b["mask"][0] = False
+        b["logits"][1] = -math.inf
+        b["logits"][2] = math.nan
+        b["weights"][2] = 0.0
+        got, grad = check_policy(b)
+        assert not bool(grad[:3].any()) and got.logp[:3].tolist() == [0.0] * 3
+
+
+def test_policy_long_rows_with_everything_in_one_part():
+    """Rows in parts where one part holds all that is legal, or all of the reference's mass."""
+    for where in (slice(0, 4000), slice(30000, 34000)):
+        a = policy_rows(None, torch.float32, dense=(2, 65536))
+        a["mask"] = torch.zeros_like(a["logits"], dtype=torch.bool)
+        a["mask"][:, where] = True
+        a["actions"] = torch.full((2,), where.start + 7, device="cuda")
+        l = torch.where(a["mask"], a["logits"].double(), -math.inf)
+        a["old"] = (l.gather(1, a["actions"][:, None])[:, 0] - torch.logsumexp(l, 1) + 0.05).float()
+        check_policy(a)
+        b = dict(a, mask=None, logits=a["logits"].clone(), ref=a["ref"].clone())
+        b["logits"][~a["mask"]] = -math.inf
+        b["ref"][:, where] += 9.0                    # the reference's mass moves there; outside it keeps some
+        l = b["logits"].double()
+        b["old"] = (l.gather(1, a["actions"][:, None])[:, 0] - torch.logsumexp(l, 1) + 0.05).float()
+        got = call_policy(b, (0.2, 0.2), 0.1)
+        q = torch.log_softmax(b["ref"].double(), 1)
+        lp = torch.log_softmax(l, 1)
+        kl = (lp.exp() * torch.where(lp > -math.inf, lp - q, 0.0)).sum(1)
+        # sums of 4,000 terms with logits of at most 20: see policy_want
+        tol = (2 * 4000 + 200) * U
+        assert bool(((got.kl.double() - kl).abs() <= tol * (1 + kl)).all())
 
 
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("width", [12, 1500])
+@pytest.mark.parametrize("width", [12, 1500, 20001])
 def test_policy_infinities_and_lowest_values(dtype, width):
     """-inf and the type's lowest value as masks inside a row; NaN and infinities under the mask."""
     dt = DT[dtype]
@@ -452,7 +477,7 @@ def test_policy_infinities_and_lowest_values(dtype, width):
     assert float(three.kl[0]) == math.inf and torch.equal(three.kl[1:], one.kl[1:])
 
 
-@pytest.mark.parametrize("width", [8, 3000])
+@pytest.mark.parametrize("width", [8, 3000, 20001])
 def test_policy_bad_rows_are_loud(width):
     a = policy_rows(None, torch.float32, dense=(4, width))
     good = call_policy(a, (0.2, 0.2), 0.1)
@@ -483,10 +508,18 @@ def test_policy_entries_of_no_row():
     pad = lambda t: torch.cat([t.new_full((4,), math.nan), t, t.new_full((300,), math.nan)])  # noqa: E731
     b = dict(a, logits=pad(a["logits"]), ref=pad(a["ref"]), offsets=a["offsets"] + 4)
     la, lb = a["logits"].requires_grad_(), b["logits"].requires_grad_()
-    x, y = call_policy(a, (0.2, 0.2), 0.1, la), call_policy(b, (0.2, 0.2), 0.1, lb)
-    assert all(torch.equal(s.detach(), t.detach()) for s, t in zip(x, y))
-    ga, gb = torch.autograd.grad(x.loss, la)[0], torch.autograd.grad(y.loss, lb)[0]
-    assert torch.equal(gb[4:82], ga) and not bool(gb[:4].any()) and not bool(gb[82:].any())
+    # (the list's mean row length picks the kernel's shape, so the two lists' sums have other orders: both are held to
+    # the bounds of the same rows)
+    want = policy_want(a, (0.2, 0.2), 0.1)
+    for l, c in ((la, a), (lb, b)):
+        got = call_policy(c, (0.2, 0.2), 0.1, l)
+        g = torch.autograd.grad(got.loss, l)[0]
+        for name, x, (v, t) in zip(("loss", "logp", "kl"), got, want):
+            within(x.detach(), v, t, name)
+        if c is b:
+            assert not bool(g[:4].any()) and not bool(g[82:].any())
+            g = g[4:82]
+        within(g, *want[3], what="grad")
     none = ops.policy_loss(lb, a["actions"][:0], a["old"][:0], a["adv"][:0], offsets=a["offsets"][:1])
     assert float(none.loss.detach()) == 0.0 and none.logp.shape == (0,)
     assert not bool(torch.autograd.grad(none.loss, lb)[0].any())

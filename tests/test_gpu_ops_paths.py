@@ -178,7 +178,7 @@ def test_policy_step_over_searched_options():
     grads = torch.autograd.grad(got.loss, params)
     # three fp32 products of at most 549 terms, a softmax of at most 60, a mean
     tol = 600 * U
-    assert abs(float(got.loss.detach()) - float(want)) <= tol * (1 + float(kl.mean()))
+    assert abs(float(got.loss.detach()) - float(want.detach())) <= tol * (1 + float(kl.detach().mean()))
     assert bool(((got.kl.double() - kl).abs() <= tol * (1 + kl)).all())
     for p, q in zip(grads, wgrads):
         assert float((p.double() - q).norm()) <= 4 * tol * float(q.norm()) + tol * 0.01

@@ -116,7 +116,7 @@ def test_entry_points_refuse(lib):
     assert bw(p, 4, None, p, 8, p, 8, p, p, p, 4, 4, 8, 1, 1, p, need, None) == -1
     assert bw(p, 3, p, p, 8, p, 8, p, p, p, 4, 4, 8, 1, 1, p, need, None) == -1
     pl = lib.cit_policy_loss
-    ok = [p, 4, None, 0, None, 0, None, 0, 3, 4, p, p, p, None, 0.2, 0.2, 0.0, 0, p, p, p, None, p, 64, None]
+    ok = [p, 4, None, 0, None, 0, None, 0, 3, 4, p, p, p, None, 0.2, 0.2, 0.0, 0, p, p, p, None, p, 1 << 16, None]
     for at, bad in [(0, None), (1, 3), (8, -1), (9, -1), (10, None), (14, -1.0), (16, math.nan), (17, 3), (18, None),
                     (19, None), (22, None), (23, 0)]:
         a = list(ok)
