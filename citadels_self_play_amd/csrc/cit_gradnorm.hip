@@ -180,6 +180,7 @@ int cit_clip_grad_norm(const void* const* grads, void* const* out, const int64_t
                        const int32_t* out_types, int tensors, double max_norm, float* norm, void* work,
                        size_t work_bytes, hipStream_t stream) {
   if (tensors < 0 || !norm || !work || work_bytes < cit_clip_grad_norm_work_bytes(tensors)) return -1;
+  if ((uintptr_t)work & 15) return -1;
   if (tensors && (!grads || !sizes || !types || (out && !out_types))) return -1;
   if (out && !(max_norm >= 0.0)) return -1;
   int64_t total = 0;

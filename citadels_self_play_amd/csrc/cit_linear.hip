@@ -1086,6 +1086,11 @@ int backward(Mat dy, const void* z, Mat x, Mat w, void* dx, void* dw, void* db, 
   return rc ? rc : launch_status();
 }
 
+// Sides whose 32-bit indexes have room for a tile past the end.
+bool bad_sides(int M, int N, int K) {
+  constexpr int MOST = INT32_MAX - 1023;
+  return M < 0 || N < 0 || K < 0 || M > MOST || N > MOST || K > MOST;
+}
 bool bad_types(int dtype, int act) { return dtype < CIT_FP32 || dtype > CIT_FP16 || act < ACT_NONE || act > ACT_SILU; }
 
 }  // namespace
@@ -1093,12 +1098,12 @@ bool bad_types(int dtype, int act) { return dtype < CIT_FP32 || dtype > CIT_FP16
 extern "C" {
 
 size_t cit_linear_forward_work_bytes(int M, int N, int K, int dtype) {
-  return bad_types(dtype, 0) || M <= 0 || N <= 0 || K <= 0 ? 0 : (size_t)split_bytes(M, N, K, elt(dtype));
+  return bad_types(dtype, 0) || bad_sides(M, N, K) || !M || !N || !K ? 0 : (size_t)split_bytes(M, N, K, elt(dtype));
 }
 
 size_t cit_linear_backward_work_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* dx,
                                       const void* dw, const void* db, int M, int N, int K, int dtype, int act) {
-  return bad_types(dtype, act) ? 0
+  return bad_types(dtype, act) || bad_sides(M, N, K) ? 0
                                : (size_t)backward_layout(x, ldx, w, ldw, dx != nullptr, dw != nullptr, db != nullptr, M,
                                                          N, K, elt(dtype), act)
                                      .bytes();
@@ -1107,11 +1112,11 @@ size_t cit_linear_backward_work_bytes(const void* x, int64_t ldx, const void* w,
 int cit_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
                        int64_t ldr, void* y, void* z, int M, int N, int K, int dtype, int act, void* work,
                        size_t work_bytes, hipStream_t stream) {
-  if (M < 0 || N < 0 || K < 0 || bad_types(dtype, act)) return -1;
+  if (bad_sides(M, N, K) || bad_types(dtype, act)) return -1;
   if (!M || !N) return 0;
   if (!y || (K && (!x || !w || ldx < K || ldw < K)) || (residual && ldr < N)) return -1;
   const size_t need = cit_linear_forward_work_bytes(M, N, K, dtype);
-  if (need && (!work || work_bytes < need)) return -1;
+  if (need && (!work || work_bytes < need || ((uintptr_t)work & 15))) return -1;
   Epilogue e = {};
   e.bias = bias, e.res = residual, e.out = y, e.z = z, e.ldr = ldr, e.ldo = N, e.act = act;
   const Mat a = {x, ldx, M, K, K}, b = {w, ldw, N, K, K};
@@ -1123,11 +1128,11 @@ int cit_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
 int cit_linear_backward(const void* dy, int64_t ldy, const void* z, const void* x, int64_t ldx, const void* w,
                         int64_t ldw, void* dx, void* dw, void* db, int M, int N, int K, int dtype, int act, void* work,
                         size_t work_bytes, hipStream_t stream) {
-  if (M <= 0 || N <= 0 || K < 0 || bad_types(dtype, act)) return -1;
+  if (bad_sides(M, N, K) || !M || !N || bad_types(dtype, act)) return -1;
   if (!dy || ldy < N || (act != ACT_NONE && !z) || (dx && K && (!w || ldw < K)) || (dw && K && (!x || ldx < K)))
     return -1;
   const size_t need = cit_linear_backward_work_bytes(x, ldx, w, ldw, dx, dw, db, M, N, K, dtype, act);
-  if (need && (!work || work_bytes < need)) return -1;
+  if (need && (!work || work_bytes < need || ((uintptr_t)work & 15))) return -1;
   const Mat a = {dy, ldy, M, N, N}, b = {x, ldx, M, K, K}, c = {w, ldw, N, K, K};
   char* p = static_cast<char*>(work);
   if (dtype == CIT_FP32) return backward<float>(a, z, b, c, dx, dw, db, M, N, K, act, p, stream);

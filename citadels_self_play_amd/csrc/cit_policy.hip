@@ -19,6 +19,8 @@
 
 #include "cit_ops.h"
 
+#define LONGEST (1 << 30)          // entries of a row: 32-bit indexes, with room for a step past the end
+
 namespace {
 
 struct Policy {
@@ -60,7 +62,7 @@ __device__ __forceinline__ Row row_of(const Policy& a, int64_t i) {
   r.bad = false;
   if (a.offsets) {
     const int64_t s = a.offsets[i], e = a.offsets[i + 1];
-    r.bad = s < 0 || e < s || e > a.total || e - s > INT32_MAX;
+    r.bad = s < 0 || e < s || e > a.total || e - s > LONGEST;
     r.at = r.at_ref = r.at_mask = r.at_grad = r.bad ? 0 : s;
     r.len = r.bad ? 0 : (int)(e - s);
   } else {
@@ -624,7 +626,7 @@ bool bad(const Policy& a, int dtype) {
   if (!a.rows) return false;
   if (!a.actions || !a.old || !a.adv) return true;
   if (a.offsets) return a.total < 0 || (a.total && !a.logits);
-  if (a.width < 0 || (a.width && !a.logits)) return true;
+  if (a.width < 0 || a.width > LONGEST || (a.width && !a.logits)) return true;
   return a.ld < a.width || (a.ref && a.ld_ref < a.width) || (a.mask && a.ld_mask < a.width);
 }
 
@@ -647,7 +649,7 @@ int cit_policy_loss(const void* logits, int64_t ld, const void* ref, int64_t ld_
               static_cast<double*>(work), grad, nullptr, 0};
   if (bad(a, dtype) || !loss || (rows && (!logp || !kl))) return -1;
   const size_t need = cit_policy_loss_work_bytes(rows, width, offsets != nullptr);
-  if (need && (!work || work_bytes < need)) return -1;
+  if (need && (!work || work_bytes < need || ((uintptr_t)work & 15))) return -1;
   set_parts(a, a.part + rows + SUM_BLOCKS);
   if (rows) {
     const int rc = run(a, dtype, stream);
@@ -677,7 +679,7 @@ int cit_policy_loss_backward(const void* logits, int64_t ld, const void* ref, in
               grad, upstream, skip_one};
   if (bad(a, dtype) || !upstream || (rows && !grad)) return -1;
   const size_t need = part_bytes(rows, parts_of(rows, width, offsets != nullptr));
-  if (need && (!work || work_bytes < need)) return -1;
+  if (need && (!work || work_bytes < need || ((uintptr_t)work & 15))) return -1;
   set_parts(a, work);
   return rows ? run(a, dtype, stream) : 0;
 }

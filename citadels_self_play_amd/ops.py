@@ -22,13 +22,12 @@ import ctypes as C
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
-_MOST = 2 ** 31 - 1
+_MOST, _LONGEST = 2 ** 31 - 1024, 2 ** 30       # a matrix's sides; a row's entries (the kernels' indexes are 32 bits)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current = torch.cuda.current_device
 _empty, _empty_like = torch.empty, torch.empty_like
@@ -59,6 +58,10 @@ def _on(index, call, *args):
         return call(*args, _raw_stream(index))
     with torch.cuda.device(index):
         return call(*args, _raw_stream(index))
+
+
+def _no_graph(what):
+    raise RuntimeError("ops.%s has first derivatives only: its backward pass cannot run with create_graph=True" % what)
 
 
 def _ptr(t):
@@ -134,9 +137,6 @@ def _linear_backward(ctx, dy):
     return dx, dw, db, dy if nr else None, None
 
 
-_linear_backward_once = once_differentiable(_linear_backward)
-
-
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, r, act):
@@ -159,7 +159,9 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return (_linear_backward_once if _grad_on() else _linear_backward)(ctx, dy)
+        if _grad_on():
+            _no_graph("linear")
+        return _linear_backward(ctx, dy)
 
 
 def linear(x, weight, bias=None, residual=None, activation="none"):
@@ -168,7 +170,8 @@ def linear(x, weight, bias=None, residual=None, activation="none"):
     x [..., K], weight [N, K] (nn.Linear's layout), bias [N], residual [..., N],
     all of one type; activation "none", "relu", "gelu" (by erf) or "silu".
     Sums are fp32.  Differentiable in every tensor; under no_grad nothing is
-    kept.  The gradient of the pre-activation is rounded to the type before the
+    kept; there are no second derivatives (create_graph=True raises RuntimeError).
+    The gradient of the pre-activation is rounded to the type before the
     two products that use it (bias gradients are summed before that)."""
     _same_place(x if isinstance(x, torch.Tensor) else torch.empty(0), x=x, weight=weight, bias=bias, residual=residual)
     dt, shape, ws = x.dtype, x.shape, weight.shape
@@ -279,9 +282,6 @@ def _policy_backward(ctx, up):
     return (grad,) + (None,) * 10
 
 
-_policy_backward_once = once_differentiable(_policy_backward)
-
-
 class _PolicyLoss(torch.autograd.Function):
     """The forward kernel has a row's probabilities in hand, so it writes the
     gradient for an upstream gradient of 1 in the same pass over the logits;
@@ -302,7 +302,9 @@ class _PolicyLoss(torch.autograd.Function):
     def backward(ctx, up, _logp, _kl):
         if up is None:
             return (None,) * 11
-        return (_policy_backward_once if _grad_on() else _policy_backward)(ctx, up)
+        if _grad_on():
+            _no_graph("policy_loss")
+        return _policy_backward(ctx, up)
 
 
 def _f32(name, t, N):
@@ -336,10 +338,11 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logits=None, offse
 
     weights [N] default to 1 / N; clip is one number or (low, high); p_ref is the
     softmax of ref_logits (as logits) over the same entries.  Only `logits` has
-    a gradient.  Rows of weight 0 are not read, rows with no legal entry (or
+    a gradient, and no second one.  Rows of weight 0 are not read, rows with no legal entry (or
     nothing over -inf) count nothing: both give logp 0, kl 0 and a gradient of 0.
     A masked action has rho 0; an action outside its row, or offsets that
-    leave the list, give NaN.  KL is infinite where p_ref is 0 and p is not, and
+    leave the list, give NaN (what gradient the entries of no row then have is
+    not defined).  KL is infinite where p_ref is 0 and p is not, and
     NaN where the reference leaves nothing of a row."""
     _same_place(logits if isinstance(logits, torch.Tensor) else torch.empty(0), logits=logits, actions=actions,
                 old_logp=old_logp, advantages=advantages, ref_logits=ref_logits, offsets=offsets, mask=mask,
@@ -363,8 +366,8 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logits=None, offse
     if offsets is None:
         if shape[0] != N:
             raise ValueError("%d rows of logits, %d actions" % (shape[0], N))
-        if shape[1] > _MOST:
-            raise ValueError("a row is over %d entries" % _MOST)
+        if shape[1] > _LONGEST:
+            raise ValueError("a row is over %d entries" % _LONGEST)
     else:
         if offsets.dtype not in (torch.int64, torch.int32) or offsets.shape != (N + 1,):
             raise ValueError("offsets must be [N + 1] whole numbers for %d actions" % N)

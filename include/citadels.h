@@ -403,7 +403,8 @@ int cit_cfr_targets(void* pool, int B, int node_cap, int edge_cap, const int32_t
 /* ---- operators of a net's training step and of serving it (ops.py) ----------
  * Element types of their buffers; matrices are rows of neighbouring elements,
  * `ld` elements apart, at the element's own alignment.  Workspaces belong to
- * one call until it has run. */
+ * one call until it has run, and start on 16 bytes; -1 says that an argument is
+ * wrong, and nothing was launched. */
 #define CIT_FP32 0
 #define CIT_BF16 1
 #define CIT_FP16 2

@@ -648,6 +648,76 @@ def test_clip_same_from_run_to_run():
     assert len({float(ops.grad_norm(g)) for _ in range(5)}) == 1
 
 
+def test_many_short_rows():
+    """More rows than one workgroup sums: the loss is their weighted sum all the same."""
+    n = 300_001
+    g = torch.Generator().manual_seed(0)
+    l = (torch.randn(n, 3, generator=g) * 2).cuda()
+    act = torch.randint(0, 3, (n,), generator=g).cuda()
+    old = torch.log_softmax(l.double(), 1).gather(1, act[:, None])[:, 0].float() + 0.05
+    adv = torch.randn(n, generator=g).cuda()
+    got = ops.policy_loss(l, act, old, adv)
+    lp = torch.log_softmax(l.double(), 1).gather(1, act[:, None])[:, 0]
+    ratio = torch.exp(lp - old.double())
+    value = -torch.minimum(ratio * adv, ratio.clamp(0.8, 1.2) * adv)
+    # each row's ratio is off by what its log probability is (3 exponentials, logits of at most 12), the weight 1 / n by u
+    tol = float(((200 * U + U) * value.abs()).sum()) / n + U * abs(float(value.mean()))
+    assert abs(float(got.loss) - float(value.mean())) <= tol
+
+
+def test_no_second_derivatives():
+    """Asked for, they are refused: never left out in silence."""
+    x, w, b, r, dy = linear_inputs(5, 6, 7, torch.float32, "gelu", True, False)
+    y = ops.linear(x.requires_grad_(), w, b, activation="gelu")
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+    a = policy_rows([4, 5], torch.float32)
+    l = a["logits"].requires_grad_()
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        torch.autograd.grad(call_policy(a, (0.2, 0.2), 0.1, l).loss, l, create_graph=True)
+
+
+def test_offsets_past_32_bits():
+    """Elements behind the 2^31st: the last rows of long inputs against the same rows alone."""
+    M, K, N = 540_000, 4096, 24
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    w, tail = torch.randn(N, K, device="cuda").bfloat16(), torch.randn(300, K, device="cuda").bfloat16()
+    x[-300:] = tail
+    want = tail.double() @ w.double().t()
+    tol = rounded((K + 4) * U * (tail.double().abs() @ w.double().abs().t()), want, torch.bfloat16)
+    y = ops.linear(x, w)
+    within(y[-300:], want, tol, "linear")
+    assert not bool(y[:-300].any())
+    ws = w.clone().requires_grad_()
+    dy = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    dy[-1] = 1.0
+    dw = torch.autograd.grad(ops.linear(x, ws), ws, dy)[0]
+    assert torch.equal(dw, tail[-1:].expand(N, K))
+    del x, y, dy
+    a = policy_rows(None, torch.bfloat16, dense=(3, 32768))
+    l = torch.zeros(66_000, 32768, dtype=torch.bfloat16, device="cuda")
+    l[-3:] = a["logits"]
+    wide = dict(a, logits=l, ref=None, mask=None, weights=torch.zeros(66_000, device="cuda"))
+    wide["weights"][-3:] = a["weights"]
+    for k in ("actions", "old", "adv"):
+        wide[k] = torch.zeros(66_000, dtype=a[k].dtype, device="cuda")
+        wide[k][-3:] = a[k]
+    want = policy_want(dict(a, ref=None), (0.2, 0.2), 0.0)
+    l.requires_grad_()
+    got = call_policy(wide, (0.2, 0.2), 0.0, l)
+    within(got.loss.detach(), *want[0], what="loss")
+    within(got.logp[-3:], *want[1], what="logp")
+    g = torch.autograd.grad(got.loss, l)[0]
+    within(g[-3:], *want[3], what="grad")
+    assert not bool(g[:-3].any())
+    del l, g, got, wide
+    t = torch.zeros(2 ** 31 + 5000, dtype=torch.bfloat16, device="cuda")
+    t[-1], t[-4000] = 3.0, 4.0
+    assert float(ops.clip_grad_norm([t], 1.0)) == 5.0
+    assert abs(float(t[-1]) - 0.6) <= 0.6 * 2 ** -8 and abs(float(t[-4000]) - 0.8) <= 0.8 * 2 ** -8
+    assert not bool(t[:-4000].any())
+
+
 # ---- together ---------------------------------------------------------------------------
 
 def step_of_a_policy(params, x, opts, a, max_norm, lib):

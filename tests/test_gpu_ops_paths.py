@@ -67,7 +67,7 @@ def test_fused_layers_match_the_module():
         for m in (plain, fused):
             m.train(mode)
             y = m(x)
-            got.append(float((y.double() - ref).abs().max()) / scale)
+            got.append(float((y.detach().double() - ref.detach()).abs().max()) / scale)
         # the fused sums are bounded like torch's: both are fp32 of the same terms (418 of them at most)
         assert got[1] <= max(4 * got[0], 418 * U), got
     grads = []

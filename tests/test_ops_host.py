@@ -98,8 +98,8 @@ def test_clip_refuses():
 
 def test_entry_points_refuse(lib):
     """Null or short buffers, unknown types, strides under a row: -1 before any launch."""
-    b = C.create_string_buffer(1 << 16)
-    p = C.addressof(b)
+    b = C.create_string_buffer(1 << 17)
+    p = (C.addressof(b) + 255) // 256 * 256
     fw = lib.cit_linear_forward
     assert fw(p, 8, p, 8, None, None, 0, p, None, 4, 4, 8, 3, 0, None, 0, None) == -1
     assert fw(p, 8, p, 8, None, None, 0, p, None, 4, 4, 8, 0, 4, None, 0, None) == -1
@@ -108,6 +108,8 @@ def test_entry_points_refuse(lib):
     assert fw(p, 8, p, 8, None, p, 3, p, None, 4, 4, 8, 0, 0, None, 0, None) == -1
     assert fw(p, 8, p, 8, None, None, 0, None, None, 4, 4, 8, 0, 0, None, 0, None) == -1
     assert fw(p, 8, p, 8, None, None, 0, p, None, -1, 4, 8, 0, 0, None, 0, None) == -1
+    assert fw(p, 2 ** 31 - 1, p, 2 ** 31 - 1, None, None, 0, p, None, 4, 4, 2 ** 31 - 1, 0, 0, None, 0, None) == -1
+    assert fw(p, 8, p, 8, None, None, 0, p, None, 2 ** 31 - 1, 4, 8, 0, 0, None, 0, None) == -1
     assert fw(None, 8, None, 8, None, None, 0, None, None, 0, 4, 8, 0, 0, None, 0, None) == 0
     need = lib.cit_linear_backward_work_bytes(p, 4000, p, 4000, p, p, p, 4000, 4000, 4000, 1, 1)
     assert need > 0
@@ -115,10 +117,11 @@ def test_entry_points_refuse(lib):
     assert bw(p, 4000, p, p, 4000, p, 4000, p, p, p, 4000, 4000, 4000, 1, 1, p, need - 1, None) == -1
     assert bw(p, 4, None, p, 8, p, 8, p, p, p, 4, 4, 8, 1, 1, p, need, None) == -1
     assert bw(p, 3, p, p, 8, p, 8, p, p, p, 4, 4, 8, 1, 1, p, need, None) == -1
+    assert bw(p, 4000, p, p, 4000, p, 4000, p, p, p, 4000, 4000, 4000, 1, 1, p + 8, need, None) == -1
     pl = lib.cit_policy_loss
     ok = [p, 4, None, 0, None, 0, None, 0, 3, 4, p, p, p, None, 0.2, 0.2, 0.0, 0, p, p, p, None, p, 1 << 16, None]
     for at, bad in [(0, None), (1, 3), (8, -1), (9, -1), (10, None), (14, -1.0), (16, math.nan), (17, 3), (18, None),
-                    (19, None), (22, None), (23, 0)]:
+                    (19, None), (22, None), (22, p + 4), (23, 0), (9, 2 ** 31 - 1)]:
         a = list(ok)
         a[at] = bad
         assert pl(*a) == -1, (at, bad)
@@ -128,6 +131,7 @@ def test_entry_points_refuse(lib):
     n, neg = (C.c_int64 * 1)(4), (C.c_int64 * 1)(-4)
     t32, t16, t9 = ((C.c_int32 * 1)(v) for v in (0, 1, 9))
     assert cl(ptr, ptr, n, t32, t32, 1, 1.0, p, p, need - 1, None) == -1
+    assert cl(ptr, ptr, n, t32, t32, 1, 1.0, p, p + 8, need, None) == -1
     assert cl(null, ptr, n, t32, t32, 1, 1.0, p, p, need, None) == -1
     assert cl(ptr, null, n, t32, t32, 1, 1.0, p, p, need, None) == -1
     assert cl(ptr, ptr, neg, t32, t32, 1, 1.0, p, p, need, None) == -1
