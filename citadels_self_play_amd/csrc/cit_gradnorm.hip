@@ -100,7 +100,7 @@ __device__ __forceinline__ double norm_of(const double* part, int count, double 
 }
 __device__ __forceinline__ float factor_of(double n, double max_norm) {
   const double c = max_norm / (n + 1e-6);
-  return max_norm == INFINITY || c >= 1.0 ? 1.0f : (float)c;           // a NaN norm makes NaN gradients
+  return c >= 1.0 ? 1.0f : (float)c;                                   // a NaN norm makes NaN gradients, inf / inf too
 }
 
 // work: [0] the factor (fp32), [2] on the partial sums.

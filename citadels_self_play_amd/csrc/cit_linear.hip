@@ -364,8 +364,9 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, 
   constexpr int STEPS = 2;                              // k steps of a tile: 64 bytes of each row
   __shared__ __attribute__((aligned(16))) char lds[2][(BM + BN) * 128];
 
-  const int tile = blockIdx.x, split = blockIdx.y;
-  const int m0 = (tile / tiles_n) * BM, n0 = (tile % tiles_n) * BN;
+  const int64_t tile = (int64_t)blockIdx.z * gridDim.x + blockIdx.x;
+  if (tile >= (int64_t)((M + BM - 1) / BM) * tiles_n) return;
+  const int split = blockIdx.y, m0 = (int)(tile / tiles_n) * BM, n0 = (int)(tile % tiles_n) * BN;
   const int kb = split * k_per_split, ke = min(K, kb + k_per_split);
   Mat a = A, b = B;                                     // the split's share of the reduction
   if (AKS) a.rows = ke; else a.cols = ke;
@@ -505,6 +506,12 @@ __device__ __forceinline__ void arrive() {
   asm volatile("s_barrier" ::: "memory");
 }
 
+// The same for all of its loads, stated rather than left to what a fence at a barrier happens to wait for.
+__device__ __forceinline__ void arrive_all() {
+  __builtin_amdgcn_s_waitcnt(15 << 8 | 7 << 4);                        // vmcnt 0
+  __syncthreads();
+}
+
 template <typename T, bool AKS, bool BKS, int BM, int BN, int WM, int WN, int STAGES, bool AHEAD>
 __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilogue e, int M, int N, int K, int tiles_m,
                                                              int tiles_n, int k_per_split) {
@@ -559,7 +566,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilo
       read(1, here);
       multiply(0);
       // tiles t + 1 .. t + STAGES - 1 are under way, near the end fewer
-      if (STAGES == 2) __syncthreads();
+      if (STAGES == 2) arrive_all();
       else if (steady.value || t + STAGES <= whole) arrive<(STAGES - 2) * LOADS>();
       else arrive<0>();
       if (steady.value || t + STAGES < whole) {
@@ -575,7 +582,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilo
       multiply(0);
       read(1, here);
       multiply(1);
-      __syncthreads();
+      arrive_all();
     }
   };
   auto round = [&](auto steady, int t) __attribute__((always_inline)) {
@@ -593,7 +600,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilo
     else arrive<0>();
     if (whole) read(0, s0);
   } else {
-    __syncthreads();
+    arrive_all();
   }
   int t = 0;
   for (; STAGES > 2 && t + 2 * STAGES <= whole; t += STAGES) round(std::true_type{}, t);    // without a branch
@@ -714,9 +721,10 @@ template <typename T, bool AKS, bool BKS>
 __global__ __launch_bounds__(SMALL_WAVES * 64, 4) void k_gemm_small(Mat A, Mat B, Epilogue e, int M, int N, int K,
                                                                  int tiles_n, int k_per_split) {
   __shared__ __attribute__((aligned(16))) char lds[SMALL_LDS];
-  const int tile = blockIdx.x;
-  small_tile<T, AKS, BKS, false>(A, nullptr, B, e, ACT_NONE, M, N, K, tile / tiles_n * 32, tile % tiles_n * 32,
-                                 blockIdx.y, k_per_split, lds);
+  const int64_t tile = (int64_t)blockIdx.z * gridDim.x + blockIdx.x;
+  if (tile >= (int64_t)((M + 31) / 32) * tiles_n) return;
+  small_tile<T, AKS, BKS, false>(A, nullptr, B, e, ACT_NONE, M, N, K, (int)(tile / tiles_n) * 32,
+                                 (int)(tile % tiles_n) * 32, blockIdx.y, k_per_split, lds);
 }
 
 // A small layer's whole backward pass in one launch: workgroups for 4 columns
@@ -960,7 +968,7 @@ template <typename T, bool AKS, bool BKS>
 int product(Mat A, Mat B, Epilogue e, int M, int N, int K, void* work, hipStream_t stream) {
   const bool d = K > 0 && direct(A, AKS, sizeof(T)) && direct(B, BKS, sizeof(T));
   const Plan p = plan(M, N, K, sizeof(T), d);
-  const dim3 grid(p.tiles_m * p.tiles_n, p.splits);
+  const dim3 tiles = wide_grid((int64_t)p.tiles_m * p.tiles_n), grid(tiles.x, p.splits, tiles.y);
   if (p.splits > 1) e.part = static_cast<float*>(work);
   if (p.tile == TILE_32)
     hipLaunchKernelGGL((k_gemm_small<T, AKS, BKS>), grid, dim3(SMALL_WAVES * 64), 0, stream, A, B, e, M, N, K,

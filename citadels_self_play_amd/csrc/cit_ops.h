@@ -47,6 +47,14 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// A grid of at least `blocks` workgroups of at most 1,024 threads: a dimension's threads have to be under 2^32, so
+// more than 2^21 of them go on in y (those past the last one have nothing to do).
+static inline dim3 wide_grid(int64_t blocks) {
+  constexpr int64_t MOST = 1 << 21;
+  const int64_t y = (blocks + MOST - 1) / MOST;
+  return y <= 1 ? dim3((unsigned)blocks) : dim3((unsigned)MOST, (unsigned)y);
+}
+
 // The launch's own error, as the other entry points report it.
 static inline int launch_status() {
   hipError_t e = hipGetLastError();

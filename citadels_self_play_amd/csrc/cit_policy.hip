@@ -12,7 +12,8 @@
 //
 // lq is the reference's log softmax.  KL is summed as p (d + exp(-d) - 1), which
 // adds sum q - sum p = 0: every term is >= 0, so policies close together
-// keep their digits (sum p d cancels to nothing there).  A row of weight 0 is
+// keep their digits (sum p d cancels to nothing there); where the reference is
+// much the flatter one, whose sum then outweighs KL, as p d.  A row of weight 0 is
 // not read; a row that leaves no entry counts nothing, and the gradients of
 // both are 0.  An action outside its row makes the row NaN.
 #include <type_traits>
@@ -45,7 +46,7 @@ struct Policy {
 };
 
 struct PartSums {                // maxima and sums of k_policy's pass 2 over one part
-  float m, mr, s, sr, f;
+  float m, mr, s, sr, f, d;
 };
 struct RowState {                // what the gradient needs of a row
   float top, top_q, log2_s, L, dlogp, kl, live;
@@ -72,9 +73,9 @@ __device__ __forceinline__ Row row_of(const Policy& a, int64_t i) {
   return r;
 }
 
-// e (x + exp(-x) - 1) from e and er = e exp(-x); where the three would cancel, x^2 e times
+// e (x + exp(-x) - 1) from e, w = e x and er = e exp(-x); where the three would cancel, x w times
 // the Chebyshev interpolation of (x + exp(-x) - 1) / x^2 on |x| <= 1/2 (off by 2^-24).
-__device__ __forceinline__ float kl_term(float e, float er, float x) {
+__device__ __forceinline__ float kl_term(float e, float er, float x, float w) {
   float s = -0.00019944873929489404f;
   s = fmaf(s, x, 0.0013982185628265142f);
   s = fmaf(s, x, -0.0083332359790802f);
@@ -82,9 +83,8 @@ __device__ __forceinline__ float kl_term(float e, float er, float x) {
   s = fmaf(s, x, -0.1666666716337204f);
   s = fmaf(s, x, 0.5f);
   // both sides worked out: as a branch a lane takes, either costs both and the exec mask's bookkeeping
-  const float near = x * x * s, far = x - 1.0f;
-  const bool close = fabsf(x) < 0.5f;
-  return fmaf(e, close ? near : far, close ? 0.0f : er);
+  const float near = x * s * w, far = (w - e) + er;
+  return fabsf(x) < 0.5f ? near : far;
 }
 
 // Sums and maxima over the G lanes that share a row: shuffles, and LDS between the waves of a wide row.
@@ -273,12 +273,14 @@ __device__ __forceinline__ float exp_less(float x, float log2_s) {
 //           s = sum e, sr = sum er, F = sum e (x + exp(-x) - 1): with
 //           eta = 1 - sr / s,  d = x - L, L = -log1p(-eta), and
 //           KL = F / s + eta - L.  One pass gives KL without its cancellation.
+//           Where sr > 2 s that would take sr away from F: D = sum e x, and
+//           KL = D / s - L.
 //   pass 3  the gradient: p = exp(l - m - log s), one exp more
 //
 // bf16 with a reference is bound by the vector units (about 50 operations an
 // entry, 12 of them the three exponentials), the others by memory.
 template <typename T, int G, int NV, int E, bool REF, bool PARTED>
-__global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 ? 4 : E > 1 && REF && !PARTED ? 5 : 2) void k_policy(Policy a, int row_blocks) {
+__global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 ? 4 : E > 1 && REF && !PARTED ? 5 : 2) void k_policy(Policy a, int64_t row_blocks, int tail) {
   constexpr int THREADS = G > 256 ? G : 256, GROUPS = THREADS / G;
   constexpr bool FINE = E == 1;
   __shared__ double sums[GROUPS];
@@ -286,12 +288,13 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
   __shared__ Verdict said;
   const float up = a.upstream ? *a.upstream : 1.0f;
   if (a.upstream && a.skip_one && up == 1.0f) return;
-  if ((int)blockIdx.x >= row_blocks) {
-    clear_ends<T>(a, (int)blockIdx.x - row_blocks, (int)gridDim.x - row_blocks);
+  const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  if (b >= row_blocks) {
+    if (b < row_blocks + tail) clear_ends<T>(a, (int)(b - row_blocks), tail);
     return;
   }
   const int lane = threadIdx.x % G;
-  int64_t i = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G;
+  int64_t i = b * GROUPS + threadIdx.x / G;
   int part = 0;
   if (PARTED) {
     part = (int)(i % a.parts);
@@ -364,7 +367,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
       lanes.template all<REF ? 2 : 1, true>(m);
       top = m[0] == -INFINITY ? 0.0f : m[0];
       if (REF) top_q = m[REF ? 1 : 0] == -INFINITY ? 0.0f : m[REF ? 1 : 0];
-      float t[REF ? 3 : 1] = {};
+      constexpr int SUMS = REF ? 4 : 1;
+      float t[SUMS] = {};
       visit([&](int, const Pack<T, E>& x, const Pack<T, E>& y) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < E; k++) {
@@ -375,16 +379,20 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
             const float dr = y.get(k) - top_q;
             const float er = exp_of<FINE>(dr);
             t[REF ? 1 : 0] += er;
-            // an entry of no probability (l = -inf, and r perhaps too) is finite here: it counts er
-            t[REF ? 2 : 0] += kl_term(e, er, fmaxf(dl - dr, -200.0f));
+            // An entry of no probability (l = -inf, and r perhaps too) is finite here: it counts er.  r = -inf
+            // counts nothing where p is 0 to its last bit.
+            const float d = fmaxf(dl - dr, -200.0f), w = e == 0.0f ? 0.0f : e * d;
+            t[REF ? 2 : 0] += kl_term(e, er, d, w);
+            t[SUMS - 1] += w;
           }
         }
       });
-      lanes.template all<REF ? 3 : 1, false>(t);
+      lanes.template all<SUMS, false>(t);
       if (PARTED && a.mode == 1) {
         if (lane == 0)
           reinterpret_cast<PartSums*>(a.part_sums)[i * a.parts + part] =
-              PartSums{m[0], m[REF ? 1 : 0], t[0], REF ? t[REF ? 1 : 0] : 0.0f, REF ? t[REF ? 2 : 0] : 0.0f};
+              PartSums{m[0], m[REF ? 1 : 0], t[0], REF ? t[REF ? 1 : 0] : 0.0f, REF ? t[REF ? 2 : 0] : 0.0f,
+                       REF ? t[SUMS - 1] : 0.0f};
         return;
       }
       live = !(t[0] == 0.0f);
@@ -394,7 +402,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
         if (REF) {
           const float eta = (t[0] - t[REF ? 1 : 0]) / t[0];
           L = -log1pf(-eta);
-          kl = t[REF ? 2 : 0] / t[0] + (fabsf(eta) < 0.01f ? -eta * eta * fmaf(eta, fmaf(eta, 0.25f, 1.0f / 3.0f), 0.5f) : eta - L);
+          kl = eta < -1.0f ? t[SUMS - 1] / t[0] - L
+                           : t[REF ? 2 : 0] / t[0] + (fabsf(eta) < 0.01f ? -eta * eta * fmaf(eta, fmaf(eta, 0.25f, 1.0f / 3.0f), 0.5f) : eta - L);
           kl = kl < 0.0f ? 0.0f : kl;
         }
         const double l_a = (double)of_action - top;
@@ -464,13 +473,16 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
   if (threadIdx.x == 0) {
     double s = 0.0;
     for (int k = 0; k < GROUPS; k++) s += sums[k];
-    a.part[blockIdx.x] = s;
+    a.part[b] = s;
   }
 }
 
 // The parts of a row together, a wave a row.  With a = exp(m_part - m) and the
 // shift of x, delta = (m_part - m) - (mr_part - mr):
+//   sum e x = a (D_part + delta s_part)
 //   sum e (x + exp(-x) - 1) = a (F_part + delta (s_part - sr_part) + (delta + exp(-delta) - 1) sr_part)
+// where a exp(-delta) = exp(mr_part - mr) stands for the product once delta is
+// not small: either factor may be 0 or infinite alone.
 template <typename T>
 __global__ __launch_bounds__(64) void k_policy_join(Policy a) {
   const float up = a.upstream ? *a.upstream : 1.0f;
@@ -480,25 +492,23 @@ __global__ __launch_bounds__(64) void k_policy_join(Policy a) {
   const float w = weight_of(a, i);
   const Row r = row_of(a, i);
   const bool ref = a.ref != nullptr;
-  PartSums p = {-INFINITY, -INFINITY, 0.0f, 0.0f, 0.0f};
+  PartSums p = {-INFINITY, -INFINITY, 0.0f, 0.0f, 0.0f, 0.0f};
   if (w != 0.0f && lane < a.parts) p = reinterpret_cast<const PartSums*>(a.part_sums)[i * a.parts + lane];
   const float m = wave_max(p.m), mr = wave_max(p.mr);
   const float top = m == -INFINITY ? 0.0f : m, top_q = !ref || mr == -INFINITY ? 0.0f : mr;
-  double s = 0.0, sr = 0.0, f = 0.0;
+  double s = 0.0, sr = 0.0, f = 0.0, d = 0.0;
+  if (ref && p.sr != 0.0f) f = sr = exp((double)p.mr - top_q) * p.sr;  // f: of a part that has no weight in the row
   if (p.s != 0.0f) {                                 // NaN too
     const double x = (double)p.m - top, y = exp(x);
     s = y * p.s;
-    if (ref) {
+    if (ref && y != 0.0) {
       const double delta = x - ((double)p.mr - top_q);
-      f = p.sr == 0.0f ? y * (p.f + delta * p.s)
-                       : y * (p.f + delta * ((double)p.s - p.sr) + (delta + expm1(-delta)) * p.sr);
+      d = y * (p.d + delta * p.s);
+      f = fabs(delta) < 1.0 ? y * (p.f + delta * ((double)p.s - p.sr) + (delta + expm1(-delta)) * p.sr)
+                            : y * (p.f + delta * p.s - p.sr) + sr;
     }
   }
-  if (ref && p.sr != 0.0f) {
-    sr = exp((double)p.mr - top_q) * p.sr;
-    if (p.s == 0.0f) f = sr;
-  }
-  s = wave_sum(s), sr = wave_sum(sr), f = wave_sum(f);
+  s = wave_sum(s), sr = wave_sum(sr), f = wave_sum(f), d = wave_sum(d);
   if (lane) return;
   Verdict v = {0.0f, 0.0f, 0.0f, 0.0};
   RowState state = {top, top_q, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -507,7 +517,7 @@ __global__ __launch_bounds__(64) void k_policy_join(Policy a) {
     if (ref) {
       const double eta = (s - sr) / s, L = -log1p(-eta);
       state.L = (float)L;
-      kl = (float)(f / s + (fabs(eta) < 1e-4 ? -eta * eta * (0.5 + eta / 3.0) : eta - L));
+      kl = (float)(eta < -1.0 ? d / s - L : f / s + (fabs(eta) < 1e-4 ? -eta * eta * (0.5 + eta / 3.0) : eta - L));
       kl = kl < 0.0f ? 0.0f : kl;
     }
     state.log2_s = (float)log2(s);
@@ -575,9 +585,9 @@ int part_len(int width, int parts) { return ((width - 1) / parts + 1 + 7) / 8 * 
 template <typename T, int G, int NV, int E, bool PARTED = false>
 void launch_shape(const Policy& a, int64_t blocks, hipStream_t stream) {
   const int tail = a.grad && a.offsets ? 64 : 0;
-  const dim3 grid((unsigned)(blocks + tail)), block(G > 256 ? G : 256);
-  if (a.ref) hipLaunchKernelGGL((k_policy<T, G, NV, E, true, PARTED>), grid, block, 0, stream, a, (int)blocks);
-  else hipLaunchKernelGGL((k_policy<T, G, NV, E, false, PARTED>), grid, block, 0, stream, a, (int)blocks);
+  const dim3 grid = wide_grid(blocks + tail), block(G > 256 ? G : 256);
+  if (a.ref) hipLaunchKernelGGL((k_policy<T, G, NV, E, true, PARTED>), grid, block, 0, stream, a, blocks, tail);
+  else hipLaunchKernelGGL((k_policy<T, G, NV, E, false, PARTED>), grid, block, 0, stream, a, blocks, tail);
 }
 
 template <typename T>

@@ -526,6 +526,76 @@ def test_policy_entries_of_no_row():
     assert float(ops.policy_loss(la.detach().view(1, -1)[:0], a["actions"][:0], a["old"][:0], a["adv"][:0]).loss) == 0.0
 
 
+def kl_want(l, q):
+    """(KL of the softmaxes of rows l against q, gradient of it in l, their tolerances), in 64 bits.
+
+    An entry's exponential is off by e = (8 max|l| + 3) u: two differences and the product with log2 e round, |l - max|
+    <= 2 max|l|.  A sum adds 100 u: at most 64 entries a lane, then 6 shuffles and 16 waves.  With x = d + L, L the log
+    of the sums' ratio (off by 2 e + 2 * 100 u + 5 u |L|), the two sums that KL comes from are off by e and 100 u of
+    sum p (|x| + 2), and by what e makes of x itself, e (1 + sum q / sum p <= 3)."""
+    lp, lq = torch.log_softmax(l, 1), torch.log_softmax(q, 1)
+    p = lp.exp()
+    d = torch.where(p > 0, lp - lq, 0.0)
+    kl = (p * d).sum(1)
+    real = torch.where(p > 0, l, 0.0)
+    e = (8 * torch.maximum(real.abs().amax(1), q.abs().amax(1)) + 3) * U
+    top = l.amax(1) - q.amax(1)
+    big = (top - (torch.logsumexp(l, 1) - torch.logsumexp(q, 1))).abs()
+    err_l = 2 * e + (200 + 5 * big) * U
+    err = (2 * e + 100 * U) * (4 + (p * d.abs()).sum(1) + 2 * big) + 2 * err_l
+    grad = p * (d - kl[:, None])
+    err_g = p * (2 * e + 100 * U)[:, None] * (d - kl[:, None]).abs() + p * (err_l + err)[:, None] + 8 * U * p * (d.abs() + kl[:, None])
+    return kl, grad, err, err_g
+
+
+def check_kl(logits, ref, want=None):
+    rows = logits.shape[0]
+    l = logits.clone().requires_grad_()
+    zero = torch.zeros(rows, device="cuda")
+    got = ops.policy_loss(l, zero.long(), zero, zero, ref_logits=ref, weights=zero + 1.0, kl_coef=1.0)
+    grad = torch.autograd.grad(got.loss, l)[0]
+    kl, g, err, err_g = want or kl_want(logits.double(), ref.double())
+    within(got.kl, kl, rounded(err, kl, torch.float32), "kl")
+    within(grad, g, rounded(err_g, g, logits.dtype), "grad")
+
+
+KL_SHAPES = [(3, 40), (3, 200), (3, 1500), (3, 6001), (130, 16500), (3, 20001), (2, 70001)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", KL_SHAPES, ids=str)
+def test_policy_reference_much_flatter(shape, dtype):
+    """A policy that is sure of one option, a reference that is of none."""
+    g = torch.Generator().manual_seed(3)
+    l = torch.randn(shape, generator=g)
+    l[:, shape[1] // 2] = 18.0
+    r = 0.1 * torch.randn(shape, generator=g)
+    check_kl(l.to(DT[dtype]).cuda(), r.to(DT[dtype]).cuda())
+    check_kl(r.to(DT[dtype]).cuda(), l.to(DT[dtype]).cuda())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", KL_SHAPES, ids=str)
+def test_policy_entries_far_below_the_others(shape, dtype):
+    """Stretches of a row, whole parts of a long one among them, that have no weight in it, with and without the
+    reference's: what they hold is a number, and counts nothing."""
+    dt = DT[dtype]
+    g = torch.Generator().manual_seed(4)
+    l, r = torch.randn(shape, generator=g).to(dt).cuda(), torch.randn(shape, generator=g).to(dt).cuda()
+    half = shape[1] // 2
+    for low in (-720.0, -1000.0, torch.finfo(dt).min):
+        a = l.clone()
+        a[:, half:] = low
+        kl, grad, err, err_g = kl_want(torch.where(a < -700, -math.inf, a.double()), r.double())
+        check_kl(a, r, (kl, grad, err, err_g))
+        b = r.clone()
+        b[:, half:] = -math.inf                      # ruled out by the reference too
+        want = kl_want(a[:, :half].double(), b[:, :half].double())
+        pad = lambda t: torch.cat([t, t.new_zeros(shape[0], shape[1] - half)], 1)  # noqa: E731
+        if low < -800:                               # (exp(-720) is no 0 to a row in parts)
+            check_kl(a, b, (want[0], pad(want[1]), want[2], pad(want[3])))
+
+
 def test_policy_strides_and_types():
     a = policy_rows(None, torch.float32, dense=(6, 700), masked=0.3)
     want = call_policy(a, (0.2, 0.2), 0.1)
@@ -716,6 +786,53 @@ def test_offsets_past_32_bits():
     assert float(ops.clip_grad_norm([t], 1.0)) == 5.0
     assert abs(float(t[-1]) - 0.6) <= 0.6 * 2 ** -8 and abs(float(t[-4000]) - 0.8) <= 0.8 * 2 ** -8
     assert not bool(t[:-4000].any())
+
+
+def test_clip_by_an_infinite_norm():
+    """max_norm inf clips nothing, and an infinite norm against it makes NaN, as torch's clip_grad_norm_ has it."""
+    for v in (1.0, math.inf, math.nan):
+        t = torch.ones(70, device="cuda")
+        t[3] = v
+        p = torch.nn.Parameter(torch.zeros(70, device="cuda"))
+        p.grad = t.clone()
+        torch.nn.utils.clip_grad_norm_([p], math.inf)
+        ops.clip_grad_norm([t], math.inf)
+        assert torch.equal(t.isnan(), p.grad.isnan()) and torch.equal(t.nan_to_num(), p.grad.nan_to_num())
+
+
+def test_more_workgroups_than_one_dimension_takes():
+    """Past 2^21 workgroups a launch goes on in its grid's next dimension."""
+    M = (1 << 26) + 100
+    x = torch.randn(M, 1, device="cuda").bfloat16()
+    for N in (1, 131):                               # 32 x 32 tiles, 64 x 64 tiles
+        w = torch.randn(N, 1, device="cuda").bfloat16()
+        y = ops.linear(x, w)
+        for at in (0, (1 << 26) - 4000, M - 5000):   # a product of two bf16 numbers is exact in fp32
+            rows = slice(at, at + 5000)
+            assert torch.equal(y[rows], (x[rows].float() * w.float().t()).bfloat16())
+        del y
+    del x
+    N = (1 << 25) + 1000
+    g = torch.Generator(device="cuda").manual_seed(0)
+    l = torch.randn(N, 2, generator=g, device="cuda").half()
+    act = torch.randint(0, 2, (N,), generator=g, device="cuda")
+    zero = torch.zeros(N, device="cuda")
+    one = torch.full((N,), 2.0 ** -10, device="cuda")
+    l.requires_grad_()
+    got = ops.policy_loss(l, act, zero, zero + 1.0, weights=one, clip=(1.0, 1.0))
+    grad = torch.autograd.grad(got.loss, l)[0]
+    total = 0.0
+    for at in range(0, N, 1 << 22):
+        rows = slice(at, min(N, at + (1 << 22)))
+        p = torch.softmax(l[rows].detach().double(), 1).gather(1, act[rows][:, None])[:, 0]
+        total += float(p.sum())
+        # two exponentials, a logarithm of their sum, logits of at most 8
+        assert bool(((got.logp[rows].double() - p.log()).abs() <= 100 * U).all())
+        want = 2.0 ** -10 * p * (1 - p)              # rho = p (old 0): -w p (1 - p) where chosen, w p (1 - p) where not
+        sign = torch.ones(len(p), 2, device="cuda", dtype=torch.float64).scatter_(1, act[rows][:, None], -1.0)
+        want = want[:, None] * sign
+        assert bool(((grad[rows].double() - want).abs() <= want.abs() * (2.0 ** -11 + 300 * U) + 2.0 ** -25).all())
+    assert abs(float(got.loss.detach()) + total * 2.0 ** -10) <= 150 * U * total * 2.0 ** -10
 
 
 # ---- together ---------------------------------------------------------------------------
