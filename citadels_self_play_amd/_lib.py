@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("CIT_LIB_PATH") or os.path.join(HERE, "libcitadels_hip.so")   # override: A/B builds only
 HEADER = os.path.join(os.path.dirname(HERE), "include", "citadels.h")
 
-_lib = None
+_lib = _torch_calls = None
 
 vp, i32, i64, u64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float
 
@@ -119,6 +119,24 @@ def load():
         fn.restype = res
     _lib = lib
     return lib
+
+
+_TORCH_CALLS = ("cit_linear_forward_work_bytes", "cit_linear_forward", "cit_linear_backward_work_bytes",
+                "cit_linear_backward", "cit_policy_loss_work_bytes", "cit_policy_loss", "cit_policy_loss_backward")
+
+
+def torch_calls():
+    """The extension with the operators' autograd nodes (csrc/cit_torch.cpp), over the library that load() gives."""
+    global _torch_calls
+    if _torch_calls is None:
+        lib = load()
+        try:
+            from . import _cit_torch as m
+        except ImportError as e:
+            raise NativeError("_cit_torch.so is not built or does not load (run __graft_entry__.build()): %s" % e) from e
+        m.bind(NativeError, {n: C.cast(getattr(lib, n), C.c_void_p).value for n in _TORCH_CALLS})
+        _torch_calls = m
+    return _torch_calls
 
 
 def check(rc, what):

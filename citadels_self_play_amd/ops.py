@@ -15,7 +15,8 @@ autograd engine joins the two graphs' streams, whatever the operators).
 Wrong arguments raise ValueError before anything is launched.
 
 The checks are written out rather than shared: at a trainer's batch of 64 a
-call's time is the host's.
+call's time is the host's.  What follows them, autograd included, is
+csrc/cit_torch.cpp.
 """
 import collections
 import ctypes as C
@@ -30,8 +31,8 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 _MOST, _LONGEST = 2 ** 31 - 1024, 2 ** 30       # a matrix's sides; a row's entries (the kernels' indexes are 32 bits)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current = torch.cuda.current_device
-_empty, _empty_like = torch.empty, torch.empty_like
-_grad_on = torch.is_grad_enabled
+_empty = torch.empty
+_calls = _lib.torch_calls
 
 
 def _same_place(first, **others):
@@ -60,109 +61,7 @@ def _on(index, call, *args):
         return call(*args, _raw_stream(index))
 
 
-def _no_graph(what):
-    raise RuntimeError("ops.%s has first derivatives only: its backward pass cannot run with create_graph=True" % what)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _rows(t, width):
-    """`t` [rows][width] with its entries side by side, and the elements between rows."""
-    if t.is_contiguous():
-        return t, width
-    if (width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width):
-        return t.contiguous(), width
-    return t, t.stride(0) if t.shape[0] > 1 else width
-
-
 # ---- linear ---------------------------------------------------------------------
-
-def _linear_forward(x, w, b, r, act, keep):
-    """(y, z) of x [M, K]: z is the pre-activation for the backward pass where `keep` asks for it."""
-    M, K = x.shape
-    N = w.shape[0]
-    y = _empty((M, N), dtype=x.dtype, device=x.device)
-    z = _empty_like(y) if keep else None
-    if not (M and N):
-        return y, z
-    lib, t = _lib.load(), TYPES[x.dtype]
-    x, ldx = _rows(x, K)
-    w, ldw = _rows(w, K)
-    ldr = N
-    if r is not None:
-        r, ldr = _rows(r, N)
-    px, pw = x.data_ptr(), w.data_ptr()
-    n = lib.cit_linear_forward_work_bytes(M, N, K, t)
-    work = _empty(n, dtype=torch.uint8, device=x.device) if n else None
-    rc = _on(x.get_device(), lib.cit_linear_forward, px, ldx, pw, ldw, _ptr(b), _ptr(r), ldr, y.data_ptr(), _ptr(z), M,
-             N, K, t, act, _ptr(work), n)
-    if rc:
-        _lib.check(rc, "cit_linear_forward")
-    return y, z
-
-
-def _linear_backward(ctx, dy):
-    x, w, z = ctx.saved_tensors
-    nx, nw, nb, nr = ctx.needs_input_grad[:4]
-    shape, M, N, K, act = ctx.dims
-    dx = dw = db = None
-    if nx or nw or nb:
-        make = _empty if M and N else torch.zeros
-        kind = dict(dtype=dy.dtype, device=dy.device)
-        dx = make((M, K), **kind) if nx else None
-        dw = make((N, K), **kind) if nw else None
-        db = make(N, **kind) if nb else None
-        if M and N:
-            lib, t = _lib.load(), TYPES[dy.dtype]
-            d2, ldy = _rows(dy if dy.dim() == 2 else dy.reshape(M, N), N)
-            ldx = ldw = K
-            if nw:
-                x, ldx = _rows(x if x.dim() == 2 else x.reshape(M, K), K)
-            if nx:
-                w, ldw = _rows(w, K)
-            if z is not None and not z.is_contiguous():
-                z = z.contiguous()
-            px, pw = x.data_ptr() if nw else None, w.data_ptr() if nx else None
-            pdx, pdw, pdb = _ptr(dx), _ptr(dw), _ptr(db)
-            n = lib.cit_linear_backward_work_bytes(px, ldx, pw, ldw, pdx, pdw, pdb, M, N, K, t, act)
-            work = _empty(n, dtype=torch.uint8, device=dy.device) if n else None
-            rc = _on(dy.get_device(), lib.cit_linear_backward, d2.data_ptr(), ldy, _ptr(z), px, ldx, pw, ldw, pdx, pdw,
-                     pdb, M, N, K, t, act, _ptr(work), n)
-            if rc:
-                _lib.check(rc, "cit_linear_backward")
-        if nx and len(shape) != 2:
-            dx = dx.reshape(shape)
-    return dx, dw, db, dy if nr else None, None
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, b, r, act):
-        # relu without a residual leaves its sign in y (fp16 aside, where a small y rounds to 0); other activations
-        # need the pre-activation
-        own_y = act == 1 and r is None and x.dtype != torch.float16
-        shape = x.shape
-        N, K = w.shape
-        x2 = x
-        if len(shape) != 2:
-            M = math.prod(shape[:-1])
-            x2 = x.reshape(M, K)
-            r = None if r is None else r.reshape(M, N)
-        y, z = _linear_forward(x2, w, b, r, act, act != 0 and not own_y)
-        out = y if x2 is x else y.reshape(shape[:-1] + (N,))
-        nx, nw = ctx.needs_input_grad[:2]
-        ctx.dims = (shape, x2.shape[0], N, K, act)
-        ctx.save_for_backward(x if nw else None, w if nx else None, out if own_y else z)
-        return out
-
-    @staticmethod
-    def backward(ctx, dy):
-        if _grad_on():
-            _no_graph("linear")
-        return _linear_backward(ctx, dy)
-
 
 def linear(x, weight, bias=None, residual=None, activation="none"):
     """activation(x @ weight.T + bias) + residual, rounded once to x's type.
@@ -200,111 +99,12 @@ def linear(x, weight, bias=None, residual=None, activation="none"):
     M = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
     if max(M, shape[-1], ws[0]) > _MOST:
         raise ValueError("a dimension is over %d" % _MOST)
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
-    if _grad_on() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                       or (residual is not None and residual.requires_grad)):
-        return _Linear.apply(x, weight, bias, residual, act)
-    if len(shape) == 2:
-        return _linear_forward(x, weight, bias, residual, act, False)[0]
-    y = _linear_forward(x.reshape(M, ws[1]), weight, bias, None if residual is None else residual.reshape(M, ws[0]),
-                        act, False)[0]
-    return y.reshape(shape[:-1] + ws[:1])
+    return _calls().linear(x, weight, bias, residual, act)
 
 
 # ---- policy loss ------------------------------------------------------------------
 
 PolicyLoss = collections.namedtuple("PolicyLoss", "loss logp kl")
-
-
-def _policy_args(logits, ref, mask, offsets, actions, old, adv, weights, low, high, beta):
-    """(tensors to keep, the entry points' common arguments)."""
-    if offsets is None:
-        width = logits.shape[1]
-        logits, ld = _rows(logits, width)
-        ref, ld_ref = (None, width) if ref is None else _rows(ref, width)
-        mask, ld_mask = (None, width) if mask is None else _rows(mask, width)
-        total = 0
-    else:
-        width = ld = ld_ref = ld_mask = 0
-        total = logits.shape[0]
-        logits, ref, mask = (None if t is None else t.contiguous() for t in (logits, ref, mask))
-    return (logits, ref, mask), (logits.data_ptr(), ld, _ptr(ref), ld_ref, _ptr(mask), ld_mask, _ptr(offsets), total,
-                                 actions.shape[0], width, actions.data_ptr(), old.data_ptr(), adv.data_ptr(),
-                                 _ptr(weights), low, high, beta, TYPES[logits.dtype])
-
-
-def _policy_forward(given, want_grad):
-    """(loss, logp, kl, gradient for an upstream gradient of 1)."""
-    logits, rows = given[0], given[4].shape[0]
-    lib, dev = _lib.load(), logits.device
-    loss = _empty((), dtype=torch.float32, device=dev)
-    logp = _empty(rows, dtype=torch.float32, device=dev)
-    kl = _empty(rows, dtype=torch.float32, device=dev)
-    grad = None
-    if want_grad:
-        grad = _empty(logits.shape, dtype=logits.dtype, device=dev)
-        if not rows:
-            grad.zero_()
-    keep, args = _policy_args(*given)
-    n = lib.cit_policy_loss_work_bytes(rows, args[9], args[6] is not None)
-    work = _empty(n, dtype=torch.uint8, device=dev) if n else None
-    rc = _on(logits.get_device(), lib.cit_policy_loss, *args, loss.data_ptr(), logp.data_ptr(), kl.data_ptr(),
-             _ptr(grad), _ptr(work), n)
-    if rc:
-        _lib.check(rc, "cit_policy_loss")
-    return loss, logp, kl, grad
-
-
-def _policy_backward(ctx, up):
-    given = ctx.saved_tensors + ctx.scalars
-    logits = given[0]
-    try:
-        grad, captured = ctx.held.pop()
-    except IndexError:                           # a second backward pass: the first one's gradient is its owner's
-        grad = None
-    # a graph replayed on its own may find the forward pass's gradient used up
-    ready = grad is not None and (captured or not torch.cuda.is_current_stream_capturing())
-    if grad is None:
-        grad = _empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    if not given[4].shape[0]:
-        return (grad.zero_(),) + (None,) * 10
-    if up.dtype != torch.float32:
-        up = up.float()
-    lib = _lib.load()
-    keep, args = _policy_args(*given)
-    n = lib.cit_policy_loss_work_bytes(args[8], args[9], args[6] is not None)
-    work = _empty(n, dtype=torch.uint8, device=logits.device) if n else None
-    rc = _on(logits.get_device(), lib.cit_policy_loss_backward, *args, up.data_ptr(), 1 if ready else 0,
-             grad.data_ptr(), _ptr(work), n)
-    if rc:
-        _lib.check(rc, "cit_policy_loss_backward")
-    return (grad,) + (None,) * 10
-
-
-class _PolicyLoss(torch.autograd.Function):
-    """The forward kernel has a row's probabilities in hand, so it writes the
-    gradient for an upstream gradient of 1 in the same pass over the logits;
-    the backward kernel reads the upstream gradient on the device and computes
-    the gradient again only where it is something else."""
-
-    @staticmethod
-    def forward(ctx, *given):
-        loss, logp, kl, grad = _policy_forward(given, True)
-        ctx.mark_non_differentiable(logp, kl)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*given[:8])
-        ctx.scalars = given[8:]
-        ctx.held = [(grad, torch.cuda.is_current_stream_capturing())]
-        return loss, logp, kl
-
-    @staticmethod
-    def backward(ctx, up, _logp, _kl):
-        if up is None:
-            return (None,) * 11
-        if _grad_on():
-            _no_graph("policy_loss")
-        return _policy_backward(ctx, up)
 
 
 def _f32(name, t, N):
@@ -380,12 +180,8 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logits=None, offse
     if mask is not None and (mask.shape != shape or mask.dtype != torch.bool):
         raise ValueError("mask must be bool and as logits %s" % (tuple(shape),))
     _gpu(logits)
-    if ref_logits is not None and ref_logits.requires_grad:
-        ref_logits = ref_logits.detach()
-    given = (logits, ref_logits, mask, offsets, _whole(actions), old_logp, advantages, weights, low, high, kl_coef)
-    if logits.requires_grad and _grad_on():
-        return PolicyLoss(*_PolicyLoss.apply(*given))
-    return PolicyLoss(*_policy_forward(given, False)[:3])
+    return PolicyLoss(*_calls().policy_loss(logits, ref_logits, mask, offsets, _whole(actions), old_logp, advantages,
+                                            weights, low, high, kl_coef))
 
 
 # ---- gradient norm ------------------------------------------------------------------
