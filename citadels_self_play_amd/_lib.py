@@ -122,7 +122,8 @@ def load():
 
 
 _TORCH_CALLS = ("cit_linear_forward_work_bytes", "cit_linear_forward", "cit_linear_backward_work_bytes",
-                "cit_linear_backward", "cit_policy_loss_work_bytes", "cit_policy_loss", "cit_policy_loss_backward")
+                "cit_linear_backward", "cit_policy_loss_work_bytes", "cit_policy_loss", "cit_policy_loss_backward",
+                "cit_clip_grad_norm_work_bytes", "cit_clip_grad_norm")
 
 
 def torch_calls():

@@ -1,7 +1,8 @@
 // The training operators' path from torch to the C ABI (include/citadels.h):
 // outputs and workspaces from torch's allocator, the current stream, and the
-// autograd nodes.  ops.py checks the arguments; what it hands over is of the
-// shapes, types and devices that it says.
+// autograd nodes.  ops.py checks the arguments of the linear layer and the
+// policy loss; what it hands over is of the shapes, types and devices that it
+// says.  Lists of gradients, which may be long, are checked here.
 //
 // The nodes are C++ because a backward pass runs on torch's own thread for the
 // device: a Python one has to be woken there with the interpreter's lock, in
@@ -40,6 +41,8 @@ struct Api {
   decltype(&cit_policy_loss_work_bytes) policy_loss_work_bytes;
   decltype(&cit_policy_loss) policy_loss;
   decltype(&cit_policy_loss_backward) policy_loss_backward;
+  decltype(&cit_clip_grad_norm_work_bytes) clip_grad_norm_work_bytes;
+  decltype(&cit_clip_grad_norm) clip_grad_norm;
 } api;
 
 void check(int rc, const char* what) {
@@ -319,6 +322,126 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Maybe
   return {loss, logp, kl};
 }
 
+// ---- gradient norm ------------------------------------------------------------------
+
+// The tensors of a Python list: dense ones of the kernels' types on one device.
+std::vector<Tensor> listed(const py::list& from, const std::string& what) {
+  std::vector<Tensor> out;
+  out.reserve(from.size());
+  for (const py::handle& h : from) {
+    if (!THPVariable_Check(h.ptr())) throw py::value_error(what + " must be a tensor");
+    out.push_back(THPVariable_Unpack(h.ptr()));
+  }
+  for (const Tensor& t : out) {
+    if (t.layout() != at::kStrided) throw py::value_error(what + " must be a dense tensor");
+    const at::ScalarType dt = t.scalar_type();
+    if (dt != at::kFloat && dt != at::kBFloat16 && dt != at::kHalf)
+      throw py::value_error(what + "s must be fp32, bf16 or fp16, not " +
+                            py::str(py::reinterpret_borrow<py::object>(from[&t - out.data()]).attr("dtype")).cast<std::string>());
+    if (t.device() != out[0].device()) throw py::value_error(what + "s must be on one device");
+  }
+  return out;
+}
+
+typedef std::vector<std::pair<uintptr_t, uintptr_t>> Spans;
+
+// Start and end of the tensors that hold something.
+Spans spans_of(const std::vector<Tensor>& list) {
+  Spans s;
+  s.reserve(list.size());
+  for (const Tensor& t : list)
+    if (t.numel()) s.emplace_back((uintptr_t)t.const_data_ptr(), (uintptr_t)t.const_data_ptr() + t.nbytes());
+  return s;
+}
+bool disjoint(Spans s) {
+  std::sort(s.begin(), s.end());
+  for (size_t i = 1; i < s.size(); i++)
+    if (s[i].first < s[i - 1].second) return false;
+  return true;
+}
+
+enum { NORM = 0, CHECK = 1, CLIP = 2 };  // the norm alone; the same after clip's checks; clip
+
+// The norm of `grads` (not empty), and their clipping into `out` (None: in place).
+Tensor clip_grad_norm(const py::list& given, double max_norm, const py::object& into, int mode) {
+  const std::vector<Tensor> grads = listed(given, "a gradient");
+  std::vector<Tensor> flat, outs;
+  flat.reserve(grads.size());
+  {
+    at::NoGradGuard none;
+    for (const Tensor& t : grads) flat.push_back(t.is_contiguous() ? t : t.contiguous());
+  }
+  const Spans spans = spans_of(flat);
+  if (mode != NORM && into.is_none()) {
+    std::vector<uintptr_t> at;
+    for (size_t i = 0; i < grads.size(); i++) {
+      const Tensor& t = grads[i];
+      if (!t.is_same(flat[i]))
+        for (int64_t d = 0; d < t.dim(); d++)
+          if (t.stride(d) == 0 && t.size(d) > 1)
+            throw py::value_error("a gradient whose elements share memory cannot be clipped in place: give out=");
+      if (t.numel()) at.push_back((uintptr_t)t.const_data_ptr());
+    }
+    std::sort(at.begin(), at.end());
+    if (!disjoint(spans) || std::adjacent_find(at.begin(), at.end()) != at.end())
+      throw py::value_error("a gradient is listed twice, or two share memory");
+    outs = flat;
+  } else if (mode != NORM) {
+    outs = listed(py::list(into), "an out tensor");
+    if (outs.size() != grads.size())
+      throw py::value_error(std::to_string(grads.size()) + " gradients, " + std::to_string(outs.size()) +
+                            " tensors in out");
+    for (size_t i = 0; i < outs.size(); i++)
+      if (!outs[i].is_contiguous() || outs[i].sizes() != grads[i].sizes() ||
+          (outs[i].scalar_type() != grads[i].scalar_type() && outs[i].scalar_type() != at::kFloat))
+        throw py::value_error("an out tensor must be contiguous, of its gradient's shape, and of its type or fp32");
+    if (outs[0].device() != grads[0].device()) throw py::value_error("out tensors must be on the gradients' device");
+    const Spans to = spans_of(outs);
+    Spans both = to;
+    both.insert(both.end(), spans.begin(), spans.end());
+    if (!disjoint(both)) {
+      // gradients may share memory among themselves, and one may be its own out tensor
+      bool bad = !disjoint(to);
+      for (size_t i = 0; i < flat.size() && !bad; i++) {
+        if (!flat[i].numel() || (flat[i].const_data_ptr() == outs[i].const_data_ptr() &&
+                                 flat[i].scalar_type() == outs[i].scalar_type()))
+          continue;
+        Spans with = to;
+        with.emplace_back((uintptr_t)flat[i].const_data_ptr(), (uintptr_t)flat[i].const_data_ptr() + flat[i].nbytes());
+        bad = !disjoint(with);
+      }
+      if (bad) throw py::value_error("out tensors share memory with one another or with other gradients");
+    }
+  }
+  if (!flat[0].is_cuda())
+    throw py::value_error("tensors must be on the GPU (there is no CPU path), not on " + flat[0].device().str());
+  const size_t n = flat.size();
+  std::vector<const void*> from(n);
+  std::vector<void*> to(n);
+  std::vector<int64_t> sizes(n);
+  std::vector<int32_t> types(n), out_types(n);
+  for (size_t i = 0; i < n; i++) {
+    from[i] = flat[i].const_data_ptr(), sizes[i] = flat[i].numel(), types[i] = type_of(flat[i]);
+    if (mode == CLIP) to[i] = outs[i].mutable_data_ptr(), out_types[i] = type_of(outs[i]);
+  }
+  py::gil_scoped_release release;
+  at::NoGradGuard none;
+  const On on(flat[0]);
+  const Tensor norm = at::empty({}, flat[0].options().dtype(at::kFloat));
+  const size_t bytes = api.clip_grad_norm_work_bytes((int)n);
+  const Tensor work = workspace(bytes, norm);
+  check(api.clip_grad_norm(from.data(), mode == CLIP ? to.data() : nullptr, sizes.data(), types.data(),
+                           mode == CLIP ? out_types.data() : nullptr, (int)n, max_norm,
+                           static_cast<float*>(writable(norm)), writable(work), bytes, on.stream),
+        "cit_clip_grad_norm");
+  if (mode == CLIP)
+    for (size_t i = 0; i < n; i++) {
+      if (into.is_none() && !grads[i].is_same(flat[i])) grads[i].copy_(flat[i]);
+      else if (!outs[i].is_inference()) torch::autograd::impl::bump_version(outs[i]);
+    }
+  return norm;
+}
+
 PyObject* native_error = nullptr;        // _lib.NativeError
 
 void bind(py::object error, const std::map<std::string, uint64_t>& at) {
@@ -333,6 +456,8 @@ void bind(py::object error, const std::map<std::string, uint64_t>& at) {
   take(api.policy_loss_work_bytes, "cit_policy_loss_work_bytes");
   take(api.policy_loss, "cit_policy_loss");
   take(api.policy_loss_backward, "cit_policy_loss_backward");
+  take(api.clip_grad_norm_work_bytes, "cit_clip_grad_norm_work_bytes");
+  take(api.clip_grad_norm, "cit_clip_grad_norm");
 }
 
 }  // namespace
@@ -348,4 +473,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind);
   m.def("linear", &linear, py::call_guard<py::gil_scoped_release>());
   m.def("policy_loss", &policy_loss, py::call_guard<py::gil_scoped_release>());
+  m.def("clip_grad_norm", &clip_grad_norm);
 }

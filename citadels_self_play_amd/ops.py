@@ -19,7 +19,6 @@ call's time is the host's.  What follows them, autograd included, is
 csrc/cit_torch.cpp.
 """
 import collections
-import ctypes as C
 import math
 
 import torch
@@ -29,9 +28,7 @@ from . import _lib
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 _MOST, _LONGEST = 2 ** 31 - 1024, 2 ** 30       # a matrix's sides; a row's entries (the kernels' indexes are 32 bits)
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current = torch.cuda.current_device
-_empty = torch.empty
+_NORM, _CHECK, _CLIP = 0, 1, 2                  # cit_torch.cpp's clip_grad_norm
 _calls = _lib.torch_calls
 
 
@@ -51,14 +48,6 @@ def _same_place(first, **others):
 def _gpu(t):
     if not t.is_cuda:
         raise ValueError("tensors must be on the GPU (there is no CPU path), not on %s" % t.device)
-
-
-def _on(index, call, *args):
-    """call(*args, stream) with the device's current stream, and the device as the current one."""
-    if index == _current():
-        return call(*args, _raw_stream(index))
-    with torch.cuda.device(index):
-        return call(*args, _raw_stream(index))
 
 
 # ---- linear ---------------------------------------------------------------------
@@ -186,65 +175,14 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logits=None, offse
 
 # ---- gradient norm ------------------------------------------------------------------
 
-def _listed(tensors, what):
-    """(the list, its type codes, whether all are contiguous)."""
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if not all(isinstance(t, torch.Tensor) for t in tensors):
-        raise ValueError("%s must be a tensor" % what)
-    kinds = {(t.dtype, t.get_device(), t.layout) for t in tensors}
-    for dt, device, layout in kinds:
-        if layout != torch.strided:
-            raise ValueError("%s must be a dense tensor" % what)
-        if dt not in TYPES:
-            raise ValueError("%ss must be fp32, bf16 or fp16, not %s" % (what, dt))
-        if device != tensors[0].get_device():
-            raise ValueError("%ss must be on one device" % what)
-    if len(kinds) == 1:
-        codes = [TYPES[tensors[0].dtype]] * len(tensors)
-    else:
-        codes = [TYPES[t.dtype] for t in tensors]
-    return tensors, codes, all(t.is_contiguous() for t in tensors)
-
-
-def _addresses(tensors, codes):
-    """(addresses, element counts, (start, end) of those that are not empty)."""
-    ptrs, sizes = [t.data_ptr() for t in tensors], [t.numel() for t in tensors]
-    return ptrs, sizes, [(p, p + n * (2 if c else 4)) for p, n, c in zip(ptrs, sizes, codes) if n]
-
-
-def _disjoint(spans):
-    end = 0
-    for a, b in sorted(spans):
-        if a < end:
-            return False
-        end = b
-    return True
-
-
-def _norm(like, codes, ptrs, sizes, max_norm=math.inf, to=None, to_codes=None):
-    """cit_clip_grad_norm over contiguous tensors at `ptrs`, into those at `to` (None: the norm alone)."""
-    _gpu(like)
-    lib, n = _lib.load(), len(ptrs)
-    norm = _empty((), dtype=torch.float32, device=like.device)
-    pointers, types = C.c_void_p * n, C.c_int32 * n
-    grads, kinds = pointers(*ptrs), types(*codes)
-    outs, out_kinds = (None, None) if to is None else (grads, kinds) if to is ptrs else (pointers(*to), types(*to_codes))
-    size = lib.cit_clip_grad_norm_work_bytes(n)
-    work = _empty(size, dtype=torch.uint8, device=like.device)
-    rc = _on(like.get_device(), lib.cit_clip_grad_norm, grads, outs, (C.c_int64 * n)(*sizes), kinds, out_kinds, n,
-             max_norm, norm.data_ptr(), work.data_ptr(), size)
-    if rc:
-        _lib.check(rc, "cit_clip_grad_norm")
-    return norm
+def _listed(tensors):
+    return [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
 
 
 def grad_norm(grads):
     """sqrt of the sum of all squares of a list of gradients (fp32 scalar on the device; no tensors: 0)."""
-    grads, codes, contiguous = _listed(grads, "a gradient")
-    if not grads:
-        return torch.zeros(())
-    flat = grads if contiguous else [t.detach().contiguous() for t in grads]
-    return _norm(flat[0], codes, *_addresses(flat, codes)[:2])
+    grads = _listed(grads)
+    return _calls().clip_grad_norm(grads, math.inf, None, _NORM) if grads else torch.zeros(())
 
 
 def clip_grad_norm(grads, max_norm, out=None, error_if_nonfinite=False):
@@ -259,41 +197,12 @@ def clip_grad_norm(grads, max_norm, out=None, error_if_nonfinite=False):
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("max_norm must be a number >= 0, not %r" % max_norm)
-    grads, codes, contiguous = _listed(grads, "a gradient")
-    flat = grads if contiguous else [t.detach().contiguous() for t in grads]
-    ptrs, sizes, spans = _addresses(flat, codes)
-    if out is None:
-        outs, to, to_codes = flat, ptrs, codes
-        if not contiguous and any(s == 0 and n > 1 for t in grads for n, s in zip(t.shape, t.stride())):
-            raise ValueError("a gradient whose elements share memory cannot be clipped in place: give out=")
-        at = [t.data_ptr() for t in grads if t.numel()]
-        if not _disjoint(spans) or len(set(at)) != len(at):
-            raise ValueError("a gradient is listed twice, or two share memory")
-    else:
-        outs, to_codes, contiguous_out = _listed(out, "an out tensor")
-        if len(outs) != len(grads):
-            raise ValueError("%d gradients, %d tensors in out" % (len(grads), len(outs)))
-        if not contiguous_out or any(o.shape != g.shape for g, o in zip(grads, outs)) or \
-                any(d != c and d for c, d in zip(codes, to_codes)):
-            raise ValueError("an out tensor must be contiguous, of its gradient's shape, and of its type or fp32")
-        if outs and outs[0].get_device() != grads[0].get_device():
-            raise ValueError("out tensors must be on the gradients' device")
-        to, _, out_spans = _addresses(outs, to_codes)
-        if not _disjoint(out_spans + spans):
-            # gradients may share memory among themselves, and one may be its own out tensor
-            alone = [(f, c) for f, p, o, c, d in zip(flat, ptrs, to, codes, to_codes) if p != o or c != d]
-            alone = _addresses([f for f, _ in alone], [c for _, c in alone])[2]
-            if not _disjoint(out_spans) or any(not _disjoint(out_spans + [s]) for s in alone):
-                raise ValueError("out tensors share memory with one another or with other gradients")
+    grads, out = _listed(grads), None if out is None else _listed(out)
     if not grads:
+        if out:
+            raise ValueError("0 gradients, %d tensors in out" % len(out))
         return torch.zeros(())
-    if error_if_nonfinite and not math.isfinite(float(_norm(flat[0], codes, ptrs, sizes))):
+    call = _calls().clip_grad_norm
+    if error_if_nonfinite and not math.isfinite(float(call(grads, max_norm, out, _CHECK))):
         raise RuntimeError("the gradients' global norm is not finite: nothing was clipped")
-    norm = _norm(flat[0], codes, ptrs, sizes, max_norm, to, to_codes)
-    torch.autograd.graph.increment_version(outs)
-    if flat is not grads and out is None:
-        with torch.no_grad():
-            for t, c in zip(grads, flat):
-                if c.data_ptr() != t.data_ptr():
-                    t.copy_(c)
-    return norm
+    return call(grads, max_norm, out, _CLIP)

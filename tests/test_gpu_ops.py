@@ -7,9 +7,11 @@ n terms in fp32, in any order, is off by at most (n + 2) u sum |terms|; a
 device exp, log or erfc by 4 u of its value (2 ulp); every rounding to the
 element type by e of the value or half of tiny."""
 import math
+import threading
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from citadels_self_play_amd import ops
 
@@ -833,6 +835,89 @@ def test_more_workgroups_than_one_dimension_takes():
         want = want[:, None] * sign
         assert bool(((grad[rows].double() - want).abs() <= want.abs() * (2.0 ** -11 + 300 * U) + 2.0 ** -25).all())
     assert abs(float(got.loss.detach()) + total * 2.0 ** -10) <= 150 * U * total * 2.0 ** -10
+
+
+def test_autograd_manners():
+    """What torch's own nodes keep to: a graph used twice, saved tensors written over, hooks that move them to the host,
+    undefined gradients, backward passes on two threads at once, no forward mode."""
+    x, w, b, r, dy = linear_inputs(37, 50, 41, torch.float32, "silu", True, True)
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    want = torch.autograd.grad(ops.linear(*leaves, activation="silu"), leaves, dy)
+    a = policy_rows([4, 9, 30], torch.float32)
+    l = a["logits"].requires_grad_()
+    want_l = torch.autograd.grad(call_policy(a, (0.2, 0.2), 0.1, l).loss, l)[0]
+    # once without retain_graph
+    for make, of, up in ((lambda: ops.linear(*leaves, activation="silu"), leaves, dy),
+                         (lambda: call_policy(a, (0.2, 0.2), 0.1, l).loss, [l], None)):
+        y = make()
+        torch.autograd.grad(y, of, up)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y, of, up)
+    # what a node saved, written over: y itself for relu, x and w, the logits
+    y = ops.linear(x, w, b, activation="relu")
+    y.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, w, dy)
+    for at in (0, 1):
+        given = [t.detach().clone().requires_grad_() for t in (x, w)]
+        y = ops.linear(*given)
+        with torch.no_grad():
+            given[at].add_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, given[1 - at], dy)
+    m = l.detach().clone().requires_grad_()
+    loss = call_policy(a, (0.2, 0.2), 0.1, m).loss
+    with torch.no_grad():
+        m.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, m)
+    # saved on the host meanwhile
+    with torch.autograd.graph.save_on_cpu():
+        y, loss = ops.linear(*leaves, activation="silu"), call_policy(a, (0.2, 0.2), 0.1, l).loss
+    assert all(torch.equal(g, v) for g, v in zip(torch.autograd.grad(y, leaves, dy), want))
+    assert torch.equal(torch.autograd.grad(loss, l)[0], want_l)
+    # a checkpointed segment works its forward pass out again
+    y = torch.utils.checkpoint.checkpoint(lambda *t: ops.linear(*t, activation="silu"), *leaves, use_reentrant=False)
+    assert all(torch.equal(g, v) for g, v in zip(torch.autograd.grad(y, leaves, dy), want))
+    # the statistics have no gradient; one of several outputs unused
+    got = call_policy(a, (0.2, 0.2), 0.1, l)
+    assert got.loss.requires_grad and not got.logp.requires_grad and not got.kl.requires_grad
+    assert torch.equal(torch.autograd.grad(got.loss + ops.linear(x, w).sum() * 0.0, l)[0], want_l)
+    # one graph, two threads
+    y, loss = ops.linear(*leaves, activation="silu"), call_policy(a, (0.2, 0.2), 0.1, l).loss
+    out = [None] * 8
+
+    def back(i):
+        out[i] = torch.autograd.grad(y, leaves, dy, retain_graph=True) + torch.autograd.grad(loss, l, retain_graph=True)
+
+    threads = [threading.Thread(target=back, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    torch.cuda.synchronize()
+    assert all(g is not None and all(torch.equal(p, q) for p, q in zip(g, want + (want_l,))) for g in out)
+    # leaves accumulate
+    for t in leaves:
+        t.grad = None
+    for _ in range(2):
+        ops.linear(*leaves, activation="silu").backward(dy)
+    assert all(torch.equal(t.grad, 2 * v) for t, v in zip(leaves, want))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="no forward-mode"):
+            ops.linear(dual, w)
+    with torch.inference_mode():
+        y = ops.linear(*leaves, activation="silu")
+        assert y.is_inference() and not y.requires_grad
+        t = torch.ones(30, device="cuda")
+        assert abs(float(ops.clip_grad_norm([t], 1.0)) - math.sqrt(30.0)) <= 4 * U * 6 and float(t[0]) < 1.0
+    # a clipped gradient's version goes up, and a graph that saved it notices
+    t = torch.ones(30, device="cuda")
+    y = (torch.ones(30, device="cuda", requires_grad=True) * t).sum()
+    ops.clip_grad_norm([t], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
 
 
 # ---- together ---------------------------------------------------------------------------
