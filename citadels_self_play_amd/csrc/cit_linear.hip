@@ -783,6 +783,7 @@ __global__ __launch_bounds__(256) void k_join(Epilogue e, int64_t M, int N, int 
   const int64_t count = M * N;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
     float v = 0.0f;
+#pragma unroll 8
     for (int s = 0; s < splits; s++) v += e.part[s * count + i];
     const int64_t m = i / N;
     finish<T>(e, m, (int)(i - m * N), N, v);
@@ -867,7 +868,7 @@ __global__ __launch_bounds__(256) void k_db(const float* part, T* db, int N, int
 // Rows that do not start on 16 bytes cost the tile kernel guarded loads through
 // registers.  The backward products, which read them down the rows, are
 // faster over copies with padded rows (bf16 3000 x 1001 x 999: dw 95 -> 42 us);
-// the forward product is not (22 us, 29 with copies).
+// the forward product only where it is large.
 
 struct Copies {
   Mat from[2];
@@ -909,26 +910,52 @@ enum { TILE_32, TILE_64, TILE_128, TILE_256 };
 // (that one has 256 tiles); fp32 1 x 4096 x 16384 68 / 262 us, 512 x 1024 x 1024 17 / 21, 2048 x 512 x 512 19 / 14.
 bool small(int M, int N) { return M <= 32 || N <= 32 || (int64_t)cdiv(M, 64) * cdiv(N, 64) < 256; }
 
-// The tile of a product whose operands take direct loads: the largest of which there are enough (a tile's loads
-// are what the L2s deliver, about 10 TB/s, and fall with its side).  Measured, 64 / 128 / 256, us:
-// bf16 M x N x K 8192 x 4096 x 4096 380 / 264 / 232; 4096 x 4096 x 2048 (256 of 256) 104 / 70 / 60;
-// 4096 x 2048 x 4096 (128 of 256, 512 of 128) 92 / 62 / 92; 2048^3 (256 of 128) 29 / 24;
-// 3000 x 999 x 1001 (192 of 128) 29 / 33; fp32 2048^3 137 / 134, 3000 x 999 x 1001 71 / 92.
-int direct_tile(int M, int N, int es) {
-  if (es == 2 && (int64_t)cdiv(M, 256) * cdiv(N, 256) >= 192) return TILE_256;
-  if ((int64_t)cdiv(M, 128) * cdiv(N, 128) >= 208) return TILE_128;
-  return TILE_64;
+// The tile of a product whose operands take direct loads.  Larger tiles load less (what the L2s deliver, about
+// 10 TB/s, bounds 64 x 64 ones of 16-bit types) but fill the last round of the 256 compute units less.  Measured,
+// us at K = 1024, by tiles of 128 in steps s of 256, r = steps of 256 tiles of 256:
+//   bf16   s   1   2   3   4   5   6   7   8   9  10  12      128: 19 ceil(s / 2), 4 less where s is odd
+//         128 13  21  34  40  53  59  71  77  88  96 114
+//         256 30  30  31  34  58  60  61  67  93  94  98      r = 1, 1, 1, 1, 2, 2, 2, 2, 3, 3, 3: 30.5 r + 1
+//          64 14  28  38  53  66  78  90 105 117 128 152
+//   fp32  the matrix cores: 64 x 64 tiles 18.3 a round of 256, 128 x 128 ones 65: by the rounds alone
+// Under K = 512 what a tile starts and ends with counts more: 64 longer (bf16 K = 256, s = 2: 10.5 / 11.0 / 15.0).
+int direct_tile(int M, int N, int K, int es) {
+  const auto steps = [&](int t) { return ((int64_t)cdiv(M, t) * cdiv(N, t) + 255) / 256; };
+  const int64_t s = steps(128);
+  if (es == 4) return K >= 512 && 36 * s < 10 * steps(64) ? TILE_128 : TILE_64;
+  if (K < 512 && s <= 3) return TILE_64;
+  if (61 * steps(256) + 2 < 38 * ((s + 1) / 2) - (s & 1 ? 8 : 0)) return TILE_256;
+  return s > 1 || (int64_t)cdiv(M, 128) * cdiv(N, 128) >= 208 ? TILE_128 : TILE_64;
 }
 
-Plan plan(int M, int N, int K, int es, bool aligned) {
+// Splits of a long reduction for few outputs, and the tile they take; 1: not of that kind.  For operands that take
+// direct loads (ks: one is read down its rows).  Split so / as before, us: bf16 dw of 65,536 rows x 256 x 512 51 / 111,
+// 32,768 x 768 x 768 72 / 261, 9000 x 1024 x 512 29 / 58, 4096 x 512 x 416 15 / 18, forward 256 x 4096 x 16,384 51 / 109,
+// 256 x 4096 x 4096 25 / 33 (but 512 x 1024 x 4096 19 / 16, dw 4096 x 256 x 128 11 / 9); fp32 dw 32,768 x 768 x 768
+// 314 / 557, forward 256 x 4096 x 16,384 281 / 445 (but dw 65,536 x 128 x 128 52 / 41).
+int long_splits(int M, int N, int K, int es, bool ks, int& tile) {
+  const int64_t c64 = (int64_t)cdiv(M, 64) * cdiv(N, 64), c128 = (int64_t)cdiv(M, 128) * cdiv(N, 128);
+  const int from = c128 > 64 || (es == 2 && !ks && c64 <= 128) ? 8192 : 4096;
+  if (K < from || M < 64 || N < 64 || c128 > 128 || c64 < (K < 32768 ? 16 : 8)) return 1;
+  tile = c64 > 96 ? TILE_128 : TILE_64;
+  // a workgroup a compute unit of large tiles, two of small ones; each split long enough to pay for its sums
+  int64_t want = tile == TILE_128 ? 256 / c128 : 512 / c64;
+  const int most = K / (es == 2 ? 1024 : 512);
+  if (want > most) want = most;
+  return (int)(want > 32 ? 32 : want);
+}
+
+Plan plan(int M, int N, int K, int es, bool aligned, bool ks) {
   Plan p;
-  p.tile = small(M, N) ? TILE_32 : aligned ? direct_tile(M, N, es) : TILE_64;
+  p.tile = small(M, N) ? TILE_32 : aligned ? direct_tile(M, N, K, es) : TILE_64;
+  int split = 1;
+  if (aligned) split = long_splits(M, N, K, es, ks, p.tile);
   const int t = 32 << p.tile, bk = 128 / es, kt = cdiv(K, bk);
   p.tiles_m = cdiv(M, t);
   p.tiles_n = cdiv(N, t);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  p.deep = p.tile == TILE_128 && tiles <= 256;   // one workgroup on a compute unit: 2048^3 bf16 31 -> 25 us
-  int want = 1;
+  p.deep = p.tile == TILE_128 && tiles * split <= 256;   // one workgroup on a compute unit: 2048^3 bf16 31 -> 25 us
+  int want = split;
   // A few small tiles over a long reduction: the launch shares it out too, at least 4 k tiles for each wave (fp32
   // 4096 x 418 x 512: dw 39 -> 34 us).
   if (p.tile == TILE_32 && tiles < 256) {
@@ -940,10 +967,10 @@ Plan plan(int M, int N, int K, int es, bool aligned) {
   p.splits = K > 0 ? cdiv(K, p.k_per) : 1;
   return p;
 }
-int64_t split_bytes(int M, int N, int K, int es) {
-  if (!small(M, N)) return 0;
-  const Plan p = plan(M, N, K, es, false);
-  return p.splits > 1 ? align256((int64_t)p.splits * M * N * 4) : 0;
+// Of either kind of operands: what the matrices' addresses allow is not known here.
+int64_t split_bytes(int M, int N, int K, int es, bool ks) {
+  const int a = plan(M, N, K, es, false, ks).splits, b = plan(M, N, K, es, true, ks).splits;
+  return a > 1 || b > 1 ? align256((int64_t)(a > b ? a : b) * M * N * 4) : 0;
 }
 
 bool aligned(const void* p, int64_t ld, int es) {
@@ -954,8 +981,22 @@ bool direct(const Mat& a, bool ks, int es) { return aligned(a.p, a.ld, es) && (!
 
 int64_t padded(int cols, int es) { return ((int64_t)cols * es + 15) / 16 * 16 / es; }
 
-// Whether the backward pass copies unaligned operands of an M x N x K product first.
-bool worth_copies(int M, int N, int K) { return !small(M, N) && K >= 256; }
+// Whether the backward pass copies unaligned operands of an M x N x K product first: of many outputs, or of few over a
+// reduction long enough to be split (dw of 65,536 rows x 512 x 418, us with / without: bf16 100 / 413, fp32 322 / 560;
+// 8192 rows 35 / 35).
+bool worth_copies(int M, int N, int K, int es) {
+  int tile;
+  return !small(M, N) ? K >= 256 : K >= 16384 && long_splits(M, N, K, es, true, tile) > 1;
+}
+
+// Whether a forward product whose rows cannot start on 16 bytes copies its operands first: of enough work, and of
+// enough work for each copied element.  With copies / without, us: fp16 4001 x 4003 x 2001 84 / 205, 65,536 x 200 x
+// 418 47 / 59, 3000 x 1001 x 999 27 / 24, 4096 x 512 x 418 13 / 10; fp32 4001 x 4003 x 2001 535 / 622, 65,536 x 200 x
+// 418 171 / 150, 3000 x 1001 x 999 67 / 66.
+bool forward_copies(int M, int N, int K, int es) {
+  return padded(K, es) != K && !small(M, N) && (double)M * N * K >= 4e9 &&
+         (int64_t)M * N / ((int64_t)M + N) >= (es == 4 ? 512 : 192);
+}
 
 template <typename T, bool AKS, bool BKS, int TILE, int WM, int WN, int STAGES, bool AHEAD>
 void launch_direct(const Mat& A, const Mat& B, const Epilogue& e, int M, int N, int K, const Plan& p,
@@ -967,7 +1008,7 @@ void launch_direct(const Mat& A, const Mat& B, const Epilogue& e, int M, int N, 
 template <typename T, bool AKS, bool BKS>
 int product(Mat A, Mat B, Epilogue e, int M, int N, int K, void* work, hipStream_t stream) {
   const bool d = K > 0 && direct(A, AKS, sizeof(T)) && direct(B, BKS, sizeof(T));
-  const Plan p = plan(M, N, K, sizeof(T), d);
+  const Plan p = plan(M, N, K, sizeof(T), d, AKS || BKS);
   const dim3 tiles = wide_grid((int64_t)p.tiles_m * p.tiles_n), grid(tiles.x, p.splits, tiles.y);
   if (p.splits > 1) e.part = static_cast<float*>(work);
   if (p.tile == TILE_32)
@@ -1020,7 +1061,7 @@ Layout backward_layout(const void* x, int64_t ldx, const void* w, int64_t ldw, b
   if (K <= 0) dx = dw = false;
   // dz in rows of its own; where there is no activation dy stands for it, unless its rows are off 16 bytes, which
   // the size alone decides here
-  const bool big_x = dx && worth_copies(M, K, N), big_w = dw && worth_copies(N, K, M);
+  const bool big_x = dx && worth_copies(M, K, N, es), big_w = dw && worth_copies(N, K, M, es);
   const bool odd = padded(N, es) != N;
   if ((dx || dw) && (act != ACT_NONE || (odd && (big_x || big_w)))) l.dz = align256(M * padded(N, es) * es);
   // the products' other operands are read down their rows: their width has to be whole chunks too
@@ -1028,7 +1069,7 @@ Layout backward_layout(const void* x, int64_t ldx, const void* w, int64_t ldw, b
   if (big_w && (!aligned(x, ldx, es) || odd_k)) l.copy[0] = align256(M * padded(K, es) * es);
   if (big_x && (!aligned(w, ldw, es) || odd_k)) l.copy[1] = align256(N * padded(K, es) * es);
   if (db && cdiv(M, dz_rows(M, N)) > 1) l.sums = align256((int64_t)cdiv(M, dz_rows(M, N)) * N * 4);
-  const int64_t a = dx ? split_bytes(M, K, N, es) : 0, b = dw ? split_bytes(N, K, M, es) : 0;
+  const int64_t a = dx ? split_bytes(M, K, N, es, true) : 0, b = dw ? split_bytes(N, K, M, es, true) : 0;
   l.split = a > b ? a : b;
   return l;
 }
@@ -1094,6 +1135,27 @@ int backward(Mat dy, const void* z, Mat x, Mat w, void* dx, void* dw, void* db, 
   return rc ? rc : launch_status();
 }
 
+// Copies of both operands of a forward product, where their rows cannot start on 16 bytes.
+Layout forward_layout(int M, int N, int K, int es) {
+  Layout l = {};
+  if (forward_copies(M, N, K, es)) {
+    l.copy[0] = align256((int64_t)M * padded(K, es) * es);
+    l.copy[1] = align256((int64_t)N * padded(K, es) * es);
+  } else {
+    l.split = split_bytes(M, N, K, es, false);
+  }
+  return l;
+}
+
+template <typename T>
+int forward(Mat x, Mat w, const Epilogue& e, int M, int N, int K, char* work, hipStream_t stream) {
+  Layout l = forward_layout(M, N, K, sizeof(T));
+  if (aligned(x.p, x.ld, sizeof(T))) l.copy[0] = 0;
+  if (aligned(w.p, w.ld, sizeof(T))) l.copy[1] = 0;
+  make_copies<T>(l, x, w, work, stream);
+  return product<T, false, false>(x, w, e, M, N, K, work, stream);
+}
+
 // Sides whose 32-bit indexes have room for a tile past the end.
 bool bad_sides(int M, int N, int K) {
   constexpr int MOST = INT32_MAX - 1023;
@@ -1106,7 +1168,7 @@ bool bad_types(int dtype, int act) { return dtype < CIT_FP32 || dtype > CIT_FP16
 extern "C" {
 
 size_t cit_linear_forward_work_bytes(int M, int N, int K, int dtype) {
-  return bad_types(dtype, 0) || bad_sides(M, N, K) || !M || !N || !K ? 0 : (size_t)split_bytes(M, N, K, elt(dtype));
+  return bad_types(dtype, 0) || bad_sides(M, N, K) || !M || !N || !K ? 0 : (size_t)forward_layout(M, N, K, elt(dtype)).bytes();
 }
 
 size_t cit_linear_backward_work_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* dx,
@@ -1128,9 +1190,10 @@ int cit_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
   Epilogue e = {};
   e.bias = bias, e.res = residual, e.out = y, e.z = z, e.ldr = ldr, e.ldo = N, e.act = act;
   const Mat a = {x, ldx, M, K, K}, b = {w, ldw, N, K, K};
-  if (dtype == CIT_FP32) return product<float, false, false>(a, b, e, M, N, K, work, stream);
-  if (dtype == CIT_BF16) return product<bf16_t, false, false>(a, b, e, M, N, K, work, stream);
-  return product<fp16_t, false, false>(a, b, e, M, N, K, work, stream);
+  char* p = static_cast<char*>(work);
+  if (dtype == CIT_FP32) return forward<float>(a, b, e, M, N, K, p, stream);
+  if (dtype == CIT_BF16) return forward<bf16_t>(a, b, e, M, N, K, p, stream);
+  return forward<fp16_t>(a, b, e, M, N, K, p, stream);
 }
 
 int cit_linear_backward(const void* dy, int64_t ldy, const void* z, const void* x, int64_t ldx, const void* w,

@@ -146,6 +146,20 @@ def test_linear_large(dtype):
         check_linear(*linear_inputs(*size, DT[dtype], "gelu", True, True), "gelu", str(size))
 
 
+# (rows, in, out): few outputs over a long reduction (dw over the rows, y over `in`), shared out by tiles of 64 and 128,
+# with and without whole chunks; many outputs in each of the larger tiles, with a part of a tile at either end; odd rows
+# of a product large enough to be copied first
+SHARED = [(4100, 520, 130), (9000, 264, 520), (16400, 768, 776), (32768, 64, 512), (16390, 130, 259), (40001, 67, 130),
+          (128, 8200, 520), (100, 16392, 264), (520, 4104, 1032), (1030, 8192, 1000)]
+LARGE = [(2570, 520, 5000), (4100, 1032, 2310), (6150, 516, 3010), (9000, 520, 1030), (4001, 1001, 2003)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("size", SHARED + LARGE, ids=str)
+def test_linear_tiles(size, dtype):
+    check_linear(*linear_inputs(*size, DT[dtype], "gelu", True, True), "gelu", "%s %s" % (size, dtype))
+
+
 @pytest.mark.parametrize("dtype", list(DT))
 def test_linear_strides_and_alignment(dtype):
     """Rows further apart than their width, storage that starts at any element, transposed and expanded tensors."""
