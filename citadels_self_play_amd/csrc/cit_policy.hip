@@ -277,8 +277,11 @@ __device__ __forceinline__ float exp_less(float x, float log2_s) {
 //           KL = D / s - L.
 //   pass 3  the gradient: p = exp(l - m - log s), one exp more
 //
-// bf16 with a reference is bound by the vector units (about 50 operations an
-// entry, 12 of them the three exponentials), the others by memory.
+// bf16 with a reference is bound by the vector units (52 instructions an entry,
+// three of them exponentials at a quarter of the rate), the others by memory.
+// 4096 x 32,768 bf16, gradient included: 250 us, 3.2 TB/s, the vector units at
+// work for 190 of them; without a reference 126 us, 4.3 TB/s; 509 x 50,001 masked,
+// evaluated only, 23 us, 3.3 TB/s.
 template <typename T, int G, int NV, int E, bool REF, bool PARTED>
 __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 ? 4 : E > 1 && REF && !PARTED ? 5 : 2) void k_policy(Policy a, int64_t row_blocks, int tail) {
   constexpr int THREADS = G > 256 ? G : 256, GROUPS = THREADS / G;
