@@ -649,8 +649,8 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilo
 // 32 x 32 outputs by 8 waves that share out the reduction, k tile by k tile:
 // each wave stages its own tiles in its own 8 KB of LDS (no barrier until the
 // end), and the 8 partial sums meet in LDS in the waves' order.  For layers too
-// small to fill the chip with larger tiles, and for a few rows against a wide
-// weight, whose bytes are then what there is to do: bf16 1 x 16,384 x 4096 34 us,
+// small to fill the chip with larger tiles, and for some rows against a wide
+// weight, whose bytes are then what there is to do: bf16 8 x 16,384 x 4096 35 us,
 // 3.9 TB/s, as fast as a sum over a large tensor reads.
 
 #define SMALL_WAVES 8
@@ -901,6 +901,73 @@ __global__ __launch_bounds__(256) void k_pack(Copies c) {
   }
 }
 
+// ---- a few rows ----------------------------------------------------------------------
+//
+// y for up to ROWS rows of x: a wave reads OUT rows of the weight at a time, 1 KB of
+// each with one load a lane, and multiplies in fp32; `share` waves of a workgroup
+// share the rows of a long reduction.  The weight's bytes are what there is to do:
+// 1 x 4096 x 16,384 bf16 23 us, 5.9 TB/s (the tiles of k_gemm_small: 34 us), fp32 50
+// us, 5.4 TB/s (69).
+
+#define FEW_WAVES 8
+
+template <typename T, int ROWS, int OUT>
+__global__ __launch_bounds__(FEW_WAVES * 64) void k_few(Mat x, Mat w, Epilogue e, int M, int N, int K, int share) {
+  constexpr int E = 16 / sizeof(T), SUMS = ROWS * OUT;
+  __shared__ float sums[FEW_WAVES][SUMS];
+  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, groups = FEW_WAVES / share;
+  const int64_t first = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * groups * OUT;
+  const int64_t n0 = first + wave / share * OUT;
+  float acc[ROWS][OUT];
+#pragma unroll
+  for (int m = 0; m < ROWS; m++)
+#pragma unroll
+    for (int o = 0; o < OUT; o++) acc[m][o] = 0.0f;
+  if (n0 < N) {
+    const T *px[ROWS], *pw[OUT];                     // rows past the last one repeat it
+#pragma unroll
+    for (int m = 0; m < ROWS; m++) px[m] = static_cast<const T*>(x.p) + (m < M ? m : M - 1) * x.ld;
+#pragma unroll
+    for (int o = 0; o < OUT; o++) pw[o] = static_cast<const T*>(w.p) + (n0 + o < N ? n0 + o : N - 1) * w.ld;
+    const int step = share * 64 * E;
+    int64_t k = (int64_t)(wave % share * 64 + l) * E;
+#pragma unroll 2
+    for (; k + E <= K; k += step) {
+      Pack16<T> u[ROWS], v[OUT];
+#pragma unroll
+      for (int o = 0; o < OUT; o++) v[o].raw = load16(pw[o] + k);
+#pragma unroll
+      for (int m = 0; m < ROWS; m++) u[m].raw = load16(px[m] + k);
+#pragma unroll
+      for (int i = 0; i < E; i++)
+#pragma unroll
+        for (int m = 0; m < ROWS; m++)
+#pragma unroll
+          for (int o = 0; o < OUT; o++) acc[m][o] = fmaf(to_f(u[m].e[i]), to_f(v[o].e[i]), acc[m][o]);
+    }
+    for (; k < K; k++)                               // the lane in whose chunk the rows end; others are past it
+#pragma unroll
+      for (int m = 0; m < ROWS; m++)
+#pragma unroll
+        for (int o = 0; o < OUT; o++) acc[m][o] = fmaf(to_f(px[m][k]), to_f(pw[o][k]), acc[m][o]);
+  }
+#pragma unroll
+  for (int m = 0; m < ROWS; m++)
+#pragma unroll
+    for (int o = 0; o < OUT; o++) {
+      const float t = wave_sum(acc[m][o]);
+      if (l == 0) sums[wave][m * OUT + o] = t;
+    }
+  __syncthreads();
+  if ((int)threadIdx.x >= groups * SUMS) return;
+  const int g = threadIdx.x / SUMS, j = threadIdx.x % SUMS, m = j / OUT;
+  const int64_t n = first + g * OUT + j % OUT;
+  if (m >= M || n >= N) return;
+  float t = 0.0f;
+  for (int i = 0; i < share; i++) t += sums[g * share + i][j];
+  finish<T>(e, m, (int)n, N, t);
+}
+
 // ---- host side ---------------------------------------------------------------------
 
 int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -1145,9 +1212,15 @@ int backward(Mat dy, const void* z, Mat x, Mat w, void* dx, void* dw, void* db, 
   return rc ? rc : launch_status();
 }
 
+// Rows that k_few takes.  Against k_gemm_small, us at 4096 -> 4096 / 50,000 x 1001 / 65,536 x 512: bf16 1 row 6.0 / 18 /
+// 12 against 9.3 / 29 / 17, 2 rows 7.1 / 22 / 18 against 9.4 / 29 / 17, 4 rows 10 / 36 / 30 against 9.4 / 29 / 17; fp32
+// 4 rows 15 / 41 / 36 against 21 / 52 / 35, 8 rows 19 / 64 / 60 against 21 / 52 / 35.
+bool few(int M, int K, int es) { return M <= (es == 4 ? 4 : 2) && (int64_t)K * es >= 1024; }
+
 // Copies of both operands of a forward product, where their rows cannot start on 16 bytes.
 Layout forward_layout(int M, int N, int K, int es) {
   Layout l = {};
+  if (few(M, K, es)) return l;
   if (forward_copies(M, N, K, es)) {
     l.copy[0] = align256((int64_t)M * padded(K, es) * es);
     l.copy[1] = align256((int64_t)N * padded(K, es) * es);
@@ -1157,8 +1230,25 @@ Layout forward_layout(int M, int N, int K, int es) {
   return l;
 }
 
+template <typename T, int ROWS, int OUT>
+void launch_few(const Mat& x, const Mat& w, const Epilogue& e, int M, int N, int K, hipStream_t stream) {
+  // waves that have 2 KB of each row: as many as 4,096, of a large weight and 1 or 2 rows 8,192 (1 x 4096 x 16,384 bf16:
+  // 34 and 23 us; 1 x 4096 x 4096 5.9 and 6.3; 3 x 4096 x 4096 fp32 15 and 20)
+  const int64_t waves = ROWS > 2 || (int64_t)N * K * sizeof(T) < 48 << 20 ? 4096 : 8192;
+  int share = 1;
+  while (share < FEW_WAVES && (int64_t)cdiv(N, OUT) * share < waves && K >= share * 256 * (16 / (int)sizeof(T))) share *= 2;
+  hipLaunchKernelGGL((k_few<T, ROWS, OUT>), wide_grid(cdiv(N, FEW_WAVES / share * OUT)), dim3(FEW_WAVES * 64), 0, stream,
+                     x, w, e, M, N, K, share);
+}
+
 template <typename T>
 int forward(Mat x, Mat w, const Epilogue& e, int M, int N, int K, char* work, hipStream_t stream) {
+  if (few(M, K, sizeof(T))) {
+    if (M == 1) launch_few<T, 1, 4>(x, w, e, M, N, K, stream);
+    else if (M == 2) launch_few<T, 2, 4>(x, w, e, M, N, K, stream);
+    else if constexpr (sizeof(T) == 4) launch_few<T, 4, 4>(x, w, e, M, N, K, stream);
+    return launch_status();
+  }
   Layout l = forward_layout(M, N, K, sizeof(T));
   if (aligned(x.p, x.ld, sizeof(T))) l.copy[0] = 0;
   if (aligned(w.p, w.ld, sizeof(T))) l.copy[1] = 0;

@@ -154,6 +154,21 @@ SHARED = [(4100, 520, 130), (9000, 264, 520), (16400, 768, 776), (32768, 64, 512
 LARGE = [(2570, 520, 5000), (4100, 1032, 2310), (6150, 516, 3010), (9000, 520, 1030), (4001, 1001, 2003)]
 
 
+# one to a few rows: reductions that end inside a lane's chunk, shared by 1 to 8 waves, outputs that end inside a wave's
+FEW = [(1, 512, 64), (1, 513, 1003), (2, 4100, 77), (3, 2051, 130), (4, 5001, 33), (1, 40003, 5), (2, 16384, 64),
+       (1, 4096, 3000), (4, 260, 9000), (1, 256, 8200), (3, 300, 1), (5, 4096, 300)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("size", FEW, ids=str)
+def test_linear_few_rows(size, dtype):
+    check_linear(*linear_inputs(*size, DT[dtype], "silu", True, True), "silu", "%s %s" % (size, dtype))
+    x, w, b, r, _ = linear_inputs(*size, DT[dtype], "gelu", True, True)
+    pad = lambda t: torch.cat([t, t.new_full((t.shape[0], 3), math.nan)], 1)[:, :t.shape[1]]  # noqa: E731
+    want = ops.linear(x, w, b, residual=r, activation="gelu")
+    assert torch.equal(ops.linear(pad(x), pad(w), b, residual=pad(r), activation="gelu"), want)
+
+
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("size", SHARED + LARGE, ids=str)
 def test_linear_tiles(size, dtype):
