@@ -355,9 +355,9 @@ __device__ __forceinline__ u32x4 frag(const char* lds, int r0, int s) {
 // Workgroup (tile, split): BM x BN outputs by WM x WN waves, over the split's
 // share of the reduction.  Two LDS buffers: while the matrix cores work on one
 // tile, the next one's loads are in flight.  Any alignment; bound by those
-// loads' latency and by what the L2s deliver to 64 x 64 tiles: fp32 4096 x 512 x
-// 418 24 us, 12 of them with the matrix cores at work; fp16 1023 x 2051 x 1537
-// 30 us.  A second tile ahead in registers gained nothing.
+// loads' latency and by what the L2s deliver to 64 x 64 tiles: fp16 1023 x 2051 x
+// 1537 30 us.  A second tile ahead in registers gained nothing.  fp32 comes here
+// only with rows 8 MB apart.
 
 template <typename T, bool AKS, bool BKS, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, int M, int N, int K, int tiles_n,
@@ -426,9 +426,9 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, 
 // ---- the tile kernel with direct loads --------------------------------------------
 //
 // The same product for matrices whose rows start on 16 bytes (and, ks, whose
-// columns are whole chunks): global memory goes straight to LDS
-// (global_load_lds_dwordx4), so a tile costs no registers and no LDS write
-// instructions.  The chunk permutation of Tile is applied to the address each
+// columns are whole chunks), and for fp32 ones of any width in single words:
+// global memory goes straight to LDS (global_load_lds_dwordx4, _dword), so a
+// tile costs no registers and no LDS write instructions.  The chunk permutation of Tile is applied to the address each
 // lane reads, since a wave's 64 chunks land side by side.
 //
 // STAGES tiles of LDS, all but one of them under way while the last is worked
@@ -446,17 +446,19 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, 
 // Bound by the matrix cores (fp32) and by the L2s' 10 TB/s and the LDS reads
 // (16-bit types).  8192 x 4096 x 4096: bf16 forward 217 us, dx 217, dw 202, 1,270
 // to 1,360 TFLOP/s (a library's 8192^3 reaches 1,390 here, its products of this
-// size 970 to 1,220); fp32 1,986 us, 138 TFLOP/s (library 136 to 150).
+// size 970 to 1,220); fp32 1,986 us, 138 TFLOP/s (library 136 to 150).  fp32 in words,
+// 4096 x 512 x 418: 25 us (through registers 27), the matrix cores at work for 12.
 
 typedef const __attribute__((address_space(1))) void* global_ptr;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
-// One thread's share of a tile, asked for but not waited for.  Rows (ks:
-// chunks) past the edge repeat the last one; nothing of them is stored.
-template <typename T, bool KS, int R, int THREADS>
+// One thread's share of a tile, asked for but not waited for, in pieces of W
+// bytes: 16, or 4 for fp32 matrices whose rows are off 16 bytes.  Rows (ks:
+// pieces) past the edge repeat the last one; nothing of them is stored.
+template <typename T, bool KS, int R, int THREADS, int W>
 struct Direct {
   typedef Tile<T, KS, R> L;
-  static constexpr int PER = L::CHUNKS / THREADS;
+  static constexpr int PER = L::CHUNKS * (16 / W) / THREADS, E = W / (int)sizeof(T);
   const char* base;              // the next tile's first row, the same for all lanes
   uint32_t off[PER];             // this thread's chunks behind it
   int64_t step;                  // bytes to the tile after it
@@ -464,17 +466,19 @@ struct Direct {
   __device__ __forceinline__ void start(const Mat& a, int r0, int k0) {
 #pragma unroll
     for (int i = 0; i < PER; i++) {
+      const int id = i * THREADS + (int)threadIdx.x;
       int row, c;
-      L::from(i * THREADS + (int)threadIdx.x, row, c);
+      L::from(id / (16 / W), row, c);
+      const int in = id % (16 / W) * E;                // the piece within its chunk
       int64_t at;
       if (KS) {
-        int col = r0 + c * L::E;
-        if (col + L::E > a.edge) col = a.edge - L::E;
+        int col = r0 + c * L::E + in;
+        if (col + E > a.edge) col = a.edge - E;
         at = row * a.ld + (col - r0);
       } else {
         int r = row;
         if (r0 + r >= a.rows) r = a.rows - 1 - r0;
-        at = r * a.ld + c * L::E;
+        at = r * a.ld + c * L::E + in;
       }
       off[i] = (uint32_t)(at * (int64_t)sizeof(T));
     }
@@ -482,10 +486,14 @@ struct Direct {
     step = KS ? a.ld * BK<T> * (int64_t)sizeof(T) : 128;
   }
   __device__ __forceinline__ void next(char* lds) {
-    char* to = lds + (__builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63) << 4);   // the wave's place; lane i lands 16 i behind it
+    char* to = lds + __builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63) * W;   // the wave's place; lane i lands W i behind it
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-      __builtin_amdgcn_global_load_lds((global_ptr)(base + off[i]), (lds_ptr)(to + i * THREADS * 16), 16, 0, 0);
+    for (int i = 0; i < PER; i++) {
+      const global_ptr from = (global_ptr)(base + off[i]);
+      const lds_ptr at = (lds_ptr)(to + i * THREADS * W);
+      if constexpr (W == 16) __builtin_amdgcn_global_load_lds(from, at, 16, 0, 0);
+      else __builtin_amdgcn_global_load_lds(from, at, 4, 0, 0);
+    }
     base += step;
   }
 };
@@ -520,7 +528,7 @@ __device__ __forceinline__ void arrive_all() {
   __syncthreads();
 }
 
-template <typename T, bool AKS, bool BKS, int BM, int BN, int WM, int WN, int STAGES, bool AHEAD>
+template <typename T, bool AKS, bool BKS, int BM, int BN, int WM, int WN, int STAGES, bool AHEAD, int W>
 __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilogue e, int M, int N, int K, int tiles_m,
                                                              int tiles_n, int k_per_split) {
   constexpr int THREADS = WM * WN * 64;
@@ -543,8 +551,8 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilo
 #pragma unroll
     for (int j = 0; j < TN; j++) acc[i][j] = f32x4{0, 0, 0, 0};
 
-  Direct<T, AKS, BM, THREADS> da;
-  Direct<T, BKS, BN, THREADS> db;
+  Direct<T, AKS, BM, THREADS, W> da;
+  Direct<T, BKS, BN, THREADS, W> db;
   constexpr int LOADS = decltype(da)::PER + decltype(db)::PER;         // a tile's, for each wave
   da.start(A, m0, kb);
   db.start(B, n0, kb);
@@ -878,7 +886,7 @@ __global__ __launch_bounds__(256) void k_db(const float* part, T* db, int N, int
 // Rows that do not start on 16 bytes cost the tile kernel guarded loads through
 // registers.  The backward products, which read them down the rows, are
 // faster over copies with padded rows (bf16 3000 x 1001 x 999: dw 95 -> 42 us);
-// the forward product only where it is large.
+// the forward product and fp32 only where they are large.
 
 struct Copies {
   Mat from[2];
@@ -1056,42 +1064,53 @@ bool aligned(const void* p, int64_t ld, int es) {
 }
 bool direct(const Mat& a, bool ks, int es) { return aligned(a.p, a.ld, es) && (!ks || a.edge % (16 / es) == 0); }
 
+// fp32 matrices of any width take direct loads too, 4 bytes a lane.
+bool by_words(const Mat& a) { return !((uintptr_t)a.p & 3) && a.ld * 4 < 1 << 23; }
+
 int64_t padded(int cols, int es) { return ((int64_t)cols * es + 15) / 16 * 16 / es; }
 
-// Whether the backward pass copies unaligned operands of an M x N x K product first: of many outputs, or of few over a
-// reduction long enough to be split (dw of 65,536 rows x 512 x 418, us with / without: bf16 100 / 413, fp32 322 / 560;
-// 8192 rows 35 / 35).
+// Whether the backward pass copies unaligned operands of an M x N x K product first.  16-bit types: of many outputs, or
+// of few over a reduction long enough to be split (bf16 dw of 65,536 rows x 512 x 418, us with / without: 100 / 413, of
+// 8192 rows 35 / 35).  fp32, which has loads of 4 bytes: of much work (with / without: dx 30,000 x 301 over 1000 183 / 210,
+// dw of 4096 rows x 1100 x 2051 220 / 248; dw of 3000 rows x 1001 x 999 85 / 70, of 65,536 rows x 512 x 418 311 / 284).
 bool worth_copies(int M, int N, int K, int es) {
   int tile;
+  if (es == 4) return !small(M, N) && (double)M * N * K >= 8e9;
   return !small(M, N) ? K >= 256 : K >= 16384 && long_splits(M, N, K, es, true, tile) > 1;
 }
 
 // Whether a forward product whose rows cannot start on 16 bytes copies its operands first: of enough work, and of
 // enough work for each copied element.  With copies / without, us: fp16 4001 x 4003 x 2001 84 / 205, 65,536 x 200 x
-// 418 47 / 59, 3000 x 1001 x 999 27 / 24, 4096 x 512 x 418 13 / 10; fp32 4001 x 4003 x 2001 535 / 622, 65,536 x 200 x
-// 418 171 / 150, 3000 x 1001 x 999 67 / 66.
+// 418 47 / 59, 3000 x 1001 x 999 27 / 24, 4096 x 512 x 418 13 / 10; fp32 4001 x 4003 x 2001 535 / 562, 65,536 x 200 x
+// 418 171 / 148, 3000 x 1001 x 999 67 / 68.
 bool forward_copies(int M, int N, int K, int es) {
   return padded(K, es) != K && !small(M, N) && (double)M * N * K >= 4e9 &&
          (int64_t)M * N / ((int64_t)M + N) >= (es == 4 ? 512 : 192);
 }
 
-template <typename T, bool AKS, bool BKS, int TILE, int WM, int WN, int STAGES, bool AHEAD>
+template <typename T, bool AKS, bool BKS, int TILE, int WM, int WN, int STAGES, bool AHEAD, int W = 16>
 void launch_direct(const Mat& A, const Mat& B, const Epilogue& e, int M, int N, int K, const Plan& p,
                    hipStream_t stream) {
-  hipLaunchKernelGGL((k_gemm_direct<T, AKS, BKS, TILE, TILE, WM, WN, STAGES, AHEAD>), dim3(p.tiles_m * p.tiles_n, p.splits),
+  hipLaunchKernelGGL((k_gemm_direct<T, AKS, BKS, TILE, TILE, WM, WN, STAGES, AHEAD, W>), dim3(p.tiles_m * p.tiles_n, p.splits),
                      dim3(WM * WN * 64), 0, stream, A, B, e, M, N, K, p.tiles_m, p.tiles_n, p.k_per);
 }
 
 template <typename T, bool AKS, bool BKS>
 int product(Mat A, Mat B, Epilogue e, int M, int N, int K, void* work, hipStream_t stream) {
   const bool d = K > 0 && direct(A, AKS, sizeof(T)) && direct(B, BKS, sizeof(T));
-  const Plan p = plan(M, N, K, sizeof(T), d, AKS || BKS);
+  const bool words = !d && K > 0 && sizeof(T) == 4 && by_words(A) && by_words(B);
+  const Plan p = plan(M, N, K, sizeof(T), d || words, AKS || BKS);
   const dim3 tiles = wide_grid((int64_t)p.tiles_m * p.tiles_n), grid(tiles.x, p.splits, tiles.y);
   if (p.splits > 1) e.part = static_cast<float*>(work);
   if (p.tile == TILE_32)
     hipLaunchKernelGGL((k_gemm_small<T, AKS, BKS>), grid, dim3(SMALL_WAVES * 64), 0, stream, A, B, e, M, N, K,
                        p.tiles_n, p.k_per);
-  else if (!d)
+  else if (words) {
+    if constexpr (sizeof(T) == 4) {
+      if (p.tile == TILE_64) launch_direct<T, AKS, BKS, 64, 2, 2, 2, true, 4>(A, B, e, M, N, K, p, stream);
+      else launch_direct<T, AKS, BKS, 128, 2, 2, 2, true, 4>(A, B, e, M, N, K, p, stream);
+    }
+  } else if (!d)
     hipLaunchKernelGGL((k_gemm<T, AKS, BKS, 64, 64, 2, 2>), grid, dim3(256), 0, stream, A, B, e, M, N, K, p.tiles_n,
                        p.k_per);
   else if (p.tile == TILE_64) launch_direct<T, AKS, BKS, 64, 2, 2, 2, true>(A, B, e, M, N, K, p, stream);

@@ -151,7 +151,7 @@ def test_linear_large(dtype):
 # of a product large enough to be copied first
 SHARED = [(4100, 520, 130), (9000, 264, 520), (16400, 768, 776), (32768, 64, 512), (16390, 130, 259), (40001, 67, 130),
           (128, 8200, 520), (100, 16392, 264), (520, 4104, 1032), (1030, 8192, 1000), (16500, 131, 523), (130, 520, 8200)]
-LARGE = [(2570, 520, 5000), (4100, 1032, 2310), (6150, 516, 3010), (9000, 520, 1030), (4001, 1001, 2003)]
+LARGE = [(4000, 801, 1023), (4200, 801, 1023), (2570, 520, 5000), (4100, 1032, 2310), (6150, 516, 3010), (9000, 520, 1030), (4001, 1001, 2003)]
 
 
 # one to a few rows: reductions that end inside a lane's chunk, shared by 1 to 8 waves, outputs that end inside a wave's
@@ -191,6 +191,15 @@ def test_linear_strides_and_alignment(dtype):
         check_linear(view(x, pad, off), view(w, pad, off), b, view(r, pad, off), view(dy, pad, off), "gelu", str((pad, off)))
     check_linear(x.t().contiguous().t(), w.t().contiguous().t(), b, r.t().contiguous().t(), dy.t().contiguous().t(), "gelu")
     check_linear(x[:1].expand(70, 96), w, b, r[:, :1].expand(70, 88), dy[:1, :1].expand(70, 88), "gelu", "expanded")
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_linear_rows_far_apart(dtype):
+    """Rows over 8 MB apart, past what a tile's 32-bit offsets reach."""
+    dt = DT[dtype]
+    x, w, b, r, dy = linear_inputs(300, 72, 3400, dt, "silu", True, True)
+    far = torch.empty(300, (1 << 23) // x.element_size() + 8, dtype=dt, device="cuda")[:, :72]
+    check_linear(far.copy_(x), w, b, r, dy, "silu", "far rows")
 
 
 def test_linear_leading_dimensions_and_empty():
