@@ -124,14 +124,14 @@ struct Lanes {
 // cycles of a wave, where a wave has several rows or a row several waves; a row
 // to a wave takes the 32-bit functions (65,536 x 1,000 bf16: 125 us, 145 with the
 // others).
-struct Verdict {
+struct RowLoss {
   float logp, kl, dlogp;
   double loss;
 };
 
 template <bool DOUBLE>
-__device__ __forceinline__ Verdict judge(const Policy& a, int64_t i, double l, double s, float kl) {
-  Verdict v;
+__device__ __forceinline__ RowLoss row_loss(const Policy& a, int64_t i, double l, double s, float kl) {
+  RowLoss v;
   const double logp = l - (DOUBLE ? log(s) : (double)logf((float)s));
   const double adv = a.adv[i], past = logp - (double)a.old[i];
   const double ratio = DOUBLE ? exp(past) : (double)expf((float)past);
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
   constexpr bool FINE = E == 1;
   __shared__ double sums[GROUPS];
   __shared__ float between[G > 64 ? G / 64 : 1][4];
-  __shared__ Verdict said;
+  __shared__ RowLoss said;
   const float up = a.upstream ? *a.upstream : 1.0f;
   if (a.upstream && a.skip_one && up == 1.0f) return;
   const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
     const T* qrow = REF ? static_cast<const T*>(a.ref) + r.at_ref : nullptr;
     const uint8_t* ok = a.mask ? a.mask + r.at_mask : nullptr;
     T* grow = a.grad ? static_cast<T*>(a.grad) + r.at_grad : nullptr;
-    Verdict v = {0.0f, 0.0f, 0.0f, 0.0};
+    RowLoss v = {0.0f, 0.0f, 0.0f, 0.0};
     bool live = w != 0.0f && !r.bad;
     const float of_action = !PARTED && live ? action_logit<T>(a, r, i) : 0.0f;
     float top = 0.0f, top_q = 0.0f, log2_s = 0.0f, L = 0.0f;
@@ -412,13 +412,13 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
         const double l_a = (double)of_action - top;
         if (G > 64) {            // the first wave for all
           if (threadIdx.x < 64) {
-            v = judge<true>(a, i, l_a, t[0], kl);
+            v = row_loss<true>(a, i, l_a, t[0], kl);
             if (threadIdx.x == 0) said = v;
           }
           __syncthreads();
           v = said;
         } else {
-          v = judge<G != 64>(a, i, l_a, t[0], kl);
+          v = row_loss<G != 64>(a, i, l_a, t[0], kl);
         }
       }
     }
@@ -513,7 +513,7 @@ __global__ __launch_bounds__(64) void k_policy_join(Policy a) {
   }
   s = wave_sum(s), sr = wave_sum(sr), f = wave_sum(f), d = wave_sum(d);
   if (lane) return;
-  Verdict v = {0.0f, 0.0f, 0.0f, 0.0};
+  RowLoss v = {0.0f, 0.0f, 0.0f, 0.0};
   RowState state = {top, top_q, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
   if (w != 0.0f && !(s == 0.0)) {
     float kl = 0.0f;
@@ -524,7 +524,7 @@ __global__ __launch_bounds__(64) void k_policy_join(Policy a) {
       kl = kl < 0.0f ? 0.0f : kl;
     }
     state.log2_s = (float)log2(s);
-    v = judge<true>(a, i, (double)action_logit<T>(a, r, i) - top, s, kl);
+    v = row_loss<true>(a, i, (double)action_logit<T>(a, r, i) - top, s, kl);
     state.dlogp = v.dlogp, state.kl = v.kl, state.live = 1.0f;
   }
   reinterpret_cast<RowState*>(a.row_state)[i] = state;

@@ -73,7 +73,7 @@ bool capturing(hipStream_t stream) {
 
 // `t` as [rows][width] with its entries side by side, and the elements between rows.
 Tensor as_rows(const Tensor& t, int64_t rows, int64_t width, int64_t& ld) {
-  Tensor m = t.dim() == 2 ? t : t.reshape({rows, width});
+  const Tensor r = t.resolve_neg(), m = r.dim() == 2 ? r : r.reshape({rows, width});
   ld = width;
   if (m.is_contiguous()) return m;
   if ((width > 1 && m.stride(1) != 1) || (rows > 1 && m.stride(0) < width)) return m.contiguous();
@@ -333,7 +333,7 @@ std::vector<Tensor> listed(const py::list& from, const std::string& what) {
     out.push_back(THPVariable_Unpack(h.ptr()));
   }
   for (const Tensor& t : out) {
-    if (t.layout() != at::kStrided) throw py::value_error(what + " must be a dense tensor");
+    if (t.layout() != at::kStrided || t.is_neg()) throw py::value_error(what + " must be a dense tensor");
     const at::ScalarType dt = t.scalar_type();
     if (dt != at::kFloat && dt != at::kBFloat16 && dt != at::kHalf)
       throw py::value_error(what + "s must be fp32, bf16 or fp16, not " +

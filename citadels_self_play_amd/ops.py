@@ -39,7 +39,7 @@ def _same_place(first, **others):
             continue
         if not isinstance(t, torch.Tensor):
             raise ValueError("%s must be a tensor, not %s" % (name, type(t).__name__))
-        if t.layout != torch.strided:
+        if t.layout != torch.strided or t.is_neg():
             raise ValueError("%s must be a dense tensor" % name)
         if t.device != first.device:
             raise ValueError("%s is on %s, the first tensor on %s" % (name, t.device, first.device))

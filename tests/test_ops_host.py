@@ -139,3 +139,23 @@ def test_entry_points_refuse(lib):
     assert cl(ptr, ptr, n, t32, t16, 1, 1.0, p, p, need, None) == -1
     assert cl(ptr, ptr, n, t32, t32, 1, math.nan, p, p, need, None) == -1
     assert cl(ptr, ptr, n, t32, t32, 1, 1.0, None, p, need, None) == -1
+
+
+def test_lazily_negated_tensors_refused():
+    """Their memory holds the values before the sign changed."""
+    n = torch._neg_view(T(3, 4))
+    with pytest.raises(ValueError, match="x must be a dense tensor"):
+        ops.linear(n, T(5, 4))
+    with pytest.raises(ValueError, match="logits must be a dense tensor"):
+        policy(logits=n)
+    with pytest.raises(ValueError, match="a gradient must be a dense tensor"):
+        ops.clip_grad_norm([n], 1.0)
+
+
+def test_missing_extension_is_loud(monkeypatch):
+    import sys
+    monkeypatch.setattr(_lib, "_torch_calls", None)
+    monkeypatch.setitem(sys.modules, "citadels_self_play_amd._cit_torch", None)
+    monkeypatch.delattr("citadels_self_play_amd._cit_torch", raising=False)
+    with pytest.raises(_lib.NativeError, match="_cit_torch.so"):
+        _lib.torch_calls()
