@@ -355,17 +355,19 @@ __device__ __forceinline__ u32x4 frag(const char* lds, int r0, int s) {
 // Workgroup (tile, split): BM x BN outputs by WM x WN waves, over the split's
 // share of the reduction.  Two LDS buffers: while the matrix cores work on one
 // tile, the next one's loads are in flight.  Any alignment; bound by those
-// loads' latency and by what the L2s deliver to 64 x 64 tiles: fp16 1023 x 2051 x
-// 1537 30 us.  A second tile ahead in registers gained nothing.  fp32 comes here
-// only with rows 8 MB apart.
+// loads' latency: a second tile ahead in registers gained nothing, but HALVES of a
+// workgroup that take the reduction's tiles in turn did where all workgroups
+// are on the chip at once, two a compute unit (fp16 1023 x 1537 x 2051, 400 tiles, 33
+// -> 29 us; 1100 x 1100 x 3001 43 -> 35; but 3000 x 1001 x 999, 752 tiles, 25 -> 30).
+// fp32 comes here only with rows 8 MB apart.
 
-template <typename T, bool AKS, bool BKS, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, int M, int N, int K, int tiles_n,
-                                                      int k_per_split) {
+template <typename T, bool AKS, bool BKS, int BM, int BN, int WM, int WN, int HALVES>
+__global__ __launch_bounds__(WM* WN * 64 * HALVES) void k_gemm(Mat A, Mat B, Epilogue e, int M, int N, int K, int tiles_n,
+                                                               int k_per_split) {
   constexpr int THREADS = WM * WN * 64;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int STEPS = 2;                              // k steps of a tile: 64 bytes of each row
-  __shared__ __attribute__((aligned(16))) char lds[2][(BM + BN) * 128];
+  __shared__ __attribute__((aligned(16))) char lds[HALVES][2][(BM + BN) * 128];
 
   const int64_t tile = (int64_t)blockIdx.z * gridDim.x + blockIdx.x;
   if (tile >= (int64_t)((M + BM - 1) / BM) * tiles_n) return;
@@ -375,7 +377,8 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, 
   if (AKS) a.rows = ke; else a.cols = ke;
   if (BKS) b.rows = ke; else b.cols = ke;
 
-  const int w = threadIdx.x >> 6;
+  const int half = HALVES > 1 ? threadIdx.x / THREADS : 0, me = threadIdx.x % THREADS;
+  const int w = me >> 6;
   const int wm = (w / WN) * (BM / WM), wn = (w % WN) * (BN / WN);
   f32x4 acc[TM][TN];
 #pragma unroll
@@ -385,20 +388,22 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, 
 
   Stage<T, AKS, BM, THREADS> sa;
   Stage<T, BKS, BN, THREADS> sb;
-  sa.load(a, m0, kb, threadIdx.x);
-  sb.load(b, n0, kb, threadIdx.x);
-  sa.store(lds[0], threadIdx.x);
-  sb.store(lds[0] + BM * 128, threadIdx.x);
+  constexpr int STEP = HALVES * BK<T>;                  // (a half's tile past the end is zeros)
+  const int mine = half * BK<T>;
+  sa.load(a, m0, kb + mine, me);
+  sb.load(b, n0, kb + mine, me);
+  sa.store(lds[half][0], me);
+  sb.store(lds[half][0] + BM * 128, me);
   __syncthreads();
   int cur = 0;
-  for (int k = kb; k < ke; k += BK<T>) {
-    const bool more = k + BK<T> < ke;
+  for (int k = kb; k < ke; k += STEP) {
+    const bool more = k + STEP < ke;
     if (more) {
-      sa.load(a, m0, k + BK<T>, threadIdx.x);
-      sb.load(b, n0, k + BK<T>, threadIdx.x);
+      sa.load(a, m0, k + STEP + mine, me);
+      sb.load(b, n0, k + STEP + mine, me);
     }
-    const char* la = lds[cur];
-    const char* lb = lds[cur] + BM * 128;
+    const char* la = lds[half][cur];
+    const char* lb = lds[half][cur] + BM * 128;
 #pragma unroll
     for (int s = 0; s < STEPS; s++) {
       u32x4 fa[TM], fb[TN];
@@ -412,15 +417,26 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm(Mat A, Mat B, Epilogue e, 
         for (int j = 0; j < TN; j++) acc[i][j] = mma(fb[j], fa[i], acc[i][j], T{});
     }
     if (more) {
-      sa.store(lds[cur ^ 1], threadIdx.x);
-      sb.store(lds[cur ^ 1] + BM * 128, threadIdx.x);
+      sa.store(lds[half][cur ^ 1], me);
+      sb.store(lds[half][cur ^ 1] + BM * 128, me);
     }
     __syncthreads();
     cur ^= 1;
   }
 
+  if (HALVES > 1) {                                     // the halves' sums meet in the second one's place
+    f32x4* other = reinterpret_cast<f32x4*>(&lds[HALVES - 1][0][0]) + me;
+    static_assert(TM * TN * 16 * THREADS <= (BM + BN) * 256, "the sums fit");
+    if (half)
+#pragma unroll
+      for (int i = 0; i < TM * TN; i++) other[i * THREADS] = acc[i / TN][i % TN];
+    __syncthreads();
+    if (half) return;
+#pragma unroll
+    for (int i = 0; i < TM * TN; i++) acc[i / TN][i % TN] += other[i * THREADS];
+  }
   constexpr int SHARE = (BM + BN) * 256 / (WM * WN);
-  write_out<T, TM, TN, SHARE>(e, acc, &lds[0][0] + w * SHARE, m0 + wm, n0 + wn, M, N, split);
+  write_out<T, TM, TN, SHARE>(e, acc, &lds[0][0][0] + w * SHARE, m0 + wm, n0 + wn, M, N, split);
 }
 
 // ---- the tile kernel with direct loads --------------------------------------------
@@ -665,8 +681,8 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilo
 #define SMALL_LDS (SMALL_WAVES * 64 * 128)
 
 template <typename T, bool AKS, bool BKS, bool DZ>
-__device__ __forceinline__ void small_tile(const Mat& A, const Mat* Z, const Mat& B, const Epilogue& e, int act, int M, int N, int K,
-                           int m0, int n0, int split, int k_per_split, char* lds) {
+__device__ __forceinline__ void small_tile(const Mat& A, const Mat* Z, const Mat& B, const Epilogue& e, int act, int M,
+                                           int N, int K, int m0, int n0, int split, int k_per_split, char* lds) {
   const int kb = split * k_per_split, ke = min(K, kb + k_per_split);
   Mat a = A, b = B;
   if (AKS) a.rows = ke; else a.cols = ke;
@@ -1110,8 +1126,12 @@ int product(Mat A, Mat B, Epilogue e, int M, int N, int K, void* work, hipStream
       if (p.tile == TILE_64) launch_direct<T, AKS, BKS, 64, 2, 2, 2, true, 4>(A, B, e, M, N, K, p, stream);
       else launch_direct<T, AKS, BKS, 128, 2, 2, 2, true, 4>(A, B, e, M, N, K, p, stream);
     }
+  } else if (!d && sizeof(T) == 2 && (int64_t)p.tiles_m * p.tiles_n <= 512) {
+    if constexpr (sizeof(T) == 2)
+      hipLaunchKernelGGL((k_gemm<T, AKS, BKS, 64, 64, 2, 2, 2>), grid, dim3(512), 0, stream, A, B, e, M, N, K, p.tiles_n,
+                         p.k_per);
   } else if (!d)
-    hipLaunchKernelGGL((k_gemm<T, AKS, BKS, 64, 64, 2, 2>), grid, dim3(256), 0, stream, A, B, e, M, N, K, p.tiles_n,
+    hipLaunchKernelGGL((k_gemm<T, AKS, BKS, 64, 64, 2, 2, 1>), grid, dim3(256), 0, stream, A, B, e, M, N, K, p.tiles_n,
                        p.k_per);
   else if (p.tile == TILE_64) launch_direct<T, AKS, BKS, 64, 2, 2, 2, true>(A, B, e, M, N, K, p, stream);
   else if (p.tile == TILE_128 && p.deep) launch_direct<T, AKS, BKS, 128, 2, 2, 4, true>(A, B, e, M, N, K, p, stream);

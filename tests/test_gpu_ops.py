@@ -168,9 +168,12 @@ def test_linear_few_rows(size, dtype):
     want = ops.linear(x, w, b, residual=r, activation="gelu")
     assert torch.equal(ops.linear(pad(x), pad(w), b, residual=pad(r), activation="gelu"), want)
 
+# odd rows through registers in each of the three products, by one or two halves of a workgroup
+ODD = [(2100, 131, 1100), (1030, 259, 1030), (3000, 700, 201), (2500, 700, 201), (200, 1501, 1500), (200, 1101, 1100)]
+
 
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("size", SHARED + LARGE, ids=str)
+@pytest.mark.parametrize("size", SHARED + LARGE + ODD, ids=str)
 def test_linear_tiles(size, dtype):
     check_linear(*linear_inputs(*size, DT[dtype], "gelu", True, True), "gelu", "%s %s" % (size, dtype))
     if size[0] == 16500:           # dy itself copied to padded rows
