@@ -11,6 +11,7 @@
 #include <hip/hip_runtime_api.h>
 #include <torch/extension.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <c10/hip/HIPStream.h>
@@ -88,6 +89,24 @@ void first_only(const char* what) {
     throw std::runtime_error(std::string("ops.") + what +
                              " has first derivatives only: its backward pass cannot run with create_graph=True");
 }
+// A backward pass under capture hands its gradients to its leaves' nodes, on the streams that these were made on.  A
+// node that an eager graph keeps alive has a stream outside the capture, and torch's engine, joining the two, would
+// end the process: refused while that is still an error.
+void leaves_in_capture(const torch::autograd::Node& node, hipStream_t stream, const char* what) {
+  if (!capturing(stream)) return;
+  for (size_t i = 0; i < node.num_outputs(); i++) {
+    const auto& leaf = node.next_edge(i).function;
+    if (!leaf || !node.task_should_compute_output(i) || !dynamic_cast<torch::autograd::AccumulateGrad*>(leaf.get()))
+      continue;
+    const std::optional<c10::Stream> s = leaf->stream();
+    if (!s) continue;
+    const hipStream_t other = c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *s).stream();
+    if (other != stream && (!other || !capturing(other)))
+      throw std::runtime_error(std::string("ops.") + what +
+                               ": a backward pass cannot be captured while an eager graph of the same leaves is alive");
+  }
+}
+
 void no_tangent(std::initializer_list<Tensor> given, const char* what) {
   for (const Tensor& t : given)
     if (t.defined() && t._fw_grad(0).defined())
@@ -115,13 +134,14 @@ struct LinearBackward : torch::autograd::Node {
     const Tensor& dy = grads[0];
     if (!dy.defined()) return out;
     first_only("linear");
+    const On on(dy);
+    leaves_in_capture(*this, on.stream, "linear");
     const bool nx = task_should_compute_output(0), nw = task_should_compute_output(1),
                nb = task_should_compute_output(2);
     if (task_should_compute_output(3)) out[3] = dy;
     if (!(nx || nw || nb)) return out;
     Tensor vx = nw ? x.unpack() : Tensor(), vw = nx ? w.unpack() : Tensor();
     Tensor vz = act ? z.unpack(own_y ? shared_from_this() : nullptr) : Tensor();
-    const On on(dy);
     const auto make = [&](at::IntArrayRef size, bool yes) {
       return !yes ? Tensor() : M && N ? at::empty(size, dy.options()) : at::zeros(size, dy.options());
     };
@@ -254,6 +274,7 @@ struct PolicyLossBackward : torch::autograd::Node {
     Tensor v[8];
     for (int i = 0; i < 8; i++) v[i] = given[i].unpack();
     const On on(v[0]);
+    leaves_in_capture(*this, on.stream, "policy_loss");
     // a second backward pass finds none: the first one's gradient is its owner's.  A graph replayed on its own may
     // find the forward pass's gradient used up
     Tensor grad = std::move(held);

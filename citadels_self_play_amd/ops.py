@@ -11,7 +11,7 @@ Tensors are fp32, bf16 or fp16 on one GPU.  Every call runs on the current
 stream of its tensors' device, takes its workspace from torch's caching
 allocator and waits for nothing.  Calls can be captured into a HIP graph (a
 backward pass too, while no eager graph of the same leaves is alive: torch's
-autograd engine joins the two graphs' streams, whatever the operators).
+autograd engine would join the two graphs' streams; RuntimeError).
 Wrong arguments raise ValueError before anything is launched.
 
 The checks are written out rather than shared: at a trainer's batch of 64 a

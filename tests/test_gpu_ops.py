@@ -1063,6 +1063,30 @@ def test_training_step_in_a_graph():
             assert torch.equal(p, q), k
 
 
+def test_capture_beside_an_eager_graph_is_refused():
+    x, w, b, r, dy = linear_inputs(37, 50, 41, torch.float32, "silu", True, False)
+    a = policy_rows([4, 9, 30], torch.float32)
+    w.requires_grad_()
+    l = a["logits"].requires_grad_()
+    want = torch.autograd.grad(ops.linear(x, w, b), w, dy)[0]
+    eager = ops.linear(x, w), call_policy(a, (0.2, 0.2), 0.1, l).loss
+    torch.cuda.synchronize()
+    for back in (lambda: torch.autograd.grad(ops.linear(x, w, b), w, dy),
+                 lambda: torch.autograd.grad(call_policy(a, (0.2, 0.2), 0.1, l).loss, l)):
+        with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                back()
+        torch.cuda.synchronize()
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(ops.linear(x, w, b), w, dy)[0]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_two_streams_at_once():
     """Two steps on two streams, one after another from the host, each with its own workspaces."""
     params, x, a = step_inputs(torch.float32)
