@@ -7,7 +7,7 @@
 // The nodes are C++ because a backward pass runs on torch's own thread for the
 // device: a Python one has to be woken there with the interpreter's lock, in
 // another core's caches (64 x 418 -> 512, forward and backward, host time:
-// 109 us with Python nodes, 44 of them work).
+// 109 us with Python nodes, 58 with these; a ReLU's own takes 46).
 #include <hip/hip_runtime_api.h>
 #include <torch/extension.h>
 #include <torch/csrc/autograd/function.h>
