@@ -1256,16 +1256,15 @@ int backward(Mat dy, const void* z, Mat x, Mat w, void* dx, void* dw, void* db, 
 // 4 rows 15 / 41 / 36 against 21 / 52 / 35, 8 rows 19 / 64 / 60 against 21 / 52 / 35.
 bool few(int M, int K, int es) { return M <= (es == 4 ? 4 : 2) && (int64_t)K * es >= 1024; }
 
-// Copies of both operands of a forward product, where their rows cannot start on 16 bytes.
+// Copies of both operands of a forward product, where their rows cannot start on 16 bytes, and the splits' sums.
 Layout forward_layout(int M, int N, int K, int es) {
   Layout l = {};
   if (few(M, K, es)) return l;
   if (forward_copies(M, N, K, es)) {
     l.copy[0] = align256((int64_t)M * padded(K, es) * es);
     l.copy[1] = align256((int64_t)N * padded(K, es) * es);
-  } else {
-    l.split = split_bytes(M, N, K, es, false);
   }
+  l.split = split_bytes(M, N, K, es, false);
   return l;
 }
 
@@ -1289,10 +1288,11 @@ int forward(Mat x, Mat w, const Epilogue& e, int M, int N, int K, char* work, hi
     return launch_status();
   }
   Layout l = forward_layout(M, N, K, sizeof(T));
+  char* sums = work + l.copy[0] + l.copy[1];
   if (aligned(x.p, x.ld, sizeof(T))) l.copy[0] = 0;
   if (aligned(w.p, w.ld, sizeof(T))) l.copy[1] = 0;
   make_copies<T>(l, x, w, work, stream);
-  return product<T, false, false>(x, w, e, M, N, K, work, stream);
+  return product<T, false, false>(x, w, e, M, N, K, sums, stream);
 }
 
 // Sides whose 32-bit indexes have room for a tile past the end.

@@ -150,7 +150,7 @@ def test_linear_large(dtype):
 # with and without whole chunks; many outputs in each of the larger tiles, with a part of a tile at either end; odd rows
 # of a product large enough to be copied first
 SHARED = [(4100, 520, 130), (9000, 264, 520), (16400, 768, 776), (32768, 64, 512), (16390, 130, 259), (40001, 67, 130),
-          (128, 8200, 520), (100, 16392, 264), (520, 4104, 1032), (1030, 8192, 1000), (16500, 131, 523), (130, 520, 8200)]
+          (128, 8200, 520), (100, 16392, 264), (520, 4104, 1032), (1030, 8192, 1000), (16500, 131, 523), (130, 520, 8200), (1000, 8201, 1100)]
 LARGE = [(4000, 801, 1023), (4200, 801, 1023), (2570, 520, 5000), (4100, 1032, 2310), (6150, 516, 3010), (9000, 520, 1030), (4001, 1001, 2003)]
 
 

@@ -159,3 +159,11 @@ def test_missing_extension_is_loud(monkeypatch):
     monkeypatch.delattr("citadels_self_play_amd._cit_torch", raising=False)
     with pytest.raises(_lib.NativeError, match="_cit_torch.so"):
         _lib.torch_calls()
+
+
+def test_copies_and_split_sums_have_room_of_their_own(lib):
+    """A forward product of odd rows whose operands are copied and whose long reduction is shared out as well."""
+    M, N, K = 1000, 1100, 8201
+    for dtype, size in ((0, 4), (1, 2), (2, 2)):
+        row = -(-K * size // 16) * 16
+        assert lib.cit_linear_forward_work_bytes(M, N, K, dtype) >= (M + N) * row + 2 * M * N * 4
