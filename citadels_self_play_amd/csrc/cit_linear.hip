@@ -176,6 +176,15 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n, int
   store8<T>(static_cast<T*>(e.out) + m * e.ldo + n, o);
 }
 
+// Until this wave's LDS writes are there for its other lanes, and its reads done before they are written over.  (A wave's
+// LDS accesses run in their order; this keeps the compiler from moving one past another, whatever it knows of their
+// addresses.)
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // A wave's sums, TM x TN blocks of 16 x 16 from (m0, n0) on, through its own
 // `bytes` of LDS so that rows leave in whole lines: a lane holds 4 columns of
 // one row (a 16-byte chunk; chunks permuted by the row against bank conflicts) and
@@ -197,6 +206,7 @@ __device__ __forceinline__ void write_out(const Epilogue& e, const f32x4 (&acc)[
         const int r = (i - i0) * 16 + (l & 15), c = j * 4 + (l >> 4);
         *reinterpret_cast<f32x4*>(lds + r * ROW + ((c ^ (r & (CHUNKS - 1))) << 4)) = acc[i][j];
       }
+    wave_fence();
     const int rows = (TM - i0 < PER ? TM - i0 : PER) * 16;
     for (int k = l; k < rows * (CHUNKS / 2); k += 64) {
       const int r = k / (CHUNKS / 2), c = k % (CHUNKS / 2) * 2, x = r & (CHUNKS - 1);
@@ -208,6 +218,7 @@ __device__ __forceinline__ void write_out(const Epilogue& e, const f32x4 (&acc)[
         finish8<T>(e, m, n, N, v, split, M);
       }
     }
+    wave_fence();
   }
 }
 
@@ -709,9 +720,7 @@ __device__ __forceinline__ void small_tile(const Mat& A, const Mat* Z, const Mat
       sa.load(a, m0, k + STEP, l, Z);
       sb.load(b, n0, k + STEP, l);
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_fence();
 #pragma unroll
     for (int s = 0; s < 2; s++) {
       u32x4 fa[2], fb[2];
@@ -723,9 +732,7 @@ __device__ __forceinline__ void small_tile(const Mat& A, const Mat* Z, const Mat
 #pragma unroll
       for (int i = 0; i < 4; i++) acc[i >> 1][i & 1] = mma(fb[i & 1], fa[i >> 1], acc[i >> 1][i & 1], T{});
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_fence();
   }
   // [wave][row][chunk of 4 columns, permuted by the row]
 #pragma unroll
