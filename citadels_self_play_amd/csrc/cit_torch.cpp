@@ -67,10 +67,17 @@ Tensor workspace(size_t bytes, const Tensor& like) {
   return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
-bool capturing(hipStream_t stream) {
+// A number of the capture that the stream is part of; 0: none.
+unsigned long long capture_of(hipStream_t stream) {
   hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
-  return hipStreamIsCapturing(stream, &s) == hipSuccess && s != hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(stream, &s, &id) != hipSuccess) {
+    (void)hipGetLastError();             // not the next launch's
+    return 0;
+  }
+  return s == hipStreamCaptureStatusNone ? 0 : id + 1;
 }
+bool capturing(hipStream_t stream) { return capture_of(stream) != 0; }
 
 // `t` as [rows][width] with its entries side by side, and the elements between rows.
 Tensor as_rows(const Tensor& t, int64_t rows, int64_t width, int64_t& ld) {
@@ -257,7 +264,7 @@ struct PolicyLossBackward : torch::autograd::Node {
   SavedVariable given[8];                // logits, ref, mask, offsets, actions, old, adv, weights
   Scalars s;
   Tensor held;                           // the gradient for an upstream gradient of 1
-  bool captured = false;                 // it was made within a graph capture
+  unsigned long long made_in = 0;        // the capture that it was made in; 0: none
 
   std::string name() const override { return "PolicyLossBackward"; }
   void release_variables() override {
@@ -275,12 +282,13 @@ struct PolicyLossBackward : torch::autograd::Node {
     for (int i = 0; i < 8; i++) v[i] = given[i].unpack();
     const On on(v[0]);
     leaves_in_capture(*this, on.stream, "policy_loss");
-    // a second backward pass finds none: the first one's gradient is its owner's.  A graph replayed on its own may
-    // find the forward pass's gradient used up
-    Tensor grad = std::move(held);
-    held = Tensor();
-    const bool ready = grad.defined() && (captured || !capturing(on.stream));
-    if (!grad.defined()) grad = at::empty(v[0].sizes(), v[0].options());
+    // The forward pass's gradient goes to one backward pass, its owner from then on, that runs as often as the forward
+    // pass does: an eager one after an eager one, or one of the same capture.  Any other works the gradient out again in
+    // memory of its own: a graph's replays would go on writing into an eager pass's, whoever has it by then, and
+    // what a graph keeps for itself may be anything when another one is replayed.
+    const bool ready = held.defined() && made_in == capture_of(on.stream);
+    Tensor grad = ready ? std::move(held) : at::empty(v[0].sizes(), v[0].options());
+    if (ready) held = Tensor();
     out[0] = grad;
     const PolicyArgs a(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
     if (!a.rows) {
@@ -313,7 +321,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Maybe
   }
   no_tangent({logits}, "policy_loss");
   Tensor loss, logp, kl, grad;
-  bool captured = false;
+  unsigned long long made_in = 0;
   {
     at::AutoDispatchBelowADInplaceOrView below;
     const On on(logits);
@@ -322,7 +330,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Maybe
     loss = at::empty({}, f32), logp = at::empty({a.rows}, f32), kl = at::empty({a.rows}, f32);
     if (node) {
       grad = a.rows ? at::empty(logits.sizes(), logits.options()) : at::zeros(logits.sizes(), logits.options());
-      captured = capturing(on.stream);
+      made_in = capture_of(on.stream);
     }
     const size_t n = a.bytes();
     const Tensor work = workspace(n, logits);
@@ -338,7 +346,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Maybe
       if (given[i].defined()) node->given[i] = SavedVariable(i && given[i].requires_grad() ? given[i].detach() : given[i], false);
     node->s = Scalars{low, high, beta};
     node->held = std::move(grad);
-    node->captured = captured;
+    node->made_in = made_in;
   }
   return {loss, logp, kl};
 }

@@ -11,7 +11,9 @@ Tensors are fp32, bf16 or fp16 on one GPU.  Every call runs on the current
 stream of its tensors' device, takes its workspace from torch's caching
 allocator and waits for nothing.  Calls can be captured into a HIP graph (a
 backward pass too, while no eager graph of the same leaves is alive: torch's
-autograd engine would join the two graphs' streams; RuntimeError).
+autograd engine would join the two graphs' streams; RuntimeError).  A backward
+pass captured apart from its forward pass needs retain_graph=True, and the
+forward pass's outputs alive as long as it is replayed.
 Wrong arguments raise ValueError before anything is launched.
 
 The checks are written out rather than shared: at a trainer's batch of 64 a

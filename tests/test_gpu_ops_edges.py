@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_ops import DT, U, call_policy
+from test_gpu_ops import DT, U, call_policy, policy_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,69 @@ def test_policy_loss_that_cancels(rows, width, dtype):
     for ref in (None, a["logits"]):
         got = call_policy(dict(a, ref=ref), (0.2, 0.2), 0.0)
         assert abs(float(got.loss) - want) <= U * abs(want) + 1e-13 * float(terms.abs().mean()), (float(got.loss), want)
+
+
+def test_policy_gradient_belongs_to_its_pass():
+    """A forward and a backward pass of two captures, or one eager and one captured: each replay gives the gradient of
+    what it finds, in memory that nothing else has."""
+    s = torch.cuda.Stream()
+    a = policy_rows([4, 9, 30, 64], torch.float32)
+    l = a["logits"].requires_grad_()
+    up = torch.ones((), device="cuda")
+
+    def want(v):
+        c = l.detach().clone().requires_grad_()
+        return torch.autograd.grad(call_policy(a, (0.2, 0.2), 0.1, c).loss, c, torch.tensor(v, device="cuda"))[0]
+
+    want(1.0)
+    torch.cuda.synchronize()
+    # both captured, each for itself: the second one replayed again, its result changed in between
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first, stream=s):
+        loss = call_policy(a, (0.2, 0.2), 0.1, l).loss
+    with torch.cuda.graph(second, stream=s):
+        grad = torch.autograd.grad(loss, l, up, retain_graph=True)[0]
+    for _ in range(3):
+        l.data.mul_(0.9)
+        first.replay()
+        for v in (0.5, 1.0, 1.0, -2.0):
+            up.fill_(v)
+            second.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(grad, want(v)), v
+            grad.mul_(3.0)
+            torch.cuda.synchronize()
+    # captured, then an eager backward pass: its gradient is the caller's, and stays
+    with torch.cuda.stream(s):
+        mine = torch.autograd.grad(loss, l, retain_graph=True)[0]
+    torch.cuda.synchronize()
+    kept = want(1.0)
+    assert torch.equal(mine, kept)
+    l.data.mul_(0.9)
+    for _ in range(2):
+        first.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(mine, kept)
+    # eager, then a captured backward pass through logits that are no leaf: what the allocator gives out meanwhile is not
+    # written to
+    with torch.cuda.stream(s):
+        leaf = l.detach().clone().requires_grad_()
+        eager = call_policy(a, (0.2, 0.2), 0.1, leaf * 1.0).loss
+    torch.cuda.synchronize()
+    third = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(third, stream=s):
+        grad = torch.autograd.grad(eager, leaf, up, retain_graph=True)[0]
+    with torch.cuda.stream(s):
+        others = [torch.full_like(leaf, 7.0) for _ in range(64)]
+    torch.cuda.synchronize()
+    for v in (1.0, 0.5, 1.0):
+        up.fill_(v)
+        third.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want(v)), v
+        assert all(bool((t == 7.0).all()) for t in others)
+    # the same node once more, eager: the gradient that its forward pass made
+    with torch.cuda.stream(s):
+        again = torch.autograd.grad(eager, leaf)[0]
+    torch.cuda.synchronize()
+    assert torch.equal(again, want(1.0))
