@@ -192,8 +192,9 @@ int cit_clip_grad_norm(const void* const* grads, void* const* out, const int64_t
     total += sizes[t];
     count += sizes[t] > 0;
   }
-  const int lists_needed = count ? (count + GN_LIST - 1) / GN_LIST : 1;
-  const int each = (count + lists_needed - 1) / lists_needed;          // lists of equal length: none left with a few
+  // lists of equal length: none left with a few; of at least one, also where no tensor holds anything
+  const int lists_needed = (count + GN_LIST - 1) / GN_LIST;
+  const int each = count ? (count + lists_needed - 1) / lists_needed : 1;
   // about 8 GN_BLOCKS chunks in all, so that each launch of a long list has enough workgroups
   int64_t chunk = (total / (8 * GN_BLOCKS) + 2047) / 2048 * 2048;
   if (chunk < 2048) chunk = 2048;

@@ -7,6 +7,7 @@ import math
 import pytest
 import torch
 
+from citadels_self_play_amd import ops
 from test_gpu_ops import DT, U, call_policy, policy_rows
 
 pytestmark = pytest.mark.gpu
@@ -105,3 +106,12 @@ def test_policy_gradient_belongs_to_its_pass():
         again = torch.autograd.grad(eager, leaf)[0]
     torch.cuda.synchronize()
     assert torch.equal(again, want(1.0))
+
+
+# ---- gradient norm ------------------------------------------------------------------
+
+def test_clip_of_tensors_that_hold_nothing():
+    for n in (1, 3, 200):
+        grads = [torch.empty((0, 3), device="cuda") for _ in range(n)]
+        assert float(ops.grad_norm(grads)) == 0.0 and float(ops.clip_grad_norm(grads, 1.0)) == 0.0
+        assert float(ops.clip_grad_norm(grads, 1.0, out=[t.clone() for t in grads])) == 0.0

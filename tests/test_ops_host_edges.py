@@ -1,0 +1,28 @@
+"""Edges of the training / serving operators (citadels_self_play_amd/ops.py and
+their C entry points) that end on the host."""
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+CLIP_EMPTY = """
+import ctypes as C
+from citadels_self_play_amd import _lib
+lib = _lib.load()
+b = C.create_string_buffer(1 << 17)
+p = (C.addressof(b) + 255) // 256 * 256
+none, sizes, types = (C.c_void_p * 3)(), (C.c_int64 * 3)(), (C.c_int32 * 3)()
+need = lib.cit_clip_grad_norm_work_bytes(3)
+for out in (none, None):
+    rc = lib.cit_clip_grad_norm(none, out, sizes, types, types, 3, 1.0, p, p, need, None)
+    assert rc not in (0, -1), rc
+"""
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the buffers are the host's: only for where there is no device to launch on")
+def test_clip_of_tensors_that_hold_nothing_ends():
+    """Every tensor of the list empty: on to the launch, which has no device here."""
+    subprocess.run([sys.executable, "-c", CLIP_EMPTY], check=True, timeout=60,
+                   cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
