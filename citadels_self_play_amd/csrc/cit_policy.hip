@@ -15,7 +15,8 @@
 // keep their digits (sum p d cancels to nothing there); where the reference is
 // much the flatter one, whose sum then outweighs KL, as p d.  A row of weight 0 is
 // not read; a row that leaves no entry counts nothing, and the gradients of
-// both are 0.  An action outside its row makes the row NaN.
+// both are 0.  An action outside its row makes the row NaN.  Where beta is 0 KL is
+// told and no part of the loss, also where it is infinite.
 #include <type_traits>
 
 #include "cit_ops.h"
@@ -139,7 +140,7 @@ __device__ __forceinline__ RowLoss row_loss(const Policy& a, int64_t i, double l
   const double free = ratio * adv, held = (ratio < low ? low : ratio > high ? high : ratio) * adv;
   v.logp = (float)logp, v.kl = kl;
   v.dlogp = (float)(free <= held ? -free : held < free ? 0.0 : (double)NAN);
-  v.loss = (free <= held || free != free ? -free : -held) + (a.ref ? (double)a.beta * (double)kl : 0.0);
+  v.loss = (free <= held || free != free ? -free : -held) + (a.ref && a.beta != 0.0f ? (double)a.beta * (double)kl : 0.0);
   return v;
 }
 

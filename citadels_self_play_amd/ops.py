@@ -134,7 +134,8 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logits=None, offse
     A masked action has rho 0; an action outside its row, or offsets that
     leave the list, give NaN (what gradient the entries of no row then have is
     not defined).  KL is infinite where p_ref is 0 and p is not, and
-    NaN where the reference leaves nothing of a row."""
+    NaN where the reference leaves nothing of a row; with kl_coef 0 it is
+    told, whatever it is, and is no part of the loss."""
     _same_place(logits if isinstance(logits, torch.Tensor) else torch.empty(0), logits=logits, actions=actions,
                 old_logp=old_logp, advantages=advantages, ref_logits=ref_logits, offsets=offsets, mask=mask,
                 weights=weights)

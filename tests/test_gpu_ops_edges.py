@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from citadels_self_play_amd import ops
-from test_gpu_ops import DT, U, call_policy, policy_rows
+from test_gpu_ops import DT, U, call_policy, policy_rows, policy_want, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -106,6 +106,28 @@ def test_policy_gradient_belongs_to_its_pass():
         again = torch.autograd.grad(eager, leaf)[0]
     torch.cuda.synchronize()
     assert torch.equal(again, want(1.0))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("dense", [(5, 12), (5, 200), (4, 1500), (3, 9001), (3, 20001)], ids=str)
+def test_policy_kl_watched_only(dense, dtype):
+    """kl_coef 0 with a reference that rules out what the policy plays, or leaves nothing: KL says so, loss and
+    gradient are those without a reference."""
+    a = policy_rows(None, DT[dtype], dense=dense)
+    a["ref"][0, int(a["actions"][0])] = -math.inf
+    a["ref"][1] = -math.inf
+    a["ref"][2, 3] = math.nan
+    want = policy_want(dict(a, ref=None), (0.2, 0.2), 0.0)
+    l = a["logits"].detach().requires_grad_()
+    for leaf in (a["logits"], l):
+        got = call_policy(a, (0.2, 0.2), 0.0, leaf)
+        within(got.loss.detach(), *want[0], what="loss")
+        within(got.logp, *want[1], what="logp")
+        assert float(got.kl[0]) == math.inf and bool(got.kl[1:3].isnan().all())
+    for up in (1.0, 0.5):
+        grad = torch.autograd.grad(got.loss, l, torch.tensor(up, device="cuda"), retain_graph=True)[0]
+        v, t = want[3]
+        within(grad, v * up, (t + U * v.abs()) * up + tiny(DT[dtype]), what="grad")
 
 
 # ---- gradient norm ------------------------------------------------------------------
