@@ -50,7 +50,7 @@ struct PartSums {                // maxima and sums of k_policy's pass 2 over on
   float m, mr, s, sr, f, d;
 };
 struct RowState {                // what the gradient needs of a row
-  float top, top_q, log2_s, L, dlogp, kl, live;
+  float top, top_q, inv_s, L, dlogp, kl, live;
 };
 
 struct Row {
@@ -253,17 +253,12 @@ __device__ void clear_ends(const Policy& a, int block, int blocks) {
 
 #define LOG2E 1.44269504088896341f
 
-// exp(x), and exp(x - ln s) from log2 s.  FINE: to the last place, for short rows; over long ones what the product
-// x log2(e) is off by, |x| last places, averages out, and the instruction alone does (fp32 2,048 x 16,384: 93 us, 108).
+// exp(x).  FINE: to the last place, for short rows; over long ones what the product x log2(e) is off by, |x| last
+// places, averages out, and the instruction alone does (fp32 2,048 x 16,384: 93 us, 108).
 template <bool FINE>
 __device__ __forceinline__ float exp_of(float x) {
   return FINE ? expf(x) : __builtin_amdgcn_exp2f(x * LOG2E);
 }
-template <bool FINE>
-__device__ __forceinline__ float exp_less(float x, float log2_s) {
-  return FINE ? expf(fmaf(log2_s, -0.693147180559945309f, x)) : __builtin_amdgcn_exp2f(fmaf(x, LOG2E, -log2_s));
-}
-
 // A row by G lanes, each with up to NV packs of E entries in registers, so that
 // the logits come from memory once; a longer row is read again in each pass.
 //
@@ -276,7 +271,9 @@ __device__ __forceinline__ float exp_less(float x, float log2_s) {
 //           KL = F / s + eta - L.  One pass gives KL without its cancellation.
 //           Where sr > 2 s that would take sr away from F: D = sum e x, and
 //           KL = D / s - L.
-//   pass 3  the gradient: p = exp(l - m - log s), one exp more
+//   pass 3  the gradient: exp(l - m) once more, 1 / s in what it is multiplied
+//           with: rounded by half a step, where a log s in the exponent would put its
+//           own rounding, up to ten steps, on all of a row alike
 //
 // bf16 with a reference is bound by the vector units (52 instructions an entry,
 // three of them exponentials at a quarter of the rate), the others by memory.
@@ -321,7 +318,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
     RowLoss v = {0.0f, 0.0f, 0.0f, 0.0};
     bool live = w != 0.0f && !r.bad;
     const float of_action = !PARTED && live ? action_logit<T>(a, r, i) : 0.0f;
-    float top = 0.0f, top_q = 0.0f, log2_s = 0.0f, L = 0.0f;
+    float top = 0.0f, top_q = 0.0f, inv_s = 0.0f, L = 0.0f;
     const bool held = r.len <= G * NV * E;
     Pack<T, E> l[NV], q[NV];
     // f(j, l, q) for every pack of the row this lane has
@@ -356,7 +353,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
     if (PARTED && a.mode == 2) {
       const RowState* state = reinterpret_cast<const RowState*>(a.row_state) + i;
       live = state->live != 0.0f;
-      top = state->top, top_q = state->top_q, log2_s = state->log2_s, L = state->L;
+      top = state->top, top_q = state->top_q, inv_s = state->inv_s, L = state->L;
       v.dlogp = state->dlogp, v.kl = state->kl;
     } else if (live) {
       float m[REF ? 2 : 1];
@@ -401,7 +398,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
       }
       live = !(t[0] == 0.0f);
       if (live) {
-        log2_s = __builtin_amdgcn_logf(t[0]);
+        inv_s = 1.0f / t[0];
         float kl = 0.0f;
         if (REF) {
           const float eta = (t[0] - t[REF ? 1 : 0]) / t[0];
@@ -434,13 +431,12 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 
       const float uw = up * w;
       if (live) {
         const float bw = REF ? uw * a.beta : 0.0f;
-        const float flat = -uw * v.dlogp - (bw != 0.0f ? bw * (L + v.kl) : 0.0f);    // p (bw x + flat)
-        auto prob = [&](float lx) __attribute__((always_inline)) {
-          return exp_less<FINE>(lx - top, log2_s);
-        };
+        // exp(l - m) (by_x x + flat), 1 / s in both
+        const float flat = (-uw * v.dlogp - (bw != 0.0f ? bw * (L + v.kl) : 0.0f)) * inv_s, by_x = bw * inv_s;
+        auto prob = [&](float lx) __attribute__((always_inline)) { return exp_of<FINE>(lx - top); };
         // x within what times 0 is 0: an entry of no probability has no gradient
         auto slope = [&](float lx, float qx) __attribute__((always_inline)) {
-          return REF ? fmaf(bw, fminf(fmaxf((lx - top) - (qx - top_q), -1e30f), 1e30f), flat) : flat;
+          return REF ? fmaf(by_x, fminf(fmaxf((lx - top) - (qx - top_q), -1e30f), 1e30f), flat) : flat;
         };
         visit([&](int j, const Pack<T, E>& x, const Pack<T, E>& y) __attribute__((always_inline)) {
           Pack<T, E> g = {};
@@ -524,7 +520,7 @@ __global__ __launch_bounds__(64) void k_policy_join(Policy a) {
       kl = (float)(eta < -1.0 ? d / s - L : f / s + (fabs(eta) < 1e-4 ? -eta * eta * (0.5 + eta / 3.0) : eta - L));
       kl = kl < 0.0f ? 0.0f : kl;
     }
-    state.log2_s = (float)log2(s);
+    state.inv_s = (float)(1.0 / s);
     v = row_loss<true>(a, i, (double)action_logit<T>(a, r, i) - top, s, kl);
     state.dlogp = v.dlogp, state.kl = v.kl, state.live = 1.0f;
   }

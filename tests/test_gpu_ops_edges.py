@@ -22,6 +22,26 @@ def even_rows(rows, width, dt=torch.float32):
             "adv": torch.ones(rows, device="cuda"), "weights": torch.ones(rows, device="cuda")}
 
 
+@pytest.mark.parametrize("widths", [range(2, 65), range(65, 257, 3), (300, 1000, 2049, 3000, 9001, 16383), (20001, 65537)],
+                         ids=lambda w: "%d-%d" % (w[0], w[-1]))
+def test_policy_gradient_of_even_rows(widths):
+    """dloss/dl_j = rho (1 / n - 1[j = a]).  rho is 64-bit (in 32 bits where a row has one wave: a logarithm of log n, an
+    exponential); it, 1 / n, their product and the result round once each."""
+    for n in widths:
+        a = even_rows(3, n)
+        l = a["logits"].requires_grad_()
+        grad = torch.autograd.grad(call_policy(a, (0.2, 0.2), 0.0, l).loss, l)[0].double()
+        rho = math.exp(-math.log(n) - float(a["old"][0].double()))
+        want = torch.full((3, n), rho / n, dtype=torch.float64, device="cuda")
+        tol = 4 * U * want
+        at = a["actions"][:, None]
+        want.scatter_add_(1, at, torch.full_like(want, -rho)[:, :1])
+        tol.scatter_(1, at, 6 * U * want.gather(1, at).abs())
+        if 64 < n <= 1024:
+            tol += want.abs() * (4 * math.log(n) + 4) * U
+        within(grad, want, tol, "width %d" % n)
+
+
 @pytest.mark.parametrize("rows,width,dtype", [(512, 50, "fp32"), (256, 4000, "fp32"), (512, 50001, "bf16"), (128, 20001, "bf16"), (4, 20001, "fp32")])
 def test_policy_loss_that_cancels(rows, width, dtype):
     """A signed mean a thousand times smaller than its terms, and more, keeps its digits: rows' values and their sum are 64-bit (1e-13 of
