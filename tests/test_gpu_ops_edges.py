@@ -128,6 +128,24 @@ def test_policy_gradient_belongs_to_its_pass():
     assert torch.equal(again, want(1.0))
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 64), (3, 200), (3, 1000), (3, 4000), (3, 9001), (130, 16500), (130, 17001), (130, 19999), (3, 20001)], ids=str)
+def test_policy_kl_of_a_sure_reference(shape, dtype):
+    """An even policy, a reference with all but e^-18 of the weight on one entry.  The policy's sum is exact; of the two
+    others' terms a lane has at most 20 (of 16-bit types 40), then 6 shuffles and 16 waves: so many half steps of 17,
+    a few of 18, and those of the logarithm of the sums' ratio, 4 of each of its units."""
+    rows, n = shape
+    l, r = torch.full(shape, 0.75, device="cuda"), torch.zeros(shape, device="cuda")
+    at = torch.arange(rows, device="cuda") * 31 % n
+    r.scatter_(1, at[:, None], 18.0)
+    zero = torch.zeros(rows, device="cuda")
+    got = ops.policy_loss(l.to(DT[dtype]), at, zero, zero, ref_logits=r.to(DT[dtype]))
+    lp, lq = torch.log_softmax(l.double(), 1), torch.log_softmax(r.double(), 1)
+    terms = (20 if dtype == "fp32" else 40) + 22
+    tol = U * (17 * (terms + 2) + 3 * 18 + 4 * math.log(n) + 10)
+    within(got.kl, (lp.exp() * (lp - lq)).sum(1), torch.full((rows,), tol), "kl")
+
+
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("dense", [(5, 12), (5, 200), (4, 1500), (3, 9001), (3, 20001)], ids=str)
 def test_policy_kl_watched_only(dense, dtype):
