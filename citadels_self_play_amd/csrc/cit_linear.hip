@@ -63,7 +63,7 @@ __device__ __forceinline__ float act_fwd(int act, float z) {
 }
 template <typename T>
 __device__ __forceinline__ float act_grad(int act, float z) {
-  if (act == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if (act == ACT_RELU) return z <= 0.0f ? 0.0f : 1.0f;              // NaN lets dy through: no 0 hides it
   if (act == ACT_GELU) {
     float cdf, e;
     normal_cdf<T>(z, cdf, e);

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from citadels_self_play_amd import ops
-from test_gpu_ops import DT, U, call_policy, policy_rows, policy_want, tiny, within
+from test_gpu_ops import DT, U, call_policy, linear_inputs, policy_rows, policy_want, rounded, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -166,6 +166,32 @@ def test_policy_kl_watched_only(dense, dtype):
         grad = torch.autograd.grad(got.loss, l, torch.tensor(up, device="cuda"), retain_graph=True)[0]
         v, t = want[3]
         within(grad, v * up, (t + U * v.abs()) * up + tiny(DT[dtype]), what="grad")
+
+
+# ---- linear ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("size", [(70, 96, 88), (2100, 131, 300)], ids=str)
+@pytest.mark.parametrize("res", [False, True])
+def test_linear_relu_passes_not_a_number_on(size, dtype, res):
+    """relu's gradient where the pre-activation is NaN is dy, as torch has it: a NaN does not hide in a 0."""
+    dt = DT[dtype]
+    x, w, b, r, dy = linear_inputs(*size, dt, "relu", True, res)
+    x[13, 5], x[29, 95] = math.nan, math.nan
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = ops.linear(x, w, b, residual=r, activation="relu")
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    z = x.detach().double() @ w.detach().double().t() + b.detach().double()
+    assert bool(z[[13, 29]].isnan().all()) and bool(y[[13, 29]].isnan().all())
+    dz = dy.double() * ~(z <= 0)
+    M, N = size[0], size[2]
+    # dz is dy or 0, exactly; the sums and their rounding
+    wd = w.detach().double()
+    want = dz @ wd
+    within(dx, want, rounded((N + 2) * U * (dz.abs() @ wd.abs()), want, dt), "dx")
+    want = dz.sum(0)
+    within(db, want, rounded((M + 2) * U * dz.abs().sum(0), want, dt), "db")
+    assert bool(dw[:, [5, 95]].isnan().any(0).all()) and not bool(dw[:, :5].isnan().any())
 
 
 # ---- gradient norm ------------------------------------------------------------------
