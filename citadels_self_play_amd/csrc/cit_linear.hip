@@ -565,8 +565,10 @@ __global__ __launch_bounds__(WM* WN * 64) void k_gemm_direct(Mat A, Mat B, Epilo
   __shared__ __attribute__((aligned(16))) char s0[BYTES], s1[BYTES], s2[STAGES > 2 ? BYTES : 16],
       s3[STAGES > 3 ? BYTES : 16];
 
+  const int block = (int)(blockIdx.z * gridDim.x + blockIdx.x), tiles = tiles_m * tiles_n;
+  if (block >= tiles) return;
   int tm, tn;
-  place(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
+  place(block, tiles, tiles_m, tiles_n, tm, tn);
   const int split = blockIdx.y, m0 = tm * BM, n0 = tn * BN;
   const int kb = split * k_per_split, ke = min(K, kb + k_per_split);
   const int whole = (ke - kb) / BK<T>;
@@ -1114,7 +1116,8 @@ bool forward_copies(int M, int N, int K, int es) {
 template <typename T, bool AKS, bool BKS, int TILE, int WM, int WN, int STAGES, bool AHEAD, int W = 16>
 void launch_direct(const Mat& A, const Mat& B, const Epilogue& e, int M, int N, int K, const Plan& p,
                    hipStream_t stream) {
-  hipLaunchKernelGGL((k_gemm_direct<T, AKS, BKS, TILE, TILE, WM, WN, STAGES, AHEAD, W>), dim3(p.tiles_m * p.tiles_n, p.splits),
+  const dim3 tiles = wide_grid((int64_t)p.tiles_m * p.tiles_n);
+  hipLaunchKernelGGL((k_gemm_direct<T, AKS, BKS, TILE, TILE, WM, WN, STAGES, AHEAD, W>), dim3(tiles.x, p.splits, tiles.y),
                      dim3(WM * WN * 64), 0, stream, A, B, e, M, N, K, p.tiles_m, p.tiles_n, p.k_per);
 }
 

@@ -194,6 +194,21 @@ def test_linear_relu_passes_not_a_number_on(size, dtype, res):
     assert bool(dw[:, [5, 95]].isnan().any(0).all()) and not bool(dw[:, :5].isnan().any())
 
 
+def test_linear_rows_past_a_grid_of_direct_loads():
+    """2^24 tiles of 256 threads are one grid dimension's most: fp32 over more rows than that takes."""
+    M, N = (1 << 30) + 1000, 33
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 4 * M * (N + 1) + (8 << 30):
+        pytest.skip("needs 154 GB of free memory on the GPU")
+    x, w = torch.empty(M, 1, device="cuda"), torch.randn(N, 1, device="cuda")
+    x.normal_()
+    y = ops.linear(x, w)
+    for at in (0, (1 << 27) - 3000, (1 << 29) + 77, (1 << 30) - 3000, M - 5000):
+        assert torch.equal(y[at:at + 5000], x[at:at + 5000] * w.t()), at   # one product each, rounded once
+    del x, y
+    torch.cuda.empty_cache()
+
+
 # ---- gradient norm ------------------------------------------------------------------
 
 def test_clip_of_tensors_that_hold_nothing():
