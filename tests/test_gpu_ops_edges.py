@@ -8,7 +8,8 @@ import pytest
 import torch
 
 from citadels_self_play_amd import ops
-from test_gpu_ops import DT, U, call_policy, linear_inputs, policy_rows, policy_want, rounded, tiny, within
+from test_gpu_ops import (DT, U, call_policy, linear_inputs, linear_want, policy_rows, policy_want, rounded, tiny,
+                          within)
 
 pytestmark = pytest.mark.gpu
 
@@ -207,6 +208,33 @@ def test_linear_rows_past_a_grid_of_direct_loads():
         assert torch.equal(y[at:at + 5000], x[at:at + 5000] * w.t()), at   # one product each, rounded once
     del x, y
     torch.cuda.empty_cache()
+
+
+def test_linear_gradient_is_the_slope():
+    """Along the gradient's own direction v (|v| = 1) the slope is the gradient's norm.  (F(+h) - F(-h)) / 2h differs
+    from it by h^2 / 6 sum |dy| |dz/ds|^3 0.8 (|gelu'''| < 0.78), by the values' rounding / h, and by that of the points."""
+    x, w, b, r, dy = linear_inputs(20, 30, 25, torch.float32, "gelu", True, True)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    grads = torch.autograd.grad(ops.linear(x, w, b, residual=r, activation="gelu"), leaves, dy)
+    h = 2.0 ** -4
+    d = dy.double()
+    for k, along in enumerate((lambda v: v @ w.detach().double().t(), lambda v: x.detach().double() @ v.t(), lambda v: v.expand(20, 25))):
+        slope = float(grads[k].double().norm())
+        v = grads[k].double() / slope
+        noise = 0.0
+
+        def at(s):
+            nonlocal noise
+            a = [(t.detach().double() + (s * h * v if i == k else 0)).float() for i, t in enumerate(leaves)]
+            noise += float((d.abs().cpu() * linear_want(*a, r, dy, "gelu")[0][1]).sum())
+            return float((ops.linear(*a, residual=r, activation="gelu").double() * d).sum())
+
+        got = (at(1) - at(-1)) / (2 * h)
+        third = 0.8 * float((d.abs() * along(v).abs() ** 3).sum()) * h * h / 6
+        points = float((grads[k].double().abs() * U * (leaves[k].detach().double().abs() + h * v.abs())).sum()) * 1.5 / h
+        tol = third + noise / (2 * h) + points
+        assert tol <= 0.02 * slope, (k, third, noise, slope)       # so that a wrong gradient fails
+        assert abs(got - slope) <= tol, (k, got, slope, third, noise)
 
 
 # ---- gradient norm ------------------------------------------------------------------
