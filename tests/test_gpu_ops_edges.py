@@ -244,3 +244,33 @@ def test_clip_of_tensors_that_hold_nothing():
         grads = [torch.empty((0, 3), device="cuda") for _ in range(n)]
         assert float(ops.grad_norm(grads)) == 0.0 and float(ops.clip_grad_norm(grads, 1.0)) == 0.0
         assert float(ops.clip_grad_norm(grads, 1.0, out=[t.clone() for t in grads])) == 0.0
+
+
+# ---- together ---------------------------------------------------------------------------
+
+def test_two_streams_with_every_workspace():
+    """Two layers on two streams at once, other inputs each, of sizes that take copies, dz, column sums and split sums:
+    each has what it has alone."""
+    inputs = [linear_inputs(16500, 131, 523, torch.bfloat16, "gelu", True, True, seed=s) for s in (1, 2)]
+    inputs += [linear_inputs(1000, 8201, 1100, torch.float32, "silu", True, False, seed=s) for s in (3, 4)]
+
+    def step(k):
+        x, w, b, r, dy = inputs[k]
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = ops.linear(*leaves, residual=r, activation="gelu" if k < 2 else "silu")
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+
+    want = []
+    for k in range(4):
+        want.append(step(k))
+        torch.cuda.synchronize()
+    assert not torch.equal(want[0][0], want[1][0])
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for pair in (0, 2):
+        for _ in range(3):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got.append((pair + i, step(pair + i)))
+    torch.cuda.synchronize()
+    for k, g in got:
+        assert all(torch.equal(p, q) for p, q in zip(g, want[k])), k
