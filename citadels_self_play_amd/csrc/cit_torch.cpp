@@ -114,6 +114,18 @@ void leaves_in_capture(const torch::autograd::Node& node, hipStream_t stream, co
   }
 }
 
+// torch.func's and vmap's tensors stand for others and have no memory; nor have batched gradients.
+void own_memory(std::initializer_list<Tensor> given, const char* what) {
+  for (const Tensor& t : given)
+    if (t.defined() && !t.has_storage())
+      throw py::value_error(std::string("ops.") + what + " takes no tensors of torch.func or vmap");
+}
+void one_gradient(const Tensor& t, const char* what) {
+  if (!t.has_storage())
+    throw std::runtime_error(std::string("ops.") + what +
+                             ": its backward pass takes one gradient, not a batch of them (is_grads_batched, vmap)");
+}
+
 void no_tangent(std::initializer_list<Tensor> given, const char* what) {
   for (const Tensor& t : given)
     if (t.defined() && t._fw_grad(0).defined())
@@ -141,6 +153,7 @@ struct LinearBackward : torch::autograd::Node {
     const Tensor& dy = grads[0];
     if (!dy.defined()) return out;
     first_only("linear");
+    one_gradient(dy, "linear");
     const On on(dy);
     leaves_in_capture(*this, on.stream, "linear");
     const bool nx = task_should_compute_output(0), nw = task_should_compute_output(1),
@@ -173,6 +186,7 @@ struct LinearBackward : torch::autograd::Node {
 
 Tensor linear(const Tensor& x, const Tensor& w, const Maybe& bias, const Maybe& residual, int act) {
   const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+  own_memory({x, w, b, r}, "linear");
   std::shared_ptr<LinearBackward> node;
   if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(b) || wanted(r))) {
     node = std::shared_ptr<LinearBackward>(new LinearBackward(), torch::autograd::deleteNode);
@@ -278,6 +292,7 @@ struct PolicyLossBackward : torch::autograd::Node {
     variable_list out(1);
     if (!grads[0].defined() || !task_should_compute_output(0)) return out;
     first_only("policy_loss");
+    one_gradient(grads[0], "policy_loss");
     Tensor v[8];
     for (int i = 0; i < 8; i++) v[i] = given[i].unpack();
     const On on(v[0]);
@@ -314,6 +329,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Maybe
                                                double beta) {
   const Tensor given[8] = {logits, ref.value_or(Tensor()), mask.value_or(Tensor()), offsets.value_or(Tensor()),
                            actions, old, adv, weights.value_or(Tensor())};
+  for (const Tensor& t : given) own_memory({t}, "policy_loss");
   std::shared_ptr<PolicyLossBackward> node;
   if (at::GradMode::is_enabled() && wanted(logits)) {
     node = std::shared_ptr<PolicyLossBackward>(new PolicyLossBackward(), torch::autograd::deleteNode);
@@ -362,7 +378,7 @@ std::vector<Tensor> listed(const py::list& from, const std::string& what) {
     out.push_back(THPVariable_Unpack(h.ptr()));
   }
   for (const Tensor& t : out) {
-    if (t.layout() != at::kStrided || t.is_neg()) throw py::value_error(what + " must be a dense tensor");
+    if (t.layout() != at::kStrided || t.is_neg() || !t.has_storage()) throw py::value_error(what + " must be a dense tensor");
     const at::ScalarType dt = t.scalar_type();
     if (dt != at::kFloat && dt != at::kBFloat16 && dt != at::kHalf)
       throw py::value_error(what + "s must be fp32, bf16 or fp16, not " +

@@ -14,7 +14,9 @@ backward pass too, while no eager graph of the same leaves is alive: torch's
 autograd engine would join the two graphs' streams; RuntimeError).  A backward
 pass captured apart from its forward pass needs retain_graph=True, and the
 forward pass's outputs alive as long as it is replayed.
-Wrong arguments raise ValueError before anything is launched.
+Wrong arguments raise ValueError before anything is launched, tensors of
+torch.func and vmap among them; a batch of gradients (is_grads_batched) raises
+RuntimeError.
 
 The checks are written out rather than shared: at a trainer's batch of 64 a
 call's time is the host's.  What follows them, autograd included, is

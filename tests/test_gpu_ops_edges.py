@@ -274,3 +274,29 @@ def test_two_streams_with_every_workspace():
     torch.cuda.synchronize()
     for k, g in got:
         assert all(torch.equal(p, q) for p, q in zip(g, want[k])), k
+
+
+def test_tensors_without_memory_are_refused():
+    """vmap's, torch.func's and batches of gradients: an error that says so, and the graph is as it was."""
+    x, w, b, r, dy = linear_inputs(37, 50, 41, torch.float32, "silu", True, True)
+    with pytest.raises(ValueError, match="torch.func or vmap"):
+        torch.vmap(lambda t: ops.linear(t, w))(x.view(37, 1, 50))
+    with pytest.raises(ValueError, match="torch.func or vmap"):
+        torch.func.grad(lambda t: ops.linear(x, t).sum())(w)
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    y = ops.linear(*leaves, activation="silu")
+    with pytest.raises(RuntimeError, match="not a batch"):
+        torch.autograd.grad(y, leaves, torch.stack([dy, dy]), is_grads_batched=True, retain_graph=True)
+    got = torch.autograd.grad(y, leaves, dy)
+    want = torch.autograd.grad(ops.linear(*leaves, activation="silu"), leaves, dy)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    a = policy_rows([4, 9, 30], torch.float32)
+    with pytest.raises(ValueError, match="torch.func or vmap"):
+        torch.func.grad(lambda t: call_policy(a, (0.2, 0.2), 0.1, t).loss)(a["logits"])
+    l = a["logits"].requires_grad_()
+    loss = call_policy(a, (0.2, 0.2), 0.1, l).loss
+    with pytest.raises(RuntimeError, match="not a batch"):
+        torch.autograd.grad(loss, l, torch.ones(3, device="cuda"), is_grads_batched=True, retain_graph=True)
+    assert torch.equal(torch.autograd.grad(loss, l)[0], torch.autograd.grad(call_policy(a, (0.2, 0.2), 0.1, l).loss, l)[0])
+    with pytest.raises(ValueError, match="dense tensor"):
+        torch.vmap(lambda t: ops.clip_grad_norm([t], 1.0))(w.detach())

@@ -7,6 +7,8 @@ import sys
 import pytest
 import torch
 
+from citadels_self_play_amd import ops
+
 CLIP_EMPTY = """
 import ctypes as C
 from citadels_self_play_amd import _lib
@@ -26,3 +28,9 @@ def test_clip_of_tensors_that_hold_nothing_ends():
     """Every tensor of the list empty: on to the launch, which has no device here."""
     subprocess.run([sys.executable, "-c", CLIP_EMPTY], check=True, timeout=60,
                    cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
+def test_clip_refuses_tensors_without_memory():
+    """What vmap hands a function stands for a batch of tensors."""
+    with pytest.raises(ValueError, match="a gradient must be a dense tensor"):
+        torch.vmap(lambda t: ops.clip_grad_norm([t], 1.0))(torch.ones(3, 4))
