@@ -31,7 +31,8 @@ from . import _lib
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
-_MOST, _LONGEST = 2 ** 31 - 1024, 2 ** 30       # a matrix's sides; a row's entries (the kernels' indexes are 32 bits)
+# a matrix's sides; a row's entries; rows (the kernels' indexes are 32 bits)
+_MOST, _LONGEST, _ROWS = 2 ** 31 - 1024, 2 ** 30, 2 ** 30 - 1
 _NORM, _CHECK, _CLIP = 0, 1, 2                  # cit_torch.cpp's clip_grad_norm
 _calls = _lib.torch_calls
 
@@ -157,6 +158,8 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logits=None, offse
     if actions.dim() != 1 or actions.dtype not in (torch.int64, torch.int32):
         raise ValueError("actions must be [N] whole numbers")
     N = actions.shape[0]
+    if N > _ROWS:
+        raise ValueError("over %d positions" % _ROWS)
     if offsets is None:
         if shape[0] != N:
             raise ValueError("%d rows of logits, %d actions" % (shape[0], N))

@@ -34,3 +34,12 @@ def test_clip_refuses_tensors_without_memory():
     """What vmap hands a function stands for a batch of tensors."""
     with pytest.raises(ValueError, match="a gradient must be a dense tensor"):
         torch.vmap(lambda t: ops.clip_grad_norm([t], 1.0))(torch.ones(3, 4))
+
+
+def test_policy_refuses_more_rows_than_it_counts():
+    n = 1 << 30
+    one = torch.zeros(1)
+    with pytest.raises(ValueError, match="over 1073741823 positions"):
+        ops.policy_loss(one.view(1, 1).expand(n, 1), one.long().expand(n), one.expand(n), one.expand(n))
+    with pytest.raises(ValueError, match="over 1073741823 positions"):
+        ops.policy_loss(one, one.long().expand(n), one.expand(n), one.expand(n), offsets=one.long().expand(n + 1))
