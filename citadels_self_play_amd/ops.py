@@ -64,8 +64,9 @@ def linear(x, weight, bias=None, residual=None, activation="none"):
     all of one type; activation "none", "relu", "gelu" (by erf) or "silu".
     Sums are fp32.  Differentiable in every tensor; under no_grad nothing is
     kept; there are no second derivatives (create_graph=True raises RuntimeError).
-    The gradient of the pre-activation is rounded to the type before the
-    two products that use it (bias gradients are summed before that)."""
+    For the backward pass the pre-activation is kept in the type, and its
+    gradient is rounded to it before the two products that use it (bias gradients
+    are summed before that); relu passes the gradient on where it is NaN."""
     _same_place(x if isinstance(x, torch.Tensor) else torch.empty(0), x=x, weight=weight, bias=bias, residual=residual)
     dt, shape, ws = x.dtype, x.shape, weight.shape
     if dt not in TYPES:
@@ -126,6 +127,8 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logits=None, offse
     list whose entries offsets[i] .. offsets[i + 1] - 1 are position i's options
     (engine.GameBatch.cfr_targets' option rows).  mask (bool, as logits): the
     legal entries.  actions [N]: the chosen entry, counted from the row's first.
+    Lists are for rows of like lengths: the lanes that share a row go by twice
+    the mean length, and one that is far longer takes its time in proportion.
     Over a row's legal entries, with rho = exp(logp[action] - old_logp),
 
         loss = sum_i weights_i (-min(rho A, clip(rho, 1 - low, 1 + high) A) + kl_coef KL(p || p_ref))
