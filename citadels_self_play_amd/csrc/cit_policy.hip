@@ -277,8 +277,8 @@ __device__ __forceinline__ float exp_of(float x) {
 //
 // bf16 with a reference is bound by the vector units (52 instructions an entry,
 // three of them exponentials at a quarter of the rate), the others by memory.
-// 4096 x 32,768 bf16, gradient included: 250 us, 3.2 TB/s, the vector units at
-// work for 190 of them; without a reference 126 us, 4.3 TB/s; 509 x 50,001 masked,
+// 4096 x 32,768 bf16, gradient included: 236 us, 3.4 TB/s, the vector units at
+// work for 190 of them; without a reference 120 us, 4.5 TB/s; 509 x 50,001 masked,
 // evaluated only, 23 us, 3.3 TB/s.
 template <typename T, int G, int NV, int E, bool REF, bool PARTED>
 __global__ __launch_bounds__(G > 256 ? G : 256, G == 1024 && !REF ? 8 : G > 256 ? 4 : E > 1 && REF && !PARTED ? 5 : 2) void k_policy(Policy a, int64_t row_blocks, int tail) {
