@@ -300,3 +300,31 @@ def test_tensors_without_memory_are_refused():
     assert torch.equal(torch.autograd.grad(loss, l)[0], torch.autograd.grad(call_policy(a, (0.2, 0.2), 0.1, l).loss, l)[0])
     with pytest.raises(ValueError, match="dense tensor"):
         torch.vmap(lambda t: ops.clip_grad_norm([t], 1.0))(w.detach())
+
+
+def test_graphed_callable():
+    """torch's own graphs of a module: the forward pass in one, the backward pass in another, each replayed with new inputs
+    and upstream gradients.  (A warm-up's graph would be alive beside the capture.)"""
+    a = policy_rows([4, 9, 30, 64], torch.float32)
+    x, w, b, _, _ = linear_inputs(107, 50, 40, torch.float32, "gelu", True, False)
+
+    class Step(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w1, self.b1 = torch.nn.Parameter(w.clone()), torch.nn.Parameter(b.clone())
+            self.w2 = torch.nn.Parameter(w[:1, :40].clone())
+
+        def forward(self, x):
+            logits = ops.linear(ops.linear(x, self.w1, self.b1, activation="gelu"), self.w2)[:, 0]
+            return call_policy(a, (0.2, 0.2), 0.1, logits).loss
+
+    plain, graphed = Step(), torch.cuda.make_graphed_callables(Step(), (x.clone(),), num_warmup_iters=0)
+    for k in range(4):
+        x = x * 0.9
+        loss, want = graphed(x), plain(x)
+        assert torch.equal(loss, want)
+        up = torch.tensor((1.0, 0.5, -2.0, 1.0)[k], device="cuda")
+        got = torch.autograd.grad(loss, list(graphed.parameters()), up)
+        want = torch.autograd.grad(want, list(plain.parameters()), up)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), k
