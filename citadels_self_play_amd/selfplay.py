@@ -117,6 +117,22 @@ POOL_FRAC = float(os.environ.get("CIT_POOL_FRAC", "0.8"))
 QUEUE_SLICE_S = float(os.environ.get("CIT_QUEUE_SLICE_S", "0.5"))
 
 
+_budgets = {}                           # per device: the last pool_budget
+
+
+def pool_budget(avail, device="cuda"):
+    """Bytes that node pools may take by default, of `avail`: POOL_FRAC of them, or what
+    the last search was given where that is within 2 %.  What the driver counts as free
+    differs by up to 0.5 GB from one search to the next, and an arena asked for a
+    little larger than the cached one is a fresh hipMalloc of all of it (246 GB: 7 s;
+    config 5's one batch 99 trees/s, 154 without it)."""
+    b, last = int(POOL_FRAC * avail), _budgets.get(str(device))
+    if last is not None and abs(b - last) <= last // 50:
+        return last
+    _budgets[str(device)] = b
+    return b
+
+
 def arena_frac_for(B, node_cap):
     from . import layout as L
     return ARENA_FRAC if B >= ARENA_MIN_TREES and L.cfr_nblocks(node_cap) >= ARENA_MIN_BLOCKS else None
@@ -135,7 +151,7 @@ def simulate_games(seeds, iters, max_move=100, node_cap=None, device=None, edge_
     summed worst case (default ARENA_FRAC: ~1.3x the measured mean; a tree
     that finds the arena exhausted is searched again, bit-identically, in a
     batch of its own).  When the seeds' pools do not fit in `max_pool_bytes`
-    (default: 80 % of the device memory not held by live tensors) they go
+    (default: pool_budget of the device memory not held by live tensors) they go
     through a tree queue over as many lanes as fit (simulate_queue; with
     queue=False: consecutive equal chunks, the returned batch then being the
     last chunk's); results are concatenated in seed order either way.
@@ -152,7 +168,7 @@ def simulate_games(seeds, iters, max_move=100, node_cap=None, device=None, edge_
     dev = torch.device(device or "cuda")
     if max_pool_bytes is None:
         from .engine import device_avail_bytes   # (cached blocks of earlier pools count as free)
-        max_pool_bytes = int(POOL_FRAC * device_avail_bytes(dev))
+        max_pool_bytes = pool_budget(device_avail_bytes(dev), dev)
     seeds = np.asarray(seeds, np.int64)
     frac = (lambda B: arena_frac_for(B, node_cap)) if arena_frac == "auto" else (lambda B: arena_frac)
     chunk = len(seeds)
@@ -339,7 +355,7 @@ class TreeQueue:
         self.t_setup = time.perf_counter()
         if max_pool_bytes is None:
             from .engine import device_avail_bytes
-            max_pool_bytes = int(POOL_FRAC * device_avail_bytes(dev))
+            max_pool_bytes = pool_budget(device_avail_bytes(dev), dev)
         frac = (lambda B: arena_frac_for(B, node_cap)) if arena_frac == "auto" else (lambda B: arena_frac)
         Q = max(1, int(per_round))
         if slots and multi_round:
