@@ -259,6 +259,7 @@ template <bool FINE>
 __device__ __forceinline__ float exp_of(float x) {
   return FINE ? expf(x) : __builtin_amdgcn_exp2f(x * LOG2E);
 }
+
 // A row by G lanes, each with up to NV packs of E entries in registers, so that
 // the logits come from memory once; a longer row is read again in each pass.
 //
