@@ -13,7 +13,9 @@ allocator and waits for nothing.  Calls can be captured into a HIP graph (a
 backward pass too, while no eager graph of the same leaves is alive: torch's
 autograd engine would join the two graphs' streams; RuntimeError).  A backward
 pass captured apart from its forward pass needs retain_graph=True, and the
-forward pass's outputs alive as long as it is replayed.
+forward pass's outputs alive as long as it is replayed.  (torch.cuda.
+make_graphed_callables: with num_warmup_iters=0, since a warm-up's graph stays
+alive beside its captures.)
 Wrong arguments raise ValueError before anything is launched, tensors of
 torch.func and vmap among them; a batch of gradients (is_grads_batched) raises
 RuntimeError.
